@@ -252,6 +252,45 @@ hipError_t sample_token(hipStream_t stream, const float* logits, const float* bo
                         const float* penalty, const float* inverse_penalty, uint8_t* seen, const int64_t* top_k,
                         const float* uniform, int64_t* token, int64_t* history, int vocab);
 
+/* ------------------------------------------------- 4-bit cache and attention
+ * The reference keeps keys and values in fp16 (kv_write_tile, ternary.cu:904-933) and reads them in
+ * attention_step and attention_tile (ternary.cu:509-611, :935-982); these entry points are this library's own.
+ *
+ * pages: [page_count, kv_heads, page_tiles, 34 * head_dim] bytes, 16-byte aligned; page_tiles (tiles of 32 tokens
+ * per page) a power of two; head_dim 64, 128 or 256.  A value is 4-bit floating point (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives); 32 neighbouring values of a row share a power-of-two scale byte.  table: [sequences, table_width]
+ * page numbers, at most 2^30 tokens per sequence; an entry outside 0 .. page_count - 1 is no page: nothing is written
+ * there, 0 is read, and attention does not see its tokens.  offsets: [sequences + 1] rows before each sequence, not
+ * decreasing, or NULL for one row per sequence (rows == sequences).  dtype: 0 fp32, 1 fp16, 2 bfloat16.  Strides are
+ * in elements; a head's dims lie side by side.  All index arrays are int32 on the device and are not read by the host.
+ *
+ * ivonar_cache_write: row r of sequence b becomes position past[b] + r - offsets[b]; a negative past[b] writes
+ * nothing.  A block of 32 values with a NaN or an infinity reads back as NaN. */
+hipError_t ivonar_cache_write(hipStream_t stream, const void* k, const void* v, int dtype, long long k_token_stride,
+                              long long k_head_stride, long long v_token_stride, long long v_head_stride, int rows,
+                              uint8_t* pages, int page_count, int kv_heads, int page_tiles, int head_dim,
+                              const int32_t* table, int table_width, const int32_t* past, const int32_t* offsets,
+                              int sequences);
+/* k and v [rows, kv_heads, head_dim], 16-byte aligned: row r of sequence b is position start[b] + r - offsets[b]
+ * (start NULL: 0).  Rows of no sequence and positions without a page are 0. */
+hipError_t ivonar_cache_read(hipStream_t stream, const uint8_t* pages, int page_count, int kv_heads, int page_tiles,
+                             int head_dim, const int32_t* table, int table_width, const int32_t* start,
+                             const int32_t* offsets, int sequences, int rows, int dtype, void* k, void* v);
+/* out [rows, heads, head_dim] = attention of q's rows over the cached keys and values; heads a multiple of kv_heads
+ * (head h reads key/value head h / (heads / kv_heads)).  The rows of sequence b are its last ones: row r is position
+ * lengths[b] - (offsets[b + 1] - offsets[b]) + r - offsets[b] and sees the positions up to its own, with a window
+ * (0: none) only the last `window` of them and the first `sinks` of the sequence.  A row that sees nothing is 0, and
+ * so are rows of no sequence.  scale > 0 multiplies q . k.  max_length: about the longest length; it sets how the keys
+ * are shared between blocks, not the result's validity.  work: ivonar_cache_attention_work bytes (same arguments; the
+ * sizes alone decide, offsets is only tested for NULL; -1 for sizes that the call refuses), 16-byte aligned. */
+long long ivonar_cache_attention_work(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
+                                      int sequences, int rows, int window, int sinks, int max_length);
+hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, long long q_token_stride,
+                                  long long q_head_stride, int heads, int rows, const uint8_t* pages, int page_count,
+                                  int kv_heads, int page_tiles, int head_dim, const int32_t* table, int table_width,
+                                  const int32_t* lengths, const int32_t* offsets, int sequences, int window, int sinks,
+                                  float scale, int max_length, void* out, void* work, long long work_bytes);
+
 /* ------------------------------------------------------ checkpoint checks
  * The packed-buffer tests of the reference loader (loader.py:94-112), on the
  * device: ORs into flags[0] bit 0 when a byte of packed[0..packed_bytes)

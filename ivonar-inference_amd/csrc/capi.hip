@@ -1,5 +1,6 @@
 // C-ABI entry points (declared in include/ivonar_ternary.h): argument checks,
 // process defines, the per-device and per-stream scratch, and dispatch to the launchers.
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -8,6 +9,7 @@
 #include <utility>
 
 #include "ivonar_ternary.h"
+#include "cache_layout.hpp"
 #include "internal.hpp"
 #include "ternary_device.hpp"
 
@@ -476,6 +478,108 @@ hipError_t ivonar_linear(hipStream_t stream, const void* input, int dtype, int m
                     m, q8 + used, work_bytes - used);
 }
 int ivonar_linear_half(int n, const void* input) { return n > 0 && quantize_half_applies(n, input) ? 1 : 0; }
+
+// The page geometry of a 4-bit cache: `tiles` per page a power of two, at most 2^30 tokens per sequence.
+static bool cache_geometry(const uint8_t* pages, int page_count, int kv_heads, int page_tiles, int head_dim,
+                           const int32_t* table, int table_width, int sequences, int rows, int* shift) {
+  if (pages == nullptr || (table == nullptr && sequences > 0) || !aligned16(pages) || !cache_head_dim(head_dim)) return false;
+  if (page_count <= 0 || kv_heads <= 0 || kv_heads > 65535 || page_tiles <= 0 || (page_tiles & (page_tiles - 1)) != 0)
+    return false;
+  if (table_width <= 0 || sequences < 0 || rows < 0) return false;
+  if ((long long)table_width * page_tiles * kCacheTile > (1LL << 30)) return false;
+  *shift = __builtin_ctz((unsigned)page_tiles);
+  return true;
+}
+
+hipError_t ivonar_cache_write(hipStream_t stream, const void* k, const void* v, int dtype, long long k_token_stride,
+                              long long k_head_stride, long long v_token_stride, long long v_head_stride, int rows,
+                              uint8_t* pages, int page_count, int kv_heads, int page_tiles, int head_dim,
+                              const int32_t* table, int table_width, const int32_t* past, const int32_t* offsets,
+                              int sequences) {
+  int shift = 0;
+  if (!cache_geometry(pages, page_count, kv_heads, page_tiles, head_dim, table, table_width, sequences, rows, &shift))
+    return hipErrorInvalidValue;
+  if (k == nullptr || v == nullptr || (past == nullptr && sequences > 0) || dtype < kFloat32 || dtype > kBfloat16)
+    return hipErrorInvalidValue;
+  if (offsets == nullptr && rows != sequences) return hipErrorInvalidValue;
+  const CacheArgs a{pages, table, past, offsets, page_count, shift, kv_heads, table_width, sequences, rows};
+  return launch_cache_write(stream, a, head_dim, dtype, k, v, RowStrides{k_token_stride, k_head_stride},
+                            RowStrides{v_token_stride, v_head_stride});
+}
+
+hipError_t ivonar_cache_read(hipStream_t stream, const uint8_t* pages, int page_count, int kv_heads, int page_tiles,
+                             int head_dim, const int32_t* table, int table_width, const int32_t* start,
+                             const int32_t* offsets, int sequences, int rows, int dtype, void* k, void* v) {
+  int shift = 0;
+  if (!cache_geometry(pages, page_count, kv_heads, page_tiles, head_dim, table, table_width, sequences, rows, &shift))
+    return hipErrorInvalidValue;
+  if (k == nullptr || v == nullptr || !aligned16(k) || !aligned16(v) || dtype < kFloat32 || dtype > kBfloat16)
+    return hipErrorInvalidValue;
+  if (offsets == nullptr && rows != sequences) return hipErrorInvalidValue;
+  const CacheArgs a{const_cast<uint8_t*>(pages), table, start,       offsets,   page_count,
+                    shift,                       kv_heads, table_width, sequences, rows};
+  return launch_cache_read(stream, a, head_dim, dtype, k, v);
+}
+
+static bool attention_sizes(int dtype, int heads, int kv_heads, int head_dim, int sequences, int rows, int window,
+                            int sinks, float scale) {
+  return dtype >= kFloat32 && dtype <= kBfloat16 && kv_heads > 0 && kv_heads <= 65535 && heads > 0 &&
+         heads % kv_heads == 0 && cache_head_dim(head_dim) && sequences >= 0 && rows >= 0 &&
+         (long long)rows * (heads / kv_heads) <= (1LL << 30) && window >= 0 && sinks >= 0 && scale > 0.0f &&
+         scale < INFINITY;
+}
+
+static CacheAttentionArgs cache_attention_sizes(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
+                                                int sequences, int rows, int window, int sinks, int max_length) {
+  CacheAttentionArgs a{};
+  a.offsets = offsets;
+  a.dtype = dtype;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.sequences = sequences;
+  a.rows = rows;
+  a.window = window < (1 << 30) ? window : (1 << 30);
+  a.sinks = sinks;
+  a.max_length = max_length > 0 ? max_length : 0;
+  return a;
+}
+
+long long ivonar_cache_attention_work(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
+                                      int sequences, int rows, int window, int sinks, int max_length) {
+  if (!attention_sizes(dtype, heads, kv_heads, head_dim, sequences, rows, window, sinks, 1.0f)) return -1;
+  return cache_attention_work(cache_attention_sizes(dtype, heads, kv_heads, head_dim, offsets, sequences, rows, window,
+                                                    sinks, max_length));
+}
+
+hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, long long q_token_stride,
+                                  long long q_head_stride, int heads, int rows, const uint8_t* pages, int page_count,
+                                  int kv_heads, int page_tiles, int head_dim, const int32_t* table, int table_width,
+                                  const int32_t* lengths, const int32_t* offsets, int sequences, int window, int sinks,
+                                  float scale, int max_length, void* out, void* work, long long work_bytes) {
+  int shift = 0;
+  if (!attention_sizes(dtype, heads, kv_heads, head_dim, sequences, rows, window, sinks, scale) ||
+      !cache_geometry(pages, page_count, kv_heads, page_tiles, head_dim, table, table_width, sequences, rows, &shift))
+    return hipErrorInvalidValue;
+  if (q == nullptr || out == nullptr || (lengths == nullptr && sequences > 0) || !aligned16(out)) return hipErrorInvalidValue;
+  if (offsets == nullptr && rows != sequences) return hipErrorInvalidValue;
+  CacheAttentionArgs a = cache_attention_sizes(dtype, heads, kv_heads, head_dim, offsets, sequences, rows, window,
+                                               sinks, max_length);
+  const long long need = cache_attention_work(a);
+  if (need > 0 && (work == nullptr || !aligned16(work) || work_bytes < need)) return hipErrorInvalidValue;
+  a.q = q;
+  a.q_strides = RowStrides{q_token_stride, q_head_stride};
+  a.pages = pages;
+  a.table = table;
+  a.lengths = lengths;
+  a.out = out;
+  a.work = static_cast<float*>(work);
+  a.page_count = page_count;
+  a.page_shift = shift;
+  a.table_width = table_width;
+  a.scale = scale;
+  return launch_cache_attention(stream, a);
+}
 
 hipError_t embed_token(hipStream_t stream, const int64_t* token, const uint8_t* packed, const uint16_t* scales,
                        float* output, int n, int row_bytes, int groups) {

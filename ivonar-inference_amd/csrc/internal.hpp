@@ -205,4 +205,75 @@ hipError_t launch_stream_read(hipStream_t stream, const void* data, long long by
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// Rows of a 4-bit cache (cache_layout.hpp): `rows` rows of ragged sequences, written or read from position start[b].
+struct CacheArgs {
+  uint8_t* pages;
+  const int* table;    // [sequences, table_width] page numbers
+  const int* start;    // [sequences]; null: 0
+  const int* offsets;  // [sequences + 1] rows before each sequence; null: one row each
+  int page_count;
+  int page_shift;  // log2 of the tiles per page
+  int kv_heads;
+  int table_width;
+  int sequences;
+  int rows;
+};
+// Elements between neighbouring tokens and neighbouring heads.
+struct RowStrides {
+  long long token;
+  long long head;
+};
+hipError_t launch_cache_write(hipStream_t stream, const CacheArgs& a, int head_dim, int dtype, const void* k,
+                              const void* v, RowStrides ks, RowStrides vs);
+hipError_t launch_cache_read(hipStream_t stream, const CacheArgs& a, int head_dim, int dtype, void* k, void* v);
+
+// Attention of q's rows over the 4-bit cache.
+struct CacheAttentionArgs {
+  const void* q;
+  RowStrides q_strides;
+  const uint8_t* pages;
+  const int* table;
+  const int* lengths;  // [sequences] tokens of each sequence, the query rows' own among them
+  const int* offsets;  // [sequences + 1] query rows before each sequence; null: one row each
+  void* out;           // [rows, heads, head_dim]
+  float* work;
+  int dtype;
+  int heads;
+  int kv_heads;
+  int head_dim;
+  int page_count;
+  int page_shift;
+  int table_width;
+  int sequences;
+  int rows;
+  int window;  // 0: no window
+  int sinks;
+  int max_length;
+  float scale;
+};
+long long cache_attention_work(const CacheAttentionArgs& a);
+hipError_t launch_cache_attention(hipStream_t stream, const CacheAttentionArgs& a);
+
+// Causal attention within packed prompts.
+struct WindowAttentionArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  RowStrides q_strides;
+  RowStrides k_strides;
+  RowStrides v_strides;
+  const int* offsets;  // [sequences + 1] rows before each sequence; null: one sequence of all rows
+  void* out;           // [rows, heads, head_dim]
+  int dtype;           // kFloat16 or kBfloat16
+  int heads;
+  int kv_heads;
+  int head_dim;
+  int sequences;
+  int rows;
+  int window;
+  int sinks;
+  float scale;
+};
+hipError_t launch_window_attention(hipStream_t stream, const WindowAttentionArgs& a);
+
 }  // namespace ivo

@@ -73,6 +73,10 @@ SIGNATURES: dict[str, list] = {
     "logit_bounds": [_P, _P, _P, _P, _P, _P, _I],
     "sample_token": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I],
     "ivonar_stream_read": [_P, ctypes.c_longlong, _P],
+    "ivonar_cache_write": [_P, _P, _I, _L, _L, _L, _L, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _I],
+    "ivonar_cache_read": [_P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _P, _P],
+    "ivonar_cache_attention": [_P, _I, _L, _L, _I, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _F, _I, _P, _P,
+                               _L],
     "ivonar_validate_ternary": [_P, ctypes.c_longlong, _P, ctypes.c_longlong, _P],
 }
 
@@ -118,6 +122,8 @@ def library() -> ctypes.CDLL:
             lib.ivonar_linear_work.restype = c_longlong
             lib.ivonar_linear_half.argtypes = [c_int, c_void_p]
             lib.ivonar_linear_half.restype = c_int
+            lib.ivonar_cache_attention_work.argtypes = [c_int, c_int, c_int, c_int, c_void_p, *[c_int] * 5]
+            lib.ivonar_cache_attention_work.restype = c_longlong
             lib.ivonar_token_finish_limit.argtypes = [c_int]
             lib.ivonar_token_finish_limit.restype = c_int
             for name, argtypes in SIGNATURES.items():
