@@ -333,7 +333,9 @@ __global__ __launch_bounds__(kThreads) void cache_attention_kernel(Params p) {
     if (__ballot(grows) != 0ull) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float raised = fmaxf(m[rt], lane_groups_max(most[rt]));
+        // Only the rows that grow: a row's rounding does not depend on its neighbours.
+        const float highest = lane_groups_max(most[rt]);
+        const float raised = highest > m[rt] + kGrowth ? highest : m[rt];
         const float factor = __builtin_amdgcn_exp2f(m[rt] - raised);
         m[rt] = raised;
         l[rt] *= factor;

@@ -581,6 +581,44 @@ hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, 
   return launch_cache_attention(stream, a);
 }
 
+hipError_t ivonar_window_attention(hipStream_t stream, const void* q, const void* k, const void* v, int dtype,
+                                   long long q_token_stride, long long q_head_stride, long long k_token_stride,
+                                   long long k_head_stride, long long v_token_stride, long long v_head_stride,
+                                   int heads, int kv_heads, int head_dim, int rows, const int32_t* offsets,
+                                   int sequences, int window, int sinks, float scale, void* out) {
+  if (dtype == kFloat32 ||
+      !attention_sizes(dtype, heads, kv_heads, head_dim, sequences, rows, window, sinks, scale))
+    return hipErrorInvalidValue;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || !aligned16(out)) return hipErrorInvalidValue;
+  if (offsets == nullptr && sequences != 1) return hipErrorInvalidValue;
+  // Rows are read 16 bytes at a time, a tile's from a buffer of less than 2 GiB.
+  const long long strides[] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+                               v_head_stride};
+  for (long long stride : strides)
+    if ((stride & 7) != 0) return hipErrorInvalidValue;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return hipErrorInvalidValue;
+  if (k_token_stride < 0 || k_token_stride >= 1 << 23 || v_token_stride < 0 || v_token_stride >= 1 << 23)
+    return hipErrorInvalidValue;
+  const WindowAttentionArgs a{q,
+                              k,
+                              v,
+                              RowStrides{q_token_stride, q_head_stride},
+                              RowStrides{k_token_stride, k_head_stride},
+                              RowStrides{v_token_stride, v_head_stride},
+                              offsets,
+                              out,
+                              dtype,
+                              heads,
+                              kv_heads,
+                              head_dim,
+                              sequences,
+                              rows,
+                              window < (1 << 30) ? window : (1 << 30),
+                              sinks,
+                              scale};
+  return launch_window_attention(stream, a);
+}
+
 hipError_t embed_token(hipStream_t stream, const int64_t* token, const uint8_t* packed, const uint16_t* scales,
                        float* output, int n, int row_bytes, int groups) {
   if (token == nullptr || packed == nullptr || scales == nullptr || output == nullptr || n <= 0 ||

@@ -9,7 +9,9 @@ The reference keeps fp16 keys and values and attends to them in ``attention_step
 * ``cache_read(pages, table, start, offsets, rows, dtype)`` -> (k, v): stretches of the sequences as tensors;
 * ``cache_attention(q, pages, table, lengths, offsets, window, sinks)``: the last rows of each sequence (one token
   while decoding, several for a chunk of a prompt) over all of its cached tokens, or over a sliding window and the
-  first few (sinks).
+  first few (sinks);
+* ``window_attention(q, k, v, offsets, window, sinks)``: causal attention within packed prompts over their fp16 or
+  bfloat16 keys and values as they are.
 
 A cached value is a 4-bit floating-point number (0, 0.5, 1, 1.5, 2, 3, 4, 6 or a negative of them) times a power of two
 that 32 neighbouring values of a head's row share: 4.25 bits per value.  A block of 32 that holds a NaN or an
@@ -187,4 +189,49 @@ def cache_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, of
     _call("ivonar_cache_attention", device, q.data_ptr(), dtype, q.stride(0), q.stride(1), heads, rows,
           pages.data_ptr(), count, kv_heads, tiles, dim, table.data_ptr(), table.shape[1], lengths.data_ptr(), address,
           sequences, window, sinks, scale, longest, out.data_ptr(), _address(work), max(need, 0))
+    return out
+
+
+def _by_sixteen_bytes(x: Tensor) -> Tensor:
+    """x with rows that start on 16 bytes, after a copy where they do not (or lie further apart than a call takes)."""
+    if x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.stride(0) < 1 << 23:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def window_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor | None = None, window: int = 0, sinks: int = 0,
+                     scale: float | None = None, out: Tensor | None = None) -> Tensor:
+    """Causal attention within packed sequences: q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim], all
+    fp16 or all bfloat16, in that type.
+
+    offsets (int32 [sequences + 1]): the rows before each sequence; None: all rows are one sequence.  A row sees its
+    sequence's rows up to its own, and with a window (0: none) only the last `window` of them and the first `sinks`
+    of the sequence.  heads is a multiple of kv_heads.  scale (default head_dim ** -0.5) multiplies q . k.  Rows that
+    do not start on 16 bytes are copied first."""
+    device = _require_device(q, k, v, offsets)
+    dim = q.shape[-1]
+    if dim not in HEAD_DIMS:
+        raise KernelError(f"head_dim {dim} is not one of {HEAD_DIMS}")
+    rows = _rows(q, None, None, device, "q")
+    heads, kv_heads = q.shape[1], k.shape[1] if k.ndim == 3 else 0
+    if _rows(k, None, dim, device, "k") != rows or _rows(v, kv_heads, dim, device, "v") != rows:
+        raise KernelError("q, k and v must have the same rows")
+    if q.dtype == torch.float32 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise KernelError("q, k and v must all be float16 or all bfloat16")
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
+        raise KernelError(f"{heads} heads do not share {kv_heads} key/value heads")
+    if rows * (heads // kv_heads) > 1 << 30 or kv_heads > 65535:
+        raise KernelError("too many rows or heads for one call")
+    sequences = 1
+    if offsets is not None:
+        sequences = offsets.shape[0] - 1 if offsets.ndim == 1 else -1
+        _index(offsets, max(sequences, 0) + 1, device, "offsets")
+    scale = _scale(scale, dim, window, sinks)
+    out = _output(q, out)
+    if rows == 0:
+        return out
+    q, k, v = _by_sixteen_bytes(q), _by_sixteen_bytes(k), _by_sixteen_bytes(v)
+    _call("ivonar_window_attention", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[q.dtype], q.stride(0),
+          q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), heads, kv_heads, dim, rows,
+          _address(offsets), sequences, min(window, 1 << 30), min(sinks, 1 << 30), scale, out.data_ptr())
     return out

@@ -77,6 +77,7 @@ SIGNATURES: dict[str, list] = {
     "ivonar_cache_read": [_P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _P, _P],
     "ivonar_cache_attention": [_P, _I, _L, _L, _I, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _F, _I, _P, _P,
                                _L],
+    "ivonar_window_attention": [_P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _I, _I, _I, _I, _P, _I, _I, _I, _F, _P],
     "ivonar_validate_ternary": [_P, ctypes.c_longlong, _P, ctypes.c_longlong, _P],
 }
 
