@@ -18,6 +18,7 @@
 //
 // The waves of a block take the tiles of its share of the keys in turn and add their results through LDS; few rows
 // and many keys are split over several blocks, whose results (unscaled sums, m, sum) a second kernel adds.
+#include "buffer_ops.hpp"
 #include "cache_layout.hpp"
 #include "ternary_device.hpp"
 
@@ -31,37 +32,70 @@ constexpr float kGrowth = 8.0f;
 struct Params {
   CacheAttentionArgs a;
   int group;
-  int slots;   // row tiles of all sequences (an upper bound), without the slot for rows of no sequence
-  int splits;  // blocks that share a row tile's keys
-  int chunk;   // key tiles of each of them
-  float scale;  // log2(e) * scale
+  int slots;     // row tiles of all sequences (an upper bound)
+  int splits;    // blocks that share a row tile's keys; 0: the keys of all row tiles are dealt out to `blocks` blocks
+  int chunk;     // key tiles of a split, or the least that a block takes of all
+  int blocks;    // of each head
+  float scale;   // log2(e) * scale
+  bool aligned;  // q's rows start on 16 bytes
+  bool stream;   // the cache is read past the caches that outlive the call
 };
 
-// A row tile of a sequence and the key tiles that its rows see: [0, sink_tiles) and [window_tile, end_tile).
+// A row tile of a sequence and the key tiles that its rows see: [0, sink_tiles) and [window_tile, ..), at least one.
 struct Span {
   int sequence;
-  int row0;        // first row of the sequence in q
-  int rows;        // rows of the sequence times group
-  int start;       // first row of the row tile
-  int first;       // position of the sequence's first query
-  int low, high;   // positions of the row tile's first and last rows
+  int row0;       // first row of the sequence in q
+  int rows;       // rows of the sequence times group
+  int start;      // first row of the row tile
+  int first;      // position of the sequence's first query
+  int low, high;  // positions of the row tile's first and last rows
   int sink_tiles;
   int window_tile;
-  int total;       // key tiles
+  int total;      // key tiles
   __device__ int tile(int i) const { return i < sink_tiles ? i : i - sink_tiles + window_tile; }
 };
+
+template <int R>
+__device__ __forceinline__ Span make_span(const Params& p, int sequence, int row0, int queries, int length, int start) {
+  const CacheAttentionArgs& a = p.a;
+  Span s;
+  s.sequence = sequence;
+  s.row0 = row0;
+  s.rows = queries * p.group;
+  s.start = start;
+  // The table's capacity is at most 2^30 tokens, so positions less the window stay within 32 bits.
+  const int capacity = (a.table_width << a.page_shift) * kCacheTile;
+  s.first = min(max(length, 0), capacity) - queries;
+  s.low = s.first + start / p.group;
+  s.high = s.first + (min(start + R, s.rows) - 1) / p.group;
+  const int end_tile = s.high < 0 ? 0 : s.high / kCacheTile + 1;
+  s.window_tile = a.window == 0 || s.low < a.window ? 0 : (s.low - a.window + 1) / kCacheTile;
+  s.window_tile = min(s.window_tile, end_tile);
+  s.sink_tiles = a.window == 0 ? 0 : min(a.sinks <= 0 ? 0 : (a.sinks - 1) / kCacheTile + 1, s.window_tile);
+  s.total = max(1, s.sink_tiles + end_tile - s.window_tile);
+  return s;
+}
+
+// First row of a sequence and its rows, none where the offsets do not make sense.
+__device__ __forceinline__ int rows_of(const CacheAttentionArgs& a, int sequence, int& row0) {
+  if (a.offsets == nullptr) {
+    row0 = sequence;
+    return 1;
+  }
+  row0 = a.offsets[sequence];
+  return row0 < 0 ? 0 : max(0, min(a.offsets[sequence + 1], a.rows) - row0);
+}
 
 // Row tile `slot`.  With offsets, sequence b's row tiles are the slots from offsets[b] * group / R + b on, which
 // leaves each sequence at least as many as it needs.
 template <int R>
 __device__ __forceinline__ bool span_of(const Params& p, int slot, Span& s) {
   const CacheAttentionArgs& a = p.a;
-  int queries = 1;
+  int sequence, start;
   if (a.offsets == nullptr) {
     const int per = (p.group + R - 1) / R;
-    s.sequence = slot / per;
-    s.start = (slot - s.sequence * per) * R;
-    s.row0 = s.sequence;
+    sequence = slot / per;
+    start = (slot - sequence * per) * R;
   } else {
     const int lane = threadIdx.x & 63;
     int before = 0;
@@ -71,68 +105,110 @@ __device__ __forceinline__ bool span_of(const Params& p, int slot, Span& s) {
       before += __popcll(__ballot(begun));
     }
     if (before == 0) return false;
-    s.sequence = __builtin_amdgcn_readfirstlane(before - 1);
-    s.row0 = a.offsets[s.sequence];
-    queries = min(a.offsets[s.sequence + 1], a.rows) - s.row0;
-    s.start = (slot - (int)((long long)s.row0 * p.group / R) - s.sequence) * R;
+    sequence = __builtin_amdgcn_readfirstlane(before - 1);
+    start = (slot - (int)((long long)a.offsets[sequence] * p.group / R) - sequence) * R;
   }
-  if (s.sequence >= a.sequences || s.row0 < 0 || queries <= 0) return false;
-  s.rows = queries * p.group;
-  if (s.start < 0 || s.start >= s.rows) return false;
-  // The table's capacity is at most 2^30 tokens, so positions less the window stay within 32 bits.
-  const int capacity = (a.table_width << a.page_shift) * kCacheTile;
-  const int length = min(max(a.lengths[s.sequence], 0), capacity);
-  s.first = length - queries;
-  s.low = s.first + s.start / p.group;
-  s.high = s.first + (min(s.start + R, s.rows) - 1) / p.group;
-  const int end_tile = s.high < 0 ? 0 : s.high / kCacheTile + 1;
-  s.window_tile = a.window == 0 || s.low < a.window ? 0 : (s.low - a.window + 1) / kCacheTile;
-  s.window_tile = min(s.window_tile, end_tile);
-  s.sink_tiles = a.window == 0 ? 0 : min(a.sinks <= 0 ? 0 : (a.sinks - 1) / kCacheTile + 1, s.window_tile);
-  s.total = s.sink_tiles + end_tile - s.window_tile;
+  if (sequence >= a.sequences) return false;
+  int row0;
+  const int queries = rows_of(a, sequence, row0);
+  if (start < 0 || start >= queries * p.group) return false;
+  s = make_span<R>(p, sequence, row0, queries, a.lengths[sequence], start);
   return true;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The key tiles of all sequences in a row: sequence by sequence, its row tiles in order (fewer than 2^31: plan() sees
+// to it).  A block takes `share` neighbouring ones of them for one head, so that blocks end together whatever the
+// lengths are, and the heads' blocks, which start together, read the heads' parts of a page at about the same time.
+template <int R>
+__device__ __forceinline__ int tiles_of(const Params& p, int sequence) {
+  if (sequence >= p.a.sequences) return 0;
+  int row0;
+  const int queries = rows_of(p.a, sequence, row0), length = p.a.lengths[sequence];
+  int tiles = 0;
+  for (int start = 0; start < queries * p.group; start += R)
+    tiles += make_span<R>(p, sequence, row0, queries, length, start).total;
+  return tiles;
+}
+// Tiles of the sequences before `upto`.  All lanes of a wave call this together.
+template <int R>
+__device__ __forceinline__ int tiles_before(const Params& p, int upto) {
+  int sum = 0;
+  for (int b = threadIdx.x & 63; b < upto; b += 64) sum += tiles_of<R>(p, b);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  return uniform(sum);
+}
+__device__ __forceinline__ int share_of(const Params& p, int all) {
+  return max(p.chunk, (int)(((long long)all + p.blocks - 1) / p.blocks));
 }
 
 // What a lane loads of one tile.
 template <int D>
 struct Tile {
-  static constexpr int W = D / 32, kGroups = W == 8 ? 2 : 1;
-  unsigned k[2][W];
+  static constexpr int W = D / 32;
+  unsigned k[2 * W];
   unsigned v[2 * W];
-  unsigned k_scale[kGroups];
+  unsigned k_scale[2];
   uint2 v_scale;
 };
 
+// A tile on its way from memory to LDS, straight: its 34 D bytes side by side (at D = 64 a dword load of all lanes
+// reaches 128 bytes past them, which the buffer's end turns into zeros).
+template <int D>
+struct Stage {
+  static constexpr int kCodeLoads = 32 * D / 1024, kScaleLoads = D == 256 ? 2 : 1;
+  static constexpr int kLoads = kCodeLoads + kScaleLoads;
+  unsigned char codes[32 * D];
+  unsigned char scales[256 * kScaleLoads];
+};
+template <int D, bool STREAM>
+__device__ __forceinline__ void load_tile(const uint8_t* base, unsigned to, int lane) {
+  const v4u buffer = wide_buffer(base, cache_tile_bytes(D));
+#pragma unroll
+  for (int j = 0; j < Stage<D>::kCodeLoads; ++j) dma<16, STREAM>(buffer, to + j * 1024, lane * 16, j * 1024);
+#pragma unroll
+  for (int j = 0; j < Stage<D>::kScaleLoads; ++j)
+    dma<4, STREAM>(buffer, to + 32 * D + j * 256, lane * 4, 32 * D + j * 256);
+}
+
 template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* at, unsigned* to) {
+__device__ __forceinline__ void read_words(const unsigned char* at, unsigned* to) {
   if constexpr (N == 2) {
-    const uint2 x = *reinterpret_cast<const uint2*>(at);
-    to[0] = x.x;
-    to[1] = x.y;
+    const u32x2 x = *reinterpret_cast<const u32x2*>(at);
+    to[0] = x[0];
+    to[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const uint4 x = *reinterpret_cast<const uint4*>(at + 4 * i);
-      to[i] = x.x;
-      to[i + 1] = x.y;
-      to[i + 2] = x.z;
-      to[i + 3] = x.w;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(at + 4 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[i + j] = x[j];
     }
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_tile(const uint8_t* base, int lane, Tile<D>& t) {
+// A lane's keys and values of a tile in LDS.  Of up to 8 rows (NARROW) lane (n, b) takes half a row of key 16 (b / 2) + n,
+// else a quarter of the rows of keys n and 16 + n.
+template <int D, bool NARROW>
+__device__ __forceinline__ void read_tile(const unsigned char* base, int lane, Tile<D>& t) {
   constexpr int W = D / 32;
   const int n = lane & 15, b = lane >> 4;
+  if constexpr (NARROW) {
+    read_words<2 * W>(base + (16 * (b >> 1) + n) * (D / 2) + (b & 1) * (D / 4), t.k);
 #pragma unroll
-  for (int s = 0; s < 2; ++s) load_words<W>(base + (16 * s + n) * (D / 2) + b * (W * 4), t.k[s]);
+    for (int g = 0; g < W / 2; ++g) t.k_scale[g] = base[32 * D + ((b & 1) * (W / 2) + g) * 32 + n * 2 + (b >> 1)];
+  } else {
 #pragma unroll
-  for (int c = 0; c < W / 2; ++c) load_words<4>(base + 16 * D + c * 1024 + lane * 16, t.v + 4 * c);
-  const int k_group = W == 2 ? b >> 1 : W == 4 ? b : 2 * b;
+    for (int h = 0; h < 2; ++h) read_words<W>(base + (16 * h + n) * (D / 2) + b * (W * 4), t.k + h * W);
+    const int group = W == 2 ? b >> 1 : W == 4 ? b : 2 * b;
 #pragma unroll
-  for (int g = 0; g < Tile<D>::kGroups; ++g)
-    t.k_scale[g] = *reinterpret_cast<const uint16_t*>(base + 32 * D + (k_group + g) * 32 + n * 2);
+    for (int g = 0; g < (W == 8 ? 2 : 1); ++g)
+      t.k_scale[g] = *reinterpret_cast<const uint16_t*>(base + 32 * D + (group + g) * 32 + n * 2);
+  }
+#pragma unroll
+  for (int c = 0; c < W / 2; ++c) read_words<4>(base + 16 * D + c * 1024 + lane * 16, t.v + 4 * c);
   t.v_scale = *reinterpret_cast<const uint2*>(base + 33 * D + (n * W / 16) * 32 + b * 8);
 }
 
@@ -149,6 +225,12 @@ __device__ __forceinline__ unsigned convert(unsigned word, float scale, int byte
     default: return bits_as<unsigned>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3));
   }
 }
+
+// The lane 8 further on (or back) of the same 16.
+__device__ __forceinline__ unsigned other_half(unsigned v) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, false);  // row_ror:8
+}
+__device__ __forceinline__ float other_half(float v) { return __uint_as_float(other_half(__float_as_uint(v))); }
 
 // x as a sum of NT bf16 terms, x replaced by what is left.
 template <int NT>
@@ -196,370 +278,659 @@ __device__ __forceinline__ void clear_rows(const Params& p, int head) {
   }
 }
 
-template <int D, typename In, int RT, int NT>
-__global__ __launch_bounds__(kThreads) void cache_attention_kernel(Params p) {
-  constexpr int W = D / 32, R = 16 * RT, kTiles = D / 16, kPad = D + 4;
+// Blocks of 4 waves per CU that the registers leave room for (waves per SIMD).
+constexpr int occupancy(int D, int R, int NT) {
+  if (R == 64) return D == 64 && NT == 1 ? 2 : 1;
+  if (R == 8 && D == 128) return NT == 1 ? 3 : 2;
+  if (R <= 16) return D == 64 ? (NT == 3 ? 3 : 4) : D == 128 ? (NT == 3 ? 2 : 3) : NT == 3 ? 1 : 2;
+  return D == 256 || (D == 128 && NT == 3) ? 1 : D == 64 && NT == 1 ? 3 : 2;
+}
+
+// Tiles in a wave's ring: as many as that number of blocks leaves room for in a CU's 160 KB.
+constexpr int stages(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
+
+// Tiles of the sequences base .. base + 63, in the lanes, summed up to and including each lane's.
+template <int R>
+__device__ __forceinline__ int tiles_up_to(const Params& p, int base) {
+  const int lane = threadIdx.x & 63;
+  int sum = tiles_of<R>(p, base + lane);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int lower = __shfl_up(sum, o);
+    if (lane >= o) sum += lower;
+  }
+  return sum;
+}
+
+// A run of key tiles of one row tile: tiles begin .. of the row tile at row `start` of the sequence.
+struct Run {
+  int sequence, start, begin;
+};
+
+// Where a share of all key tiles begins, and how many tiles it has.
+template <int R>
+__device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run, int& left) {
+  const CacheAttentionArgs& a = p.a;
+  int sum = tiles_up_to<R>(p, 0);
+  const int all = a.sequences <= 64 ? __builtin_amdgcn_readlane(sum, 63) : tiles_before<R>(p, a.sequences);
+  const int share = share_of(p, all);
+  if ((long long)block * share >= all) return false;
+  int at = block * share, base = 0;
+  left = min(share, all - at);
+  for (;;) {
+    const int here = __builtin_amdgcn_readlane(sum, 63);
+    if (at < here) break;
+    at -= here;
+    base += 64;
+    sum = tiles_up_to<R>(p, base);
+  }
+  const int found = __builtin_ctzll(__ballot(sum > at));
+  if (found > 0) at -= __builtin_amdgcn_readlane(sum, found - 1);
+  run.sequence = base + found;
+  int row0;
+  const int queries = rows_of(a, run.sequence, row0), length = a.lengths[run.sequence];
+  for (run.start = 0;; run.start += R) {
+    const int total = make_span<R>(p, run.sequence, row0, queries, length, run.start).total;
+    if (at < total) {
+      run.begin = at;
+      return true;
+    }
+    at -= total;
+  }
+}
+
+template <int D, typename In, int R, int NT, bool STREAM>
+__global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention_kernel(Params p) {
+  constexpr bool kNarrow = R == 8;
+  constexpr int RT = kNarrow ? 1 : R / 16, kHalves = kNarrow ? 1 : 2;
+  constexpr int W = D / 32, kChunks = kNarrow ? 2 * W : W, kTiles = D / 16, kPad = D + 4;
   constexpr int NP = NT < 2 ? 2 : NT;  // terms of a weight
   const CacheAttentionArgs& a = p.a;
-  __shared__ float sums[kWaves][16][kPad];
-  __shared__ float stats[2][kWaves][R];
-  const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.x % a.kv_heads;
-  const int unit = blockIdx.x / a.kv_heads;
-  const int split = unit % p.splits, slot = unit / p.splits;
-  if (slot >= p.slots) {
-    if (split == 0) clear_rows<D, In>(p, head);
-    return;
-  }
-  Span s;
-  if (!span_of<R>(p, slot, s)) return;
-  const int begin = split * p.chunk;
-  const int end = split == p.splits - 1 ? s.total : min(s.total, begin + p.chunk);
-  if (split > 0 && begin >= end) return;
-
-  // q as the B operand: row n of row tile rt, dims 8 (b W + c) + j.
-  bf16x8 q[RT][NT][W];
-  int position[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = s.start + rt * 16 + n;
-    const bool live = row < s.rows;
-    const int token = live ? row / p.group : 0, h = live ? row - token * p.group : 0;
-    position[rt] = live ? s.first + token : -1;
-    const In* from = static_cast<const In*>(a.q) + (long long)(s.row0 + token) * a.q_strides.token +
-                     (long long)(head * p.group + h) * a.q_strides.head + b * (8 * W);
-#pragma unroll
-    for (int c = 0; c < W; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        __bf16 terms[NT];
-        split_terms<NT>(to_float(from[8 * c + j]), terms);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) q[rt][t][c][j] = terms[t];
-      }
-  }
-
-  f32x4 o[kTiles][RT];
-  float m[RT], l[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = kNoKey;
-    l[rt] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) o[i][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  const int* table = a.table + (long long)s.sequence * a.table_width;
-  const int page_mask = (1 << a.page_shift) - 1;
-  // Tile i of the span: its address, or the first page's where the sequence has no page there.
-  auto locate = [&](int i, bool& there) {
-    const int tile = s.tile(i);
-    const int page = table[tile >> a.page_shift];
-    there = (unsigned)page < (unsigned)a.page_count;
-    const long long at = ((((long long)(there ? page : 0) * a.kv_heads + head) << a.page_shift) + (tile & page_mask));
-    return a.pages + at * cache_tile_bytes(D);
+  // A ring of stages per wave, and at the end of a run the waves' sums.
+  constexpr int kStages = stages(D);
+  union Room {
+    Stage<D> ring[kWaves][kStages];
+    float sums[kWaves][16][kPad];
   };
+  __shared__ __align__(16) unsigned char room_bytes[sizeof(Room)];
+  Room& room = *reinterpret_cast<Room*>(room_bytes);
+  auto& sums = room.sums;
+  __shared__ float stats[2][kWaves][16 * RT];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool shared = p.splits == 0;
 
-  Tile<D> next;
-  bool next_there = false;
-  int i = begin + wave;
-  if (i < end) load_tile<D>(locate(i, next_there), lane, next);
-  for (; i < end; i += kWaves) {
-    const Tile<D> t = next;
-    const bool there = next_there;
-    if (i + kWaves < end) load_tile<D>(locate(i + kWaves, next_there), lane, next);
-    if (!there) continue;
+  // The block's runs of tiles: one, or as many as its share of all tiles has; and where the first one's result goes.
+  Run run;
+  int left = 0;
+  long long part;
+  const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+  if (shared) {
+    if (unit >= p.blocks) {
+      clear_rows<D, In>(p, head);
+      return;
+    }
+    if (!share_begin<R>(p, unit, run, left)) return;
+    part = 2LL * unit * a.kv_heads + head;
+  } else {
+    const int split = unit % p.splits, slot = unit / p.splits;
+    if (slot >= p.slots) {
+      if (split == 0) clear_rows<D, In>(p, head);
+      return;
+    }
+    Span s;
+    if (!span_of<R>(p, slot, s)) return;
+    run.sequence = s.sequence;
+    run.start = s.start;
+    run.begin = split * p.chunk;
+    left = split == p.splits - 1 ? s.total - run.begin : min(s.total - run.begin, p.chunk);
+    if (left <= 0) return;
+    part = ((long long)slot * p.splits + split) * a.kv_heads + head;
+  }
 
-    const int key0 = s.tile(i) * kCacheTile;
-    f32x4 x[2][RT];
+  for (;;) {
+    int row0;
+    const int sequence = uniform(run.sequence), begin = uniform(run.begin);
+    const int queries = uniform(rows_of(a, sequence, row0)), length = a.lengths[sequence];
+    const Span s = make_span<R>(p, sequence, uniform(row0), queries, length, uniform(run.start));
+    const int end = begin + min(s.total - begin, uniform(left));
+    // Opaque to the compiler, which would otherwise compute every address of the loop's body ahead of it, and hold
+    // them in registers throughout.
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & 63, n = lane & 15, b = lane >> 4;
+    // In the constant address space, so that pages are looked up by scalar loads: the wait for a vector load would be
+    // a wait for every tile under way.
+    typedef const __attribute__((address_space(4))) int* Constants;
+    const Constants table = (Constants)(uintptr_t)(a.table + (long long)s.sequence * a.table_width);
+    const int page_mask = (1 << a.page_shift) - 1;
+    // Page of tile i of the span.
+    auto page_of = [&](int i) { return table[s.tile(i) >> a.page_shift]; };
+    // Begins to load tile i, or the first page's where the sequence has no page there.
+    auto load = [&](int i, int page, int stage) {
+      const bool there = (unsigned)page < (unsigned)a.page_count;
+      const long long at =
+          (((long long)(there ? page : 0) * a.kv_heads + head) << a.page_shift) + (s.tile(i) & page_mask);
+      load_tile<D, STREAM>(a.pages + at * cache_tile_bytes(D), lds_address(&room.ring[wave][stage]), lane);
+      return there;
+    };
+
+    // A wave takes every fourth tile, and has up to kStages - 1 of them under way from memory to its ring.
+    int i = begin + wave;
+    const int last = i < end ? i + (end - 1 - i) / kWaves * kWaves : i;
+    unsigned there = 0;  // bit k: the tile k turns ahead has a page
+    int page = 0;        // of the next tile to load
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int k = 0; k < kStages - 1; ++k)
+      if (i + k * kWaves <= last && i < end) there |= (unsigned)load(i + k * kWaves, page_of(i + k * kWaves), k) << k;
+    if (i < end) page = page_of(min(i + (kStages - 1) * kWaves, last));
+    int stage = 0;
+    // q as the B operand.  Row n of row tile rt, dims 8 (b W + c) + j; of up to 8 rows, row n % 8 and dims
+    // (b % 2) D / 2 + 8 c + j, where the keys b / 2 = n / 8, and zero elsewhere: columns 0 .. 7 of the product are then the
+    // rows with the tile's first 16 keys, columns 8 .. 15 with its others, so that every lane has logits of its own.
+    bf16x8 q[RT][NT][kChunks];
+    int position[RT];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) x[h][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = s.start + rt * 16 + (kNarrow ? n & 7 : n);
+      const bool live = row < s.rows, mine = !kNarrow || b >> 1 == n >> 3;
+      const int token = live ? row / p.group : 0, h = live ? row - token * p.group : 0;
+      position[rt] = live ? s.first + token : -1;
+      const In* from = static_cast<const In*>(a.q) + (long long)(s.row0 + token) * a.q_strides.token +
+                       (long long)(head * p.group + h) * a.q_strides.head + (kNarrow ? b & 1 : b) * (8 * kChunks);
 #pragma unroll
-      for (int c = 0; c < W; ++c) {
-        const float scale = scale_operand(t.k_scale[W == 8 ? c / 4 : 0], h);
-        u32x4 words;
+      for (int c = 0; c < kChunks; ++c) {
+        float x[8];
+        load8(from + 8 * c, p.aligned, x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) words[j] = convert(t.k[h][c], scale, j);
-        const bf16x8 key = bits_as<bf16x8>(words);
+        for (int j = 0; j < 8; ++j) {
+          __bf16 terms[NT];
+          split_terms<NT>(mine ? x[j] : 0.0f, terms);
+#pragma unroll
+          for (int z = 0; z < NT; ++z) q[rt][z][c][j] = terms[z];
+        }
+      }
+    }
+
+    f32x4 o[kTiles][RT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = kNoKey;
+      l[rt] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) o[i][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    for (; i < end; i += kWaves) {
+      // This tile has arrived when only the ones after it are under way; towards the end there are fewer of those.
+      if (i + (kStages - 2) * kWaves <= last)
+        wait_loads<(kStages - 2) * Stage<D>::kLoads>();
+      else
+        wait_loads<0>();
+      // The stage of the tile before this one, which has been used, takes the next tile.
+      if (i + (kStages - 1) * kWaves <= last) {
+        there |= (unsigned)load(i + (kStages - 1) * kWaves, page, stage == 0 ? kStages - 1 : stage - 1) << (kStages - 1);
+        page = page_of(min(i + kStages * kWaves, last));
+      }
+      Tile<D> t;
+      read_tile<D, kNarrow>(reinterpret_cast<const unsigned char*>(&room.ring[wave][stage]), lane, t);
+      const int key0 = s.tile(i) * kCacheTile;
+      const bool whole = (there & 1) != 0 && key0 + kCacheTile - 1 <= s.low &&
+                         (a.window == 0 || key0 > s.high - a.window || key0 + kCacheTile <= a.sinks);
+      // Zero times a key that is no number would be no number as well.  Where rows see different keys, such scales of
+      // up to 8 rows' tiles become one here, and the logits of the keys get their NaN below.  Scales above kScaleMax
+      // are never written, but unwritten bytes may hold them.
+      unsigned long long strange = 0;
+      if (kNarrow && !whole) {
+        bool found = false;
+#pragma unroll
+        for (int g = 0; g < W / 2; ++g) {
+          if (t.k_scale[g] > (unsigned)kScaleMax) {
+            t.k_scale[g] = 127;
+            found = true;
+          }
+        }
+        strange = __ballot(found);
+      }
+      // x[h][rt][r]: the logit of key 16 h + 4 b + r, or of up to 8 rows 16 (n / 8) + 4 b + r.
+      f32x4 x[kHalves][RT];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) x[h][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 upper = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // of up to 8 rows, a second chain of products
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const float scale = kNarrow ? scale_operand(t.k_scale[c / 4], 0) : scale_operand(t.k_scale[W == 8 ? c / 4 : 0], h);
+          u32x4 words;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) words[j] = convert(t.k[h * W + c], scale, j);
+          const bf16x8 key = bits_as<bf16x8>(words);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int z = 0; z < NT; ++z) {
+              f32x4& sum = kNarrow && c >= kChunks / 2 ? upper : x[h][rt];
+              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, q[rt][z][c], sum, 0, 0, 0);
+            }
+        }
+        if constexpr (kNarrow) x[h][0] += upper;
+      }
+
+      uint2 v_scale = t.v_scale;
+      unsigned hidden = 0;  // bit e: the scale of the lane's token e stands for no number
+      if (!whole) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int z = 0; z < NT; ++z)
-            x[h][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, q[rt][z][c], x[h][rt], 0, 0, 0);
-      }
-    }
-
-    uint2 v_scale = t.v_scale;
-    const bool whole = key0 + kCacheTile - 1 <= s.low &&
-                       (a.window == 0 || key0 > s.high - a.window || key0 + kCacheTile <= a.sinks);
-    unsigned hidden = 0;  // bit e: the scale of the lane's token e stands for no number
-    if (!whole) {
+          for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+            for (int r = 0; r < 4; ++r) {
+              const int key = key0 + 16 * (kNarrow ? n >> 3 : h) + 4 * b + r;
+              const bool seen = (there & 1) != 0 && key <= position[rt] &&
+                                (a.window == 0 || key > position[rt] - a.window || key < a.sinks);
+              x[h][rt][r] = seen ? x[h][rt][r] : -INFINITY;
+            }
+        if (kNarrow && strange != 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int r = 0; r < 4; ++r)
+            if (((strange >> (32 * (n >> 3) + 4 * b + r)) & 0x10001u) != 0 && x[0][0][r] != -INFINITY) x[0][0][r] = NAN;
+        }
+        // A weight of zero times a value that is no number likewise: such scales become one, and the rows that do see
+        // their tokens get NaN below.
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = key0 + 16 * h + 4 * b + r;
-            const bool seen = key <= position[rt] &&
-                              (a.window == 0 || key > position[rt] - a.window || key < a.sinks);
-            x[h][rt][r] = seen ? x[h][rt][r] : -INFINITY;
+        for (int e = 0; e < 8; ++e) {
+          unsigned& word = e < 4 ? v_scale.x : v_scale.y;
+          const int shift = 8 * (e & 3);
+          if (((word >> shift) & 255u) > (unsigned)kScaleMax) {
+            hidden |= 1u << e;
+            word = (word & ~(255u << shift)) | (127u << shift);
           }
-      // A weight of zero times a value that is no number would be no number: such scales become one here, and the
-      // rows that do see them get their NaN below.  Scales above kScaleMax are never written, but unwritten bytes
-      // may hold them.
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        unsigned& word = e < 4 ? v_scale.x : v_scale.y;
-        const int shift = 8 * (e & 3);
-        if (((word >> shift) & 255u) > (unsigned)kScaleMax) {
-          hidden |= 1u << e;
-          word = (word & ~(255u << shift)) | (127u << shift);
         }
       }
-    }
 
-    float most[RT];
-    bool grows = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const f32x4 u = x[0][rt], w = x[1][rt];
-      most[rt] = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))) * p.scale;
-      grows |= most[rt] > m[rt] + kGrowth;
-    }
-    if (__ballot(grows) != 0ull) {
+      float most[RT];
+      bool grows = false;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        // Only the rows that grow: a row's rounding does not depend on its neighbours.
-        const float highest = lane_groups_max(most[rt]);
-        const float raised = highest > m[rt] + kGrowth ? highest : m[rt];
-        const float factor = __builtin_amdgcn_exp2f(m[rt] - raised);
-        m[rt] = raised;
-        l[rt] *= factor;
+        most[rt] = x[0][rt][0];
 #pragma unroll
-        for (int k = 0; k < kTiles; ++k) o[k][rt] *= factor;
+        for (int e = 1; e < 4 * kHalves; ++e) most[rt] = fmaxf(most[rt], x[e / 4][rt][e & 3]);
+        most[rt] *= p.scale;
+        grows |= most[rt] > m[rt] + kGrowth;
       }
-    }
-
-    bf16x8 weights[RT][NP];
+      if (__ballot(grows) != 0ull) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float sum = 0.0f;
+        for (int rt = 0; rt < RT; ++rt) {
+          // Only the rows that grow: a row's rounding does not depend on its neighbours.
+          const float highest = lane_groups_max(kNarrow ? fmaxf(most[rt], other_half(most[rt])) : most[rt]);
+          const float raised = highest > m[rt] + kGrowth ? highest : m[rt];
+          const float factor = __builtin_amdgcn_exp2f(m[rt] - raised);
+          m[rt] = raised;
+          l[rt] *= factor;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float w = __builtin_amdgcn_exp2f(fmaf(x[h][rt][r], p.scale, -m[rt]));
-          sum += w;
-          __bf16 terms[NP];
-          split_terms<NP>(w, terms);
-#pragma unroll
-          for (int z = 0; z < NP; ++z) weights[rt][z][4 * h + r] = terms[z];
+          for (int k = 0; k < kTiles; ++k) o[k][rt] *= factor;
         }
-      l[rt] += sum;
-    }
-
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      unsigned pairs[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        constexpr int kPer = 16 / W;
-        const int byte = (e % kPer) * W + w;
-        pairs[e] = convert(t.v[(e / kPer) * 4 + byte / 4], scale_operand(e < 4 ? v_scale.x : v_scale.y, e & 3),
-                           byte & 3);
       }
-      u32x4 even, odd;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        even[e] = __builtin_amdgcn_perm(pairs[2 * e + 1], pairs[2 * e], 0x05040100u);
-        odd[e] = __builtin_amdgcn_perm(pairs[2 * e + 1], pairs[2 * e], 0x07060302u);
-      }
-      const bf16x8 value0 = bits_as<bf16x8>(even), value1 = bits_as<bf16x8>(odd);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int z = 0; z < NP; ++z) {
-          o[2 * w][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value0, weights[rt][z], o[2 * w][rt], 0, 0, 0);
-          o[2 * w + 1][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value1, weights[rt][z], o[2 * w + 1][rt], 0, 0, 0);
-        }
-    }
 
-    if (!whole && __ballot(hidden != 0u) != 0ull) {
-      // How many tokens without a number each row sees, per 2 W dims: the product of the flags and the visibility.
-      bf16x8 flags;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) flags[e] = (__bf16)((hidden >> e) & 1u ? 1.0f : 0.0f);
+      // The weights as the B operand: row n, keys 4 b + r and 16 + 4 b + r in elements r and 4 + r.  Of up to 8 rows,
+      // columns 0 .. 7 take the first terms of a row's weights and columns 8 .. 15 the second ones, for all of its keys.
+      constexpr int kOperands = kNarrow ? NP / 2 + NP % 2 : NP;
+      bf16x8 weights[RT][kOperands];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        bf16x8 seen;
+        unsigned words[NP][2 * kHalves];
+        float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) seen[e] = (__bf16)(x[e / 4][rt][e & 3] == -INFINITY ? 0.0f : 1.0f);
-        f32x4 count = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(flags, seen, count, 0, 0, 0);
+        for (int e = 0; e < 4 * kHalves; e += 2) {
+          __bf16 terms[2][NP];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (count[r] > 0.0f)
+          for (int f = 0; f < 2; ++f) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(x[e / 4][rt][(e + f) & 3], p.scale, -m[rt]));
+            sum += w;
+            split_terms<NP>(w, terms[f]);
+          }
 #pragma unroll
-            for (int k = 0; k < kTiles; ++k) o[k][rt][r] = NAN;
+          for (int z = 0; z < NP; ++z) words[z][e / 2] = bits_as<unsigned>(bf16x2{terms[0][z], terms[1][z]});
+        }
+        l[rt] += sum;
+        if constexpr (kNarrow) {
+          const bool lower = n < 8;
+#pragma unroll
+          for (int z = 0; z < NP; z += 2) {
+            unsigned own[2], others[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const unsigned second = z + 1 < NP ? words[z + 1 < NP ? z + 1 : z][e] : 0u;
+              own[e] = lower ? words[z][e] : second;
+              others[e] = other_half(lower ? second : words[z][e]);
+              if (z + 1 == NP && !lower) others[e] = 0u;
+            }
+            weights[rt][z / 2] = bits_as<bf16x8>(lower ? u32x4{own[0], own[1], others[0], others[1]}
+                                                       : u32x4{others[0], others[1], own[0], own[1]});
+          }
+        } else {
+#pragma unroll
+          for (int z = 0; z < NP; ++z)
+            weights[rt][z] = bits_as<bf16x8>(u32x4{words[z][0], words[z][1], words[z][2], words[z][3]});
+        }
+      }
+
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        unsigned pairs[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          constexpr int kPer = 16 / W;
+          const int byte = (e % kPer) * W + w;
+          pairs[e] = convert(t.v[(e / kPer) * 4 + byte / 4], scale_operand(e < 4 ? v_scale.x : v_scale.y, e & 3),
+                             byte & 3);
+        }
+        u32x4 even, odd;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          even[e] = __builtin_amdgcn_perm(pairs[2 * e + 1], pairs[2 * e], 0x05040100u);
+          odd[e] = __builtin_amdgcn_perm(pairs[2 * e + 1], pairs[2 * e], 0x07060302u);
+        }
+        const bf16x8 value0 = bits_as<bf16x8>(even), value1 = bits_as<bf16x8>(odd);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int z = 0; z < kOperands; ++z) {
+            o[2 * w][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value0, weights[rt][z], o[2 * w][rt], 0, 0, 0);
+            o[2 * w + 1][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value1, weights[rt][z], o[2 * w + 1][rt], 0, 0, 0);
+          }
+      }
+
+      there >>= 1;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+
+      if (!whole && __ballot(hidden != 0u) != 0ull) {
+        // How many tokens without a number each row sees, per 2 W dims: the product of the flags and the visibility.
+        bf16x8 flags;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) flags[e] = (__bf16)((hidden >> e) & 1u ? 1.0f : 0.0f);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          bf16x8 seen;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool of_lane = !kNarrow || e / 4 == n >> 3;
+            seen[e] = (__bf16)(!of_lane || x[kNarrow ? 0 : e / 4][rt][e & 3] == -INFINITY ? 0.0f : 1.0f);
+          }
+          f32x4 count = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(flags, seen, count, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (count[r] > 0.0f)
+#pragma unroll
+              for (int k = 0; k < kTiles; ++k) o[k][rt][r] = NAN;
+        }
       }
     }
-  }
 
-  // The waves' results, relative to the block's maximum of each row, added in the waves' order.
+    const bool all = begin == 0 && end == s.total;
+    __syncthreads();  // the rings are in use no more
+    // The waves' results, relative to the block's maximum of each row, added in the waves' order.
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] = lane_groups_sum(l[rt]);
-    if (b == 0) {
-      stats[0][wave][rt * 16 + n] = m[rt];
-      stats[1][wave][rt * 16 + n] = l[rt];
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] = lane_groups_sum(kNarrow ? l[rt] + other_half(l[rt]) : l[rt]);
+      if (b == 0) {
+        stats[0][wave][rt * 16 + n] = m[rt];
+        stats[1][wave][rt * 16 + n] = l[rt];
+      }
     }
-  }
-  __syncthreads();
-  const long long part = ((long long)slot * a.kv_heads + head) * p.splits + split;
-  float* sums_out = a.work + part * (R * (D + 2));
-  float* stats_out = sums_out + R * D;
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float highest = kNoKey;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) highest = fmaxf(highest, stats[0][w][rt * 16 + n]);
-    const float factor = __builtin_amdgcn_exp2f(m[rt] - highest);
-    if (rt > 0) __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int k = 0; k < kTiles; ++k) sums[wave][n][kTiles * (4 * b + r) + k] = o[k][rt][r] * factor;
     __syncthreads();
-    for (int at = threadIdx.x; at < 16 * D / 4; at += kThreads) {
-      const int line = at / (D / 4), column = at % (D / 4) * 4;
-      const int row = s.start + rt * 16 + line;
-      if (row >= s.rows) continue;
-      float top = kNoKey, total = 0.0f;
+    constexpr int kLines = kNarrow ? 8 : 16;
+    float* sums_out = a.work + part * (R * (D + 2));
+    float* stats_out = sums_out + R * D;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[0][w][rt * 16 + line]);
+    for (int rt = 0; rt < RT; ++rt) {
+      float highest = kNoKey;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        total += stats[1][w][rt * 16 + line] * __builtin_amdgcn_exp2f(stats[0][w][rt * 16 + line] - top);
-      float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int w = 0; w < kWaves; ++w) highest = fmaxf(highest, stats[0][w][rt * 16 + n]);
+      const float factor = __builtin_amdgcn_exp2f(m[rt] - highest);
+      if (rt > 0) __syncthreads();
+      // Of up to 8 rows, columns n and n + 8 hold parts of one row.
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float4 v = *reinterpret_cast<const float4*>(&sums[w][line][column]);
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-      }
-      if (p.splits == 1) {
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-        const int token = row / p.group, h = row - token * p.group;
-        In* to = static_cast<In*>(a.out) + ((long long)(s.row0 + token) * a.heads + head * p.group + h) * D + column;
-        store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
-      } else {
-        *reinterpret_cast<float4*>(sums_out + (rt * 16 + line) * D + column) = sum;
-        if (column == 0) {
-          stats_out[2 * (rt * 16 + line)] = top;
-          stats_out[2 * (rt * 16 + line) + 1] = total;
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < kTiles; k += 4)
+          *reinterpret_cast<float4*>(&sums[wave][n][kTiles * (4 * b + r) + k]) =
+              float4{o[k][rt][r] * factor, o[k + 1][rt][r] * factor, o[k + 2][rt][r] * factor, o[k + 3][rt][r] * factor};
+      __syncthreads();
+      for (int at = thread; at < kLines * D / 4; at += kThreads) {
+        const int line = at / (D / 4), column = at % (D / 4) * 4;
+        const int row = s.start + rt * 16 + line;
+        if (row >= s.rows) continue;
+        float top = kNoKey, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[0][w][rt * 16 + line]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+          total += stats[1][w][rt * 16 + line] * __builtin_amdgcn_exp2f(stats[0][w][rt * 16 + line] - top);
+        float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(&sums[w][line][column]);
+          sum.x += v.x;
+          sum.y += v.y;
+          sum.z += v.z;
+          sum.w += v.w;
+          if constexpr (kNarrow) {
+            const float4 u = *reinterpret_cast<const float4*>(&sums[w][line + 8][column]);
+            sum.x += u.x;
+            sum.y += u.y;
+            sum.z += u.z;
+            sum.w += u.w;
+          }
+        }
+        if (all) {
+          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          const int token = row / p.group, h = row - token * p.group;
+          In* to = static_cast<In*>(a.out) + ((long long)(s.row0 + token) * a.heads + head * p.group + h) * D + column;
+          store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
+        } else {
+          *reinterpret_cast<float4*>(sums_out + (rt * 16 + line) * D + column) = sum;
+          if (column == 0) {
+            stats_out[2 * (rt * 16 + line)] = top;
+            stats_out[2 * (rt * 16 + line) + 1] = total;
+          }
         }
       }
     }
+
+    left -= end - begin;
+    if (left <= 0) return;
+    // The next run starts with the first tile of the next row tile or sequence.
+    part = (2LL * unit + 1) * a.kv_heads + head;
+    run.begin = 0;
+    run.start = s.start + R;
+    if (run.start >= s.rows) {
+      run.start = 0;
+      do {
+        if (++run.sequence >= a.sequences) return;
+      } while (rows_of(a, run.sequence, row0) == 0);
+    }
+    __syncthreads();  // the statistics in LDS have been read
   }
 }
 
-// Adds the parts of a row in their order: a wave per row, D / 64 dims per lane.
-template <int D, typename In, int R>
+// Adds the parts of a row: THREADS threads per row (query token and head), four dims each, so that several parts are
+// read at a time; every thread adds its parts in their order, and the threads' sums are added in theirs.
+template <int D, typename In, int R, int THREADS>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
-  constexpr int kDims = D / 64;
+  constexpr int kLanes = D / 4, kRowsPerBlock = kThreads / THREADS, kAtOnce = THREADS / kLanes, kPart = R * (D + 2);
   const CacheAttentionArgs& a = p.a;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long id = (long long)blockIdx.x * kWaves + wave;
-  const int line = (int)(id % R);
-  const long long unit = id / R;
-  const int head = (int)(unit % a.kv_heads), slot = (int)(unit / a.kv_heads);
-  Span s;
-  if (slot >= p.slots || !span_of<R>(p, slot, s)) return;
-  const int row = s.start + line;
-  if (row >= s.rows) return;
-  const int parts = max(1, min(p.splits, (s.total + p.chunk - 1) / p.chunk));
-  const float* from = a.work + unit * p.splits * (R * (D + 2));
-  float top = kNoKey;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, from[(long long)i * (R * (D + 2)) + R * D + 2 * line]);
-  float total = 0.0f, sum[kDims] = {};
-  for (int i = 0; i < parts; ++i) {
-    const float* part = from + (long long)i * (R * (D + 2));
-    const float factor = __builtin_amdgcn_exp2f(part[R * D + 2 * line] - top);
-    total += part[R * D + 2 * line + 1] * factor;
+  __shared__ float4 sums[kThreads];
+  __shared__ float totals[kThreads];
+  const int thread = threadIdx.x % THREADS;
+  const int group_of = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
+  const long long id = (long long)blockIdx.x * kRowsPerBlock + group_of;
+  const int row = (int)(id / a.heads), h = (int)(id % a.heads);
+  int sequence = 0, index = 0;
+  const bool live = row < a.rows && find_sequence(a.offsets, a.sequences, row, row, sequence, index);
+  bool merging = false;
+  float top = kNoKey, total = 0.0f;
+  float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (live) {
+    const int head = h / p.group, line = index * p.group + h % p.group;
+    int row0;
+    const int queries = rows_of(a, sequence, row0), length = a.lengths[sequence];
+    const Span s = make_span<R>(p, sequence, row0, queries, length, line / R * R);
+    // The parts of this row tile and head are part 0 and then those `step` apart from `second` on.
+    int parts, step;
+    long long part0, second;
+    if (p.splits > 0) {
+      const int first_slot = a.offsets == nullptr ? sequence * ((p.group + R - 1) / R)
+                                                  : (int)((long long)row0 * p.group / R) + sequence;
+      parts = min(p.splits, (s.total + p.chunk - 1) / p.chunk);
+      part0 = (long long)(first_slot + line / R) * p.splits * a.kv_heads + head;
+      second = part0 + a.kv_heads;
+      step = a.kv_heads;
+    } else {
+      const int share = share_of(p, tiles_before<R>(p, a.sequences));
+      int begin = tiles_before<R>(p, sequence);
+      for (int start = 0; start < s.start; start += R)
+        begin += make_span<R>(p, sequence, row0, queries, length, start).total;
+      const int first_block = begin / share;
+      parts = (begin + s.total - 1) / share - first_block + 1;
+      part0 = (2LL * first_block + (begin % share == 0 ? 0 : 1)) * a.kv_heads + head;
+      second = 2LL * (first_block + 1) * a.kv_heads + head;
+      step = 2 * a.kv_heads;
+    }
+    merging = parts > 1;  // a single part went to its place at once
+    if (merging) {
+      const float* from = a.work;
+      auto part_of = [&](int i) { return (i == 0 ? part0 : second + (long long)(i - 1) * step) * kPart; };
+      const float* stats = from + R * D + 2 * (line % R);
+      const float* values = from + (line % R) * D + thread % kLanes * 4;
+      for (int i = threadIdx.x & 63; i < parts; i += 64) top = fmaxf(top, stats[part_of(i)]);
 #pragma unroll
-    for (int k = 0; k < kDims; ++k) sum[k] += part[line * D + lane * kDims + k] * factor;
+      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+#pragma unroll 4
+      for (int i = thread / kLanes; i < parts; i += kAtOnce) {
+        const long long at = part_of(i);
+        const float factor = __builtin_amdgcn_exp2f(stats[at] - top);
+        const float4 v = *reinterpret_cast<const float4*>(values + at);
+        total += stats[at + 1] * factor;
+        sum.x += v.x * factor;
+        sum.y += v.y * factor;
+        sum.z += v.z * factor;
+        sum.w += v.w * factor;
+      }
+    }
+  }
+  sums[threadIdx.x] = sum;
+  totals[threadIdx.x] = total;
+  __syncthreads();
+  if (!merging || thread >= kLanes) return;
+#pragma unroll
+  for (int k = 1; k < kAtOnce; ++k) {
+    const float4 v = sums[threadIdx.x + k * kLanes];
+    total += totals[threadIdx.x + k * kLanes];
+    sum.x += v.x;
+    sum.y += v.y;
+    sum.z += v.z;
+    sum.w += v.w;
   }
   const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-  const int token = row / p.group, h = row - token * p.group;
-  In* to = static_cast<In*>(a.out) + ((long long)(s.row0 + token) * a.heads + head * p.group + h) * D + lane * kDims;
-#pragma unroll
-  for (int k = 0; k < kDims; ++k) store_value(to + k, sum[k] * inverse);
+  In* to = static_cast<In*>(a.out) + ((long long)row * a.heads + h) * D + thread * 4;
+  store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
 }
 
-// Row tiles per wave: as many as the sequences' rows fill on average, within the registers.
-int row_tiles(const CacheAttentionArgs& a) {
+constexpr int kUnitsOnDevice = 256;  // CUs
+constexpr int kLeastTiles = 8;       // least share of a block: two tiles per wave
+constexpr int kChunkBlocks = 512;
+// Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.
+constexpr long long kStreamBytes = 128LL << 20;
+// Row tiles and heads, and their key tiles, at which each goes to one block as a whole.
+constexpr int kWholeUnits = 512, kWholeTiles = 64;
+
+// Rows of a row tile: 8, or a multiple of 16 as the sequences' rows fill on average, within the registers.
+int tile_rows(const CacheAttentionArgs& a) {
   const long long rows = (long long)a.rows * (a.heads / a.kv_heads) / (a.sequences > 0 ? a.sequences : 1);
-  if (rows <= 16 || (a.head_dim == 256 && a.dtype != kBfloat16)) return 1;
-  if (rows <= 32 || a.head_dim == 256 || a.dtype == kFloat32) return 2;
-  return 4;
+  if (a.head_dim == 256) return rows <= 16 || a.dtype != kBfloat16 ? 16 : 32;
+  if (rows <= 8) return 8;
+  if (rows <= 16) return 16;
+  return rows <= 32 || a.dtype == kFloat32 ? 32 : 64;
 }
 
 Params plan(const CacheAttentionArgs& a) {
-  Params p{a, a.heads / a.kv_heads, 0, 1, 1, 1.44269504088896340736f * a.scale};
-  const int R = 16 * row_tiles(a);
+  Params p{a, a.heads / a.kv_heads, 0, 1, 0, 0, 1.44269504088896340736f * a.scale, false, false};
+  const int size = a.dtype == kFloat32 ? 4 : 2;
+  p.aligned = (((uintptr_t)a.q | (uintptr_t)(a.q_strides.token * size) | (uintptr_t)(a.q_strides.head * size)) & 15u) == 0;
+  const int R = tile_rows(a);
   const long long rows = (long long)a.rows * p.group;
   p.slots = (int)(a.offsets == nullptr ? (long long)a.sequences * ((p.group + R - 1) / R) : rows / R + a.sequences);
-  // Key tiles that a row tile sees at most, in shares of at least kLeastTiles such that about kBlocks blocks run.
-  constexpr long long kBlocks = 1024, kLeastTiles = 16;
+  // Key tiles that a row tile sees at most, and the row tiles and heads that there may be.
   long long keys = a.max_length;
   if (a.window > 0) keys = min(keys, (long long)a.window + (R + p.group - 1) / p.group + a.sinks + 2 * kCacheTile);
   const long long tiles = max(1LL, (keys + kCacheTile - 1) / kCacheTile);
-  const long long live = a.offsets == nullptr ? p.slots : min((long long)p.slots, rows / R + (rows % R > 0) + a.sequences / 2);
-  const long long wanted = max(1LL, kBlocks / max(1LL, live * a.kv_heads));
-  p.chunk = (int)max(kLeastTiles, (tiles + wanted - 1) / wanted);
-  p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+  const long long units = (rows / R + (rows % R > 0 || a.offsets == nullptr ? 1 : 0)) * a.kv_heads;
+  const int terms = a.dtype == kFloat32 ? 3 : a.dtype == kFloat16 ? 2 : 1;
+  const int resident = kUnitsOnDevice * occupancy(a.head_dim, R, terms);
+  const long long few = (long long)max(a.sequences, 1) * 4;
+  const long long live = max((long long)a.sequences * a.kv_heads, units);
+  p.stream = live * tiles * cache_tile_bytes(a.head_dim) > kStreamBytes;
+  const bool dealt = rows / R <= few && a.sequences <= 4096 &&
+                     ((long long)a.table_width << a.page_shift) * a.sequences <= 0x7fffffffLL / (few / max(a.sequences, 1)) && (tiles > kWholeTiles || live < kWholeUnits) && tiles > kLeastTiles;
+  if (dealt) {
+    p.splits = 0;
+    p.chunk = kLeastTiles;
+    p.blocks = (int)max(1LL, min((long long)resident, (live * tiles + kLeastTiles - 1) / kLeastTiles) / a.kv_heads);
+  } else {
+    const long long wanted = max(1LL, kChunkBlocks / max(1LL, live));
+    p.chunk = (int)max((long long)kLeastTiles, (tiles + wanted - 1) / wanted);
+    p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+  }
   return p;
 }
 
-template <int D, typename In, int RT, int NT>
+template <int D, typename In, int R, int NT>
 hipError_t run(hipStream_t stream, const Params& p) {
-  const long long blocks = (long long)(p.slots + (p.a.offsets != nullptr ? 1 : 0)) * p.splits * p.a.kv_heads;
+  const bool clears = p.a.offsets != nullptr;  // rows of no sequence
+  const long long blocks = ((long long)(p.splits == 0 ? p.blocks : p.slots * p.splits) + (clears ? max(p.splits, 1) : 0)) * p.a.kv_heads;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((cache_attention_kernel<D, In, RT, NT>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
-  if (p.splits > 1) {
-    const long long merges = (long long)p.slots * p.a.kv_heads * (16 * RT) / kWaves;
+  if (R <= 16 && p.stream)
+    hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, R <= 16>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
+                       p);
+  else
+    hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
+                       p);
+  if (p.splits != 1) {
+    const long long rows = (long long)p.a.rows * p.a.heads;
+    // A whole block per row where rows may have many parts.
+    const bool wide = p.splits > 16 || (p.splits == 0 && p.blocks > 16 * rows / p.a.heads);
+    const long long merges = wide ? rows : (rows + kWaves - 1) / kWaves;
     if (merges > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((merge_kernel<D, In, 16 * RT>), dim3((unsigned)merges), dim3(kThreads), 0, stream, p);
+    if (wide)
+      hipLaunchKernelGGL((merge_kernel<D, In, R, kThreads>), dim3((unsigned)merges), dim3(kThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((merge_kernel<D, In, R, 64>), dim3((unsigned)merges), dim3(kThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
 
+template <int D, typename In, int NT>
+hipError_t run_rows(hipStream_t stream, const Params& p) {
+  const int rows = tile_rows(p.a);
+  if constexpr (D < 256) {
+    if (rows == 8) return run<D, In, 8, NT>(stream, p);
+    if (rows == 32) return run<D, In, 32, NT>(stream, p);
+    if constexpr (NT < 3)
+      if (rows == 64) return run<D, In, 64, NT>(stream, p);
+  } else if constexpr (NT == 1) {
+    if (rows == 32) return run<D, In, 32, NT>(stream, p);
+  }
+  return run<D, In, 16, NT>(stream, p);
+}
+
 template <int D>
 hipError_t run_types(hipStream_t stream, const Params& p) {
-  const int tiles = row_tiles(p.a);
-  if (p.a.dtype == kFloat32) {
-    if constexpr (D < 256)
-      if (tiles == 2) return run<D, float, 2, 3>(stream, p);
-    return run<D, float, 1, 3>(stream, p);
-  }
-  if (p.a.dtype == kFloat16) {
-    if constexpr (D < 256) {
-      if (tiles == 4) return run<D, Half, 4, 2>(stream, p);
-      if (tiles == 2) return run<D, Half, 2, 2>(stream, p);
-    }
-    return run<D, Half, 1, 2>(stream, p);
-  }
-  if constexpr (D < 256)
-    if (tiles == 4) return run<D, Bfloat, 4, 1>(stream, p);
-  if (tiles == 2) return run<D, Bfloat, 2, 1>(stream, p);
-  return run<D, Bfloat, 1, 1>(stream, p);
+  if (p.a.dtype == kFloat32) return run_rows<D, float, 3>(stream, p);
+  if (p.a.dtype == kFloat16) return run_rows<D, Half, 2>(stream, p);
+  return run_rows<D, Bfloat, 1>(stream, p);
 }
 
 }  // namespace
@@ -567,7 +938,8 @@ hipError_t run_types(hipStream_t stream, const Params& p) {
 long long cache_attention_work(const CacheAttentionArgs& a) {
   const Params p = plan(a);
   if (p.splits == 1) return 0;
-  return (long long)p.slots * a.kv_heads * p.splits * (16 * row_tiles(a)) * (a.head_dim + 2) * 4;
+  const long long parts = (p.splits == 0 ? 2LL * p.blocks : (long long)p.slots * p.splits) * a.kv_heads;
+  return parts * tile_rows(a) * (a.head_dim + 2) * 4;
 }
 
 hipError_t launch_cache_attention(hipStream_t stream, const CacheAttentionArgs& a) {

@@ -44,6 +44,30 @@ __device__ __forceinline__ void dma16(v4u buffer, unsigned lds_base, int voffset
       : "memory");
 }
 
+// The same for pieces of BYTES (16 or 4) per lane, past the memory-side cache with STREAM.
+template <int BYTES, bool STREAM>
+__device__ __forceinline__ void dma(v4u buffer, unsigned lds_base, int voffset, int soffset) {
+  int saved;
+#define IVO_DMA(LOAD)                                                              \
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t" LOAD "\n\t" \
+               "s_mov_b32 m0, %0"                                                  \
+               : "=&s"(saved)                                                      \
+               : "s"(lds_base), "v"(voffset), "s"(buffer), "s"(soffset)            \
+               : "memory")
+  if constexpr (BYTES == 16 && STREAM) IVO_DMA("buffer_load_dwordx4 %2, %3, %4 offen nt lds");
+  if constexpr (BYTES == 16 && !STREAM) IVO_DMA("buffer_load_dwordx4 %2, %3, %4 offen lds");
+  if constexpr (BYTES == 4 && STREAM) IVO_DMA("buffer_load_dword %2, %3, %4 offen nt lds");
+  if constexpr (BYTES == 4 && !STREAM) IVO_DMA("buffer_load_dword %2, %3, %4 offen lds");
+#undef IVO_DMA
+}
+
+// Waits until at most N of the wave's loads are under way.  A direct load counts until its bytes are in LDS, so the
+// wave itself may read them then; other waves need a barrier as well (direct_load_sync).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ int load_b32(v4u buffer, int voffset, int soffset) {
   int r;
   asm volatile("buffer_load_dword %0, %1, %2, %3 offen" : "=v"(r) : "v"(voffset), "s"(buffer), "s"(soffset) : "memory");

@@ -13,18 +13,6 @@
 namespace ivo {
 namespace {
 
-template <typename In>
-__device__ __forceinline__ void load8(const In* p, bool aligned, float (&x)[8]) {
-  if (aligned) {
-    const float4 a = load4(p, 0), b = load4(p, 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = to_float(p[j]);
-  }
-}
-
 __device__ __forceinline__ unsigned quad_max(unsigned v) {
   v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));  // lane ^ 1
   return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));  // lane ^ 2

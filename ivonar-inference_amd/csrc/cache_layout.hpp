@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include "internal.hpp"
+#include "ternary_device.hpp"
 
 namespace ivo {
 
@@ -39,6 +40,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename To, typename From>
@@ -47,6 +49,19 @@ __device__ __forceinline__ To bits_as(const From& v) {
   To out;
   __builtin_memcpy(&out, &v, sizeof(To));
   return out;
+}
+
+// Eight neighbouring values as fp32: in loads of 16 or 8 bytes where rows start on 16 bytes, else one by one.
+template <typename In>
+__device__ __forceinline__ void load8(const In* p, bool aligned, float (&x)[8]) {
+  if (aligned) {
+    const float4 a = load4(p, 0), b = load4(p, 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = to_float(p[j]);
+  }
 }
 
 // Which sequence of a ragged batch a row belongs to, and its index there.  offsets is the row prefix [sequences + 1]
