@@ -118,30 +118,33 @@ __device__ __forceinline__ bool span_of(const Params& p, int slot, Span& s) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The key tiles of all sequences in a row: sequence by sequence, its row tiles in order (fewer than 2^31: plan() sees
-// to it).  A block takes `share` neighbouring ones of them for one head, so that blocks end together whatever the
+// The key tiles of all sequences in a row: sequence by sequence, its row tiles in order.  A block takes `share` neighbouring ones of them for one head, so that blocks end together whatever the
 // lengths are, and the heads' blocks, which start together, read the heads' parts of a page at about the same time.
 template <int R>
-__device__ __forceinline__ int tiles_of(const Params& p, int sequence) {
+__device__ __forceinline__ long long tiles_of(const Params& p, int sequence) {
   if (sequence >= p.a.sequences) return 0;
   int row0;
   const int queries = rows_of(p.a, sequence, row0), length = p.a.lengths[sequence];
-  int tiles = 0;
+  long long tiles = 0;
   for (int start = 0; start < queries * p.group; start += R)
     tiles += make_span<R>(p, sequence, row0, queries, length, start).total;
   return tiles;
 }
+__device__ __forceinline__ long long uniform(long long v) {
+  const unsigned low = (unsigned)uniform((int)v);
+  return (long long)((unsigned long long)(unsigned)uniform((int)(v >> 32)) << 32 | low);
+}
 // Tiles of the sequences before `upto`.  All lanes of a wave call this together.
 template <int R>
-__device__ __forceinline__ int tiles_before(const Params& p, int upto) {
-  int sum = 0;
+__device__ __forceinline__ long long tiles_before(const Params& p, int upto) {
+  long long sum = 0;
   for (int b = threadIdx.x & 63; b < upto; b += 64) sum += tiles_of<R>(p, b);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   return uniform(sum);
 }
-__device__ __forceinline__ int share_of(const Params& p, int all) {
-  return max(p.chunk, (int)(((long long)all + p.blocks - 1) / p.blocks));
+__device__ __forceinline__ long long share_of(const Params& p, long long all) {
+  return max((long long)p.chunk, (all + p.blocks - 1) / p.blocks);
 }
 
 // What a lane loads of one tile.
@@ -291,12 +294,12 @@ constexpr int stages(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
 
 // Tiles of the sequences base .. base + 63, in the lanes, summed up to and including each lane's.
 template <int R>
-__device__ __forceinline__ int tiles_up_to(const Params& p, int base) {
+__device__ __forceinline__ long long tiles_up_to(const Params& p, int base) {
   const int lane = threadIdx.x & 63;
-  int sum = tiles_of<R>(p, base + lane);
+  long long sum = tiles_of<R>(p, base + lane);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int lower = __shfl_up(sum, o);
+    const long long lower = __shfl_up(sum, o);
     if (lane >= o) sum += lower;
   }
   return sum;
@@ -309,30 +312,31 @@ struct Run {
 
 // Where a share of all key tiles begins, and how many tiles it has.
 template <int R>
-__device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run, int& left) {
+__device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run, long long& left) {
   const CacheAttentionArgs& a = p.a;
-  int sum = tiles_up_to<R>(p, 0);
-  const int all = a.sequences <= 64 ? __builtin_amdgcn_readlane(sum, 63) : tiles_before<R>(p, a.sequences);
-  const int share = share_of(p, all);
-  if ((long long)block * share >= all) return false;
-  int at = block * share, base = 0;
+  long long sum = tiles_up_to<R>(p, 0);
+  const long long all = a.sequences <= 64 ? uniform(__shfl(sum, 63)) : tiles_before<R>(p, a.sequences);
+  const long long share = share_of(p, all);
+  long long at = block * share;
+  if (at >= all) return false;
   left = min(share, all - at);
+  int base = 0;
   for (;;) {
-    const int here = __builtin_amdgcn_readlane(sum, 63);
+    const long long here = uniform(__shfl(sum, 63));
     if (at < here) break;
     at -= here;
     base += 64;
     sum = tiles_up_to<R>(p, base);
   }
   const int found = __builtin_ctzll(__ballot(sum > at));
-  if (found > 0) at -= __builtin_amdgcn_readlane(sum, found - 1);
+  if (found > 0) at -= uniform(__shfl(sum, found - 1));
   run.sequence = base + found;
   int row0;
   const int queries = rows_of(a, run.sequence, row0), length = a.lengths[run.sequence];
   for (run.start = 0;; run.start += R) {
     const int total = make_span<R>(p, run.sequence, row0, queries, length, run.start).total;
     if (at < total) {
-      run.begin = at;
+      run.begin = (int)at;
       return true;
     }
     at -= total;
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
 
   // The block's runs of tiles: one, or as many as its share of all tiles has; and where the first one's result goes.
   Run run;
-  int left = 0;
+  long long left = 0;
   long long part;
   const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
   if (shared) {
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
     const int sequence = uniform(run.sequence), begin = uniform(run.begin);
     const int queries = uniform(rows_of(a, sequence, row0)), length = a.lengths[sequence];
     const Span s = make_span<R>(p, sequence, uniform(row0), queries, length, uniform(run.start));
-    const int end = begin + min(s.total - begin, uniform(left));
+    const int end = begin + (int)min((long long)(s.total - begin), uniform(left));
     // Opaque to the compiler, which would otherwise compute every address of the loop's body ahead of it, and hold
     // them in registers throughout.
     int thread = threadIdx.x;
@@ -789,14 +793,14 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
       second = part0 + a.kv_heads;
       step = a.kv_heads;
     } else {
-      const int share = share_of(p, tiles_before<R>(p, a.sequences));
-      int begin = tiles_before<R>(p, sequence);
+      const long long share = share_of(p, tiles_before<R>(p, a.sequences));
+      long long begin = tiles_before<R>(p, sequence);
       for (int start = 0; start < s.start; start += R)
         begin += make_span<R>(p, sequence, row0, queries, length, start).total;
-      const int first_block = begin / share;
-      parts = (begin + s.total - 1) / share - first_block + 1;
-      part0 = (2LL * first_block + (begin % share == 0 ? 0 : 1)) * a.kv_heads + head;
-      second = 2LL * (first_block + 1) * a.kv_heads + head;
+      const long long first_block = begin / share;
+      parts = (int)((begin + s.total - 1) / share - first_block) + 1;
+      part0 = (2 * first_block + (begin % share == 0 ? 0 : 1)) * a.kv_heads + head;
+      second = 2 * (first_block + 1) * a.kv_heads + head;
       step = 2 * a.kv_heads;
     }
     merging = parts > 1;  // a single part went to its place at once
@@ -873,8 +877,8 @@ Params plan(const CacheAttentionArgs& a) {
   const long long few = (long long)max(a.sequences, 1) * 4;
   const long long live = max((long long)a.sequences * a.kv_heads, units);
   p.stream = live * tiles * cache_tile_bytes(a.head_dim) > kStreamBytes;
-  const bool dealt = rows / R <= few && a.sequences <= 4096 &&
-                     ((long long)a.table_width << a.page_shift) * a.sequences <= 0x7fffffffLL / (few / max(a.sequences, 1)) && (tiles > kWholeTiles || live < kWholeUnits) && tiles > kLeastTiles;
+  const bool dealt = rows / R <= few && a.sequences <= 4096 && (tiles > kWholeTiles || live < kWholeUnits) &&
+                     tiles > kLeastTiles;
   if (dealt) {
     p.splits = 0;
     p.chunk = kLeastTiles;

@@ -27,17 +27,20 @@ its results and a workspace, or synchronises, so all of them can be captured int
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 from torch import Tensor
 
-from .ops import _address, _call, _require_device
-from .runtime import KernelError, library
+from . import runtime
+from .ops import _address
+from .runtime import KernelError, check, initialise, library
 
 TOKENS_PER_TILE = 32
 HEAD_DIMS = (64, 128, 256)
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def cache_pages(pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
@@ -52,86 +55,106 @@ def cache_pages(pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
     return torch.zeros((pages, kv_heads, page_size // TOKENS_PER_TILE, 34 * head_dim), dtype=torch.uint8, device=device)
 
 
-def _geometry(pages: Tensor, table: Tensor, what: str) -> tuple[int, int, int, int]:
-    """(pages, kv_heads, tiles per page, head_dim) of a cache, with its table checked."""
-    if pages.dtype != torch.uint8 or pages.ndim != 4 or not pages.is_contiguous():
+# The checks below read as few attributes as they can: each costs as much host time as a few instructions of the launch,
+# and a decoder makes these calls once per layer and token.
+
+
+def _device(first: Tensor, *others: Tensor | None) -> int:
+    index = first.get_device()
+    for tensor in others:
+        if tensor is not None and tensor.get_device() != index:
+            raise KernelError("the tensors of a call must be on one ROCm device")
+    if index < 0:
+        raise KernelError("attention and its cache need tensors on a ROCm device")
+    if index not in runtime._initialised:
+        initialise(index)
+    return index
+
+
+def _run(name: str, index: int, *args) -> None:
+    status = getattr(library(), name)(_raw_stream(index), *args)
+    if status != 0:
+        check(status, name)
+
+
+def _geometry(pages: Tensor, table: Tensor, what: str) -> tuple[int, int, int, int, int, int]:
+    """(pages, kv_heads, tiles per page, head_dim, sequences, width) of a cache and its table."""
+    shape = pages.shape
+    if len(shape) != 4 or pages.dtype is not torch.uint8 or not pages.is_contiguous():
         raise KernelError(f"{what} needs pages as cache_pages() makes them")
-    count, heads, tiles, size = pages.shape
-    if size % 34 or size // 34 not in HEAD_DIMS or tiles & (tiles - 1) or pages.numel() == 0:
+    count, heads, tiles, size = shape
+    dim = size // 34
+    if dim * 34 != size or dim not in HEAD_DIMS or tiles & (tiles - 1) or not (count and heads and tiles):
         raise KernelError(f"{what} needs pages as cache_pages() makes them")
-    if table.dtype != torch.int32 or table.ndim != 2 or not table.is_contiguous():
+    shape = table.shape
+    if len(shape) != 2 or table.dtype is not torch.int32 or not table.is_contiguous():
         raise KernelError(f"{what} needs a contiguous int32 table [sequences, width]")
-    if table.shape[1] * tiles * TOKENS_PER_TILE > 1 << 30:
+    sequences, width = shape
+    if width * tiles * TOKENS_PER_TILE > 1 << 30:
         raise KernelError(f"{what}: a sequence has at most 2**30 tokens")
-    return count, heads, tiles, size // 34
+    return count, heads, tiles, dim, sequences, width
 
 
-def _index(tensor: Tensor, count: int, device: torch.device, what: str) -> None:
-    if (tensor.dtype != torch.int32 or tensor.ndim != 1 or tensor.shape[0] != count or not tensor.is_contiguous()
-            or tensor.device != device):
-        raise KernelError(f"{what} must be contiguous int32 [{count}] on the cache's device")
+def _index(tensor: Tensor, count: int, what: str) -> None:
+    if tensor.dtype is not torch.int32 or tensor.shape != (count,) or not tensor.is_contiguous():
+        raise KernelError(f"{what} must be contiguous int32 [{count}]")
 
 
-def _sequences(table: Tensor, offsets: Tensor | None, rows: int, device: torch.device) -> int:
-    sequences = table.shape[0]
+def _offsets(offsets: Tensor | None, sequences: int, rows: int) -> None:
     if offsets is not None:
-        _index(offsets, sequences + 1, device, "offsets")
+        _index(offsets, sequences + 1, "offsets")
     elif rows != sequences:
         raise KernelError(f"{rows} rows of {sequences} sequences need offsets")
-    return sequences
 
 
-def _rows(x: Tensor, heads: int | None, head_dim: int | None, device: torch.device, what: str) -> int:
-    if x.ndim != 3 or (heads is not None and x.shape[1] != heads) or (head_dim is not None and x.shape[2] != head_dim):
-        raise KernelError(f"{what} must be [rows, {heads or 'heads'}, {head_dim or 'head_dim'}], not {list(x.shape)}")
+def _rows(x: Tensor, heads: int | None, head_dim: int | None, what: str) -> tuple[int, int, int, int]:
+    """(rows, heads, stride of a row, stride of a head) of x."""
+    shape = x.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
+        raise KernelError(f"{what} must be [rows, {heads or 'heads'}, {head_dim or 'head_dim'}], not {list(shape)}")
     if x.dtype not in _DTYPES:
         raise KernelError(f"{what} must be float32, float16 or bfloat16, not {x.dtype}")
-    if x.stride(2) != 1 or x.device != device:
-        raise KernelError(f"{what} must have a head's values side by side, on the device of the other tensors")
-    return x.shape[0]
-
-
-def _same_device(device: torch.device, *tensors: Tensor) -> None:
-    if any(tensor.device != device for tensor in tensors):
-        raise KernelError("the tensors of a call must be on one device")
+    row, head, value = x.stride()
+    if value != 1:
+        raise KernelError(f"{what} must have a head's values side by side")
+    return shape[0], shape[1], row, head
 
 
 def cache_write(pages: Tensor, k: Tensor, v: Tensor, table: Tensor, past: Tensor, offsets: Tensor | None = None) -> None:
     """Quantises rows of k and v [rows, kv_heads, head_dim] (fp32, fp16 or bfloat16, any row and head stride) into the
     cache: row r of sequence b becomes position past[b] + r - offsets[b]."""
-    device = _require_device(pages, k, v, table, past, offsets)
-    count, heads, tiles, dim = _geometry(pages, table, "cache_write")
-    rows = _rows(k, heads, dim, device, "k")
-    if _rows(v, heads, dim, device, "v") != rows or v.dtype != k.dtype:
+    device = _device(pages, k, v, table, past, offsets)
+    count, heads, tiles, dim, sequences, width = _geometry(pages, table, "cache_write")
+    rows, _, k_row, k_head = _rows(k, heads, dim, "k")
+    v_rows, _, v_row, v_head = _rows(v, heads, dim, "v")
+    if v_rows != rows or v.dtype is not k.dtype:
         raise KernelError("k and v must have the same rows and type")
-    _same_device(device, pages, table)
-    sequences = _sequences(table, offsets, rows, device)
-    _index(past, sequences, device, "past")
-    if rows == 0:
-        return
-    _call("ivonar_cache_write", device, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], k.stride(0), k.stride(1),
-          v.stride(0), v.stride(1), rows, pages.data_ptr(), count, heads, tiles, dim, table.data_ptr(), table.shape[1],
-          past.data_ptr(), _address(offsets), sequences)
+    _offsets(offsets, sequences, rows)
+    _index(past, sequences, "past")
+    if rows:
+        _run("ivonar_cache_write", device, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], k_row, k_head, v_row, v_head,
+             rows, pages.data_ptr(), count, heads, tiles, dim, table.data_ptr(), width, past.data_ptr(),
+             _address(offsets), sequences)
 
 
 def cache_read(pages: Tensor, table: Tensor, start: Tensor | None, offsets: Tensor | None, rows: int,
                dtype: torch.dtype = torch.float32) -> tuple[Tensor, Tensor]:
     """(k, v) [rows, kv_heads, head_dim] as `dtype`: row r of sequence b is position start[b] + r - offsets[b] (start
     None: 0)."""
-    device = _require_device(pages, table, start, offsets)
-    count, heads, tiles, dim = _geometry(pages, table, "cache_read")
-    _same_device(device, pages, table)
+    device = _device(pages, table, start, offsets)
+    count, heads, tiles, dim, sequences, width = _geometry(pages, table, "cache_read")
     if dtype not in _DTYPES:
         raise KernelError(f"the cache is read as float32, float16 or bfloat16, not {dtype}")
     if rows < 0:
         raise KernelError("rows must not be negative")
-    sequences = _sequences(table, offsets, rows, device)
+    _offsets(offsets, sequences, rows)
     if start is not None:
-        _index(start, sequences, device, "start")
-    k, v = torch.empty((2, rows, heads, dim), dtype=dtype, device=device)
+        _index(start, sequences, "start")
+    k = pages.new_empty((rows, heads, dim), dtype=dtype)
+    v = torch.empty_like(k)
     if rows:
-        _call("ivonar_cache_read", device, pages.data_ptr(), count, heads, tiles, dim, table.data_ptr(), table.shape[1],
-              _address(start), _address(offsets), sequences, rows, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
+        _run("ivonar_cache_read", device, pages.data_ptr(), count, heads, tiles, dim, table.data_ptr(), width,
+             _address(start), _address(offsets), sequences, rows, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -147,10 +170,17 @@ def _scale(scale: float | None, head_dim: int, window: int, sinks: int) -> float
 
 def _output(q: Tensor, out: Tensor | None) -> Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise KernelError("out must be contiguous and of q's shape, type and device")
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
+        raise KernelError("out must be contiguous and of q's shape and type")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(*sizes: int) -> int:
+    """Bytes that a call of these sizes needs besides its operands."""
+    *head, ragged, sequences, rows, window, sinks, longest = sizes
+    return library().ivonar_cache_attention_work(*head, 1 if ragged else None, sequences, rows, window, sinks, longest)
 
 
 def cache_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, offsets: Tensor | None = None,
@@ -164,39 +194,29 @@ def cache_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, of
     that sees nothing is zero.  scale (default head_dim ** -0.5) multiplies q . k.  max_length, about the longest
     length, sets how keys are shared between blocks (default: what the table can hold); any value gives the same
     result up to the order of sums."""
-    device = _require_device(q, pages, table, lengths, offsets)
-    count, kv_heads, tiles, dim = _geometry(pages, table, "cache_attention")
-    rows = _rows(q, None, dim, device, "q")
-    heads = q.shape[1]
+    device = _device(q, pages, table, lengths, offsets, out)
+    count, kv_heads, tiles, dim, sequences, width = _geometry(pages, table, "cache_attention")
+    rows, heads, q_row, q_head = _rows(q, None, dim, "q")
     if heads == 0 or heads % kv_heads:
         raise KernelError(f"{heads} heads do not share {kv_heads} key/value heads")
     if rows * (heads // kv_heads) > 1 << 30:
         raise KernelError("too many rows for one call")
-    _same_device(device, pages, table)
-    sequences = _sequences(table, offsets, rows, device)
-    _index(lengths, sequences, device, "lengths")
+    _offsets(offsets, sequences, rows)
+    _index(lengths, sequences, "lengths")
     scale = _scale(scale, dim, window, sinks)
     out = _output(q, out)
     if rows == 0:
         return out
-    capacity = table.shape[1] * tiles * TOKENS_PER_TILE
+    capacity = width * tiles * TOKENS_PER_TILE
     longest = capacity if max_length is None else max(1, min(int(max_length), capacity))
     window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-    dtype, address = _DTYPES[q.dtype], _address(offsets)
-    need = library().ivonar_cache_attention_work(dtype, heads, kv_heads, dim, address, sequences, rows, window, sinks,
-                                                 longest)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    _call("ivonar_cache_attention", device, q.data_ptr(), dtype, q.stride(0), q.stride(1), heads, rows,
-          pages.data_ptr(), count, kv_heads, tiles, dim, table.data_ptr(), table.shape[1], lengths.data_ptr(), address,
-          sequences, window, sinks, scale, longest, out.data_ptr(), _address(work), max(need, 0))
+    dtype = _DTYPES[q.dtype]
+    need = _workspace(dtype, heads, kv_heads, dim, offsets is not None, sequences, rows, window, sinks, longest)
+    work = pages.new_empty(need) if need > 0 else None
+    _run("ivonar_cache_attention", device, q.data_ptr(), dtype, q_row, q_head, heads, rows, pages.data_ptr(), count,
+         kv_heads, tiles, dim, table.data_ptr(), width, lengths.data_ptr(), _address(offsets), sequences, window, sinks,
+         scale, longest, out.data_ptr(), _address(work), need)
     return out
-
-
-def _by_sixteen_bytes(x: Tensor) -> Tensor:
-    """x with rows that start on 16 bytes, after a copy where they do not (or lie further apart than a call takes)."""
-    if x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.stride(0) < 1 << 23:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
 
 
 def window_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor | None = None, window: int = 0, sinks: int = 0,
@@ -208,15 +228,17 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor | None = N
     sequence's rows up to its own, and with a window (0: none) only the last `window` of them and the first `sinks`
     of the sequence.  heads is a multiple of kv_heads.  scale (default head_dim ** -0.5) multiplies q . k.  Rows that
     do not start on 16 bytes are copied first."""
-    device = _require_device(q, k, v, offsets)
-    dim = q.shape[-1]
+    device = _device(q, k, v, offsets, out)
+    rows, heads, q_row, q_head = _rows(q, None, None, "q")
+    dim = q.shape[2]
     if dim not in HEAD_DIMS:
         raise KernelError(f"head_dim {dim} is not one of {HEAD_DIMS}")
-    rows = _rows(q, None, None, device, "q")
-    heads, kv_heads = q.shape[1], k.shape[1] if k.ndim == 3 else 0
-    if _rows(k, None, dim, device, "k") != rows or _rows(v, kv_heads, dim, device, "v") != rows:
+    k_rows, kv_heads, k_row, k_head = _rows(k, None, dim, "k")
+    v_rows, _, v_row, v_head = _rows(v, kv_heads, dim, "v")
+    if k_rows != rows or v_rows != rows:
         raise KernelError("q, k and v must have the same rows")
-    if q.dtype == torch.float32 or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype is torch.float32 or k.dtype is not dtype or v.dtype is not dtype:
         raise KernelError("q, k and v must all be float16 or all bfloat16")
     if heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise KernelError(f"{heads} heads do not share {kv_heads} key/value heads")
@@ -224,14 +246,17 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor | None = N
         raise KernelError("too many rows or heads for one call")
     sequences = 1
     if offsets is not None:
-        sequences = offsets.shape[0] - 1 if offsets.ndim == 1 else -1
-        _index(offsets, max(sequences, 0) + 1, device, "offsets")
+        sequences = offsets.shape[0] - 1 if offsets.dim() == 1 else -1
+        _index(offsets, max(sequences, 0) + 1, "offsets")
     scale = _scale(scale, dim, window, sinks)
     out = _output(q, out)
     if rows == 0:
         return out
-    q, k, v = _by_sixteen_bytes(q), _by_sixteen_bytes(k), _by_sixteen_bytes(v)
-    _call("ivonar_window_attention", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[q.dtype], q.stride(0),
-          q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), heads, kv_heads, dim, rows,
-          _address(offsets), sequences, min(window, 1 << 30), min(sinks, 1 << 30), scale, out.data_ptr())
+    if ((q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 or (q_row | q_head | k_row | k_head | v_row | v_head) & 7
+            or k_row >= 1 << 23 or v_row >= 1 << 23):
+        q, k, v = (x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
+        (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
+    _run("ivonar_window_attention", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], q_row, q_head,
+         k_row, k_head, v_row, v_head, heads, kv_heads, dim, rows, _address(offsets), sequences, min(window, 1 << 30),
+         min(sinks, 1 << 30), scale, out.data_ptr())
     return out
