@@ -294,7 +294,7 @@ hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, 
 /* Causal attention within packed prompts over fp16 or bf16 rows (dtype 1 or 2): out [rows, heads, head_dim], a row of
  * sequence b at position r - offsets[b] sees the sequence's rows up to its own, with a window and sinks as above.
  * offsets NULL: one sequence of all rows (sequences == 1).  Rows of no sequence are 0.  Addresses are multiples of 16
- * bytes and strides of 8 elements; the token strides of k and v lie in 0 .. 2^23 - 1. */
+ * bytes and strides of 8 elements; the token strides of k and v lie in head_dim .. 2^23 - 1. */
 hipError_t ivonar_window_attention(hipStream_t stream, const void* q, const void* k, const void* v, int dtype,
                                    long long q_token_stride, long long q_head_stride, long long k_token_stride,
                                    long long k_head_stride, long long v_token_stride, long long v_head_stride,

@@ -100,6 +100,19 @@ __device__ __forceinline__ void clear_rows(const Params& p, int head) {
   }
 }
 
+// Whether a piece of eight values holds one that is no finite number.
+template <typename T>
+__device__ __forceinline__ bool strange(const u32x4& words) {
+  bool found = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    found |= (words[j] & T::kNonFinite) == T::kNonFinite || (words[j] >> 16 & T::kNonFinite) == T::kNonFinite;
+  return found;
+}
+__device__ __forceinline__ u32x4 piece_of(const unsigned char* rows, int slot) {
+  return *reinterpret_cast<const u32x4*>(rows + slot * 16);
+}
+
 template <int D, int KEYS>
 struct Stage {
   unsigned char k[KEYS * D * 2];
@@ -136,31 +149,30 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
   const int tiles = sink_tiles + end_tile - window_tile;
   auto tile_of = [&](int i) { return i < sink_tiles ? i : i - sink_tiles + window_tile; };
 
-  // A tile's rows from memory to LDS; rows past the sequence are zeros.
+  // A tile's rows from memory to LDS: a thread takes the same place of kLoads rows kStep apart, whose swizzle is the
+  // same (at D = 256, every other's).  Rows past the sequence start past the buffer's end, and are zeros.
+  constexpr int kStep = kThreads / kPieces, kPlaces = D == 256 ? 2 : 1;
   const uint16_t* k0 = static_cast<const uint16_t*>(a.k) + rows.begin * a.k_strides.token + kv_head * a.k_strides.head;
   const uint16_t* v0 = static_cast<const uint16_t*>(a.v) + rows.begin * a.v_strides.token + kv_head * a.v_strides.head;
+  const int k_step = (int)a.k_strides.token * 2 * kStep, v_step = (int)a.v_strides.token * 2 * kStep;
+  int k_at[kPlaces], v_at[kPlaces];
+#pragma unroll
+  for (int j = 0; j < kPlaces; ++j) {
+    const int row = (int)threadIdx.x / kPieces, piece = (int)threadIdx.x % kPieces;
+    k_at[j] = row * (int)a.k_strides.token * 2 + (piece ^ k_swizzle<D>(row + j * kStep)) * 16;
+    v_at[j] = row * (int)a.v_strides.token * 2 + (piece ^ v_swizzle<D>(row + j * kStep)) * 16;
+  }
   auto load_tile = [&](int i, int stage) {
     const int key0 = tile_of(i) * KEYS;
     const int count = min(KEYS, rows.count - key0);
     const v4u k_buffer = wide_buffer(k0 + key0 * a.k_strides.token, ((count - 1) * a.k_strides.token + D) * 2);
     const v4u v_buffer = wide_buffer(v0 + key0 * a.v_strides.token, ((count - 1) * a.v_strides.token + D) * 2);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int slot = j * kThreads + (int)threadIdx.x, row = slot / kPieces, piece = slot % kPieces;
-      const int to = (j * kThreads + wave * 64) * 16;
-      // A row past the sequence starts past the buffer, whatever the stride.
-      const bool there = row < count;
-      dma16(k_buffer, lds_address(stages[stage].k + to),
-            there ? (int)(row * a.k_strides.token * 2) + (piece ^ k_swizzle<D>(row)) * 16 : 0x7ffffff0, 0);
-    }
+    for (int j = 0; j < kLoads; ++j)
+      dma16(k_buffer, lds_address(stages[stage].k + (j * kThreads + wave * 64) * 16), k_at[j % kPlaces], j * k_step);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int slot = j * kThreads + (int)threadIdx.x, row = slot / kPieces, piece = slot % kPieces;
-      const int to = (j * kThreads + wave * 64) * 16;
-      const bool there = row < count;
-      dma16(v_buffer, lds_address(stages[stage].v + to),
-            there ? (int)(row * a.v_strides.token * 2) + (piece ^ v_swizzle<D>(row)) * 16 : 0x7ffffff0, 0);
-    }
+    for (int j = 0; j < kLoads; ++j)
+      dma16(v_buffer, lds_address(stages[stage].v + (j * kThreads + wave * 64) * 16), v_at[j % kPlaces], j * v_step);
   };
 
   load_tile(0, 0);
@@ -172,6 +184,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
                            head * a.q_strides.head + half * 8;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) q[c] = *reinterpret_cast<const vec*>(from + c * 16);
+    // Waits for q here: a wait inside the loop would be one for the next tile's loads in every turn.
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) asm volatile("" : "+v"(q[c]));
   }
 
   f32x16 o[kDims];
@@ -183,9 +198,56 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
 
   for (int i = 0; i < tiles; ++i) {
     const int key0 = tile_of(i) * KEYS;
-    const Stage<D, KEYS>& stage = stages[i & 1];
+    Stage<D, KEYS>& stage = stages[i & 1];
     direct_load_sync();  // this tile has arrived, and nobody reads the other buffer any more
     if (i + 1 < tiles) load_tile(i + 1, (i + 1) & 1);
+    // A weight of zero times a value that is no finite number would be no number.  Where rows see different keys, such
+    // values go to the sums of the rows that see them here, and become zeros in LDS.
+    const bool edge = key0 + KEYS - 1 > rows.start ||
+                      (a.window > 0 && key0 <= last - a.window && key0 + KEYS > a.sinks);
+    if (edge) {
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) found |= strange<T>(piece_of(stage.v, j * kThreads + (int)threadIdx.x));
+      if (__syncthreads_or(found)) {
+#pragma unroll 1
+        for (int slot = lane; slot < KEYS * kPieces; slot += 64) {
+          const u32x4 words = piece_of(stage.v, slot);
+          unsigned long long left = __ballot(strange<T>(words));
+          while (left != 0ull) {
+            const int from = __builtin_ctzll(left), at = slot - lane + from, row = at / kPieces;
+            left &= left - 1;
+            const int key = key0 + row;
+            const bool seen = key <= position && (a.window == 0 || key > position - a.window || key < a.sinks);
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {
+              const unsigned word = e < 4 ? (e < 2 ? words[0] : words[1]) : (e < 6 ? words[2] : words[3]);
+              const unsigned bits = __builtin_amdgcn_readlane((int)word, from) >> (16 * (e & 1)) & 0xffffu;
+              if ((bits & T::kNonFinite) != T::kNonFinite) continue;
+              const float number = (bits & 0x7fffu) != T::kNonFinite ? NAN : bits >> 15 ? -INFINITY : INFINITY;
+              const int dim = ((at % kPieces) ^ v_swizzle<D>(row)) * 8 + e;
+#pragma unroll
+              for (int k = 0; k < kDims; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  if (seen && 32 * k + 8 * (r / 4) + 4 * half + r % 4 == dim) o[k][r] += number;
+            }
+          }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int slot = threadIdx.x; slot < KEYS * kPieces; slot += kThreads) {
+          u32x4 words = piece_of(stage.v, slot);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if ((words[j] & T::kNonFinite) == T::kNonFinite) words[j] &= 0xffff0000u;
+            if ((words[j] >> 16 & T::kNonFinite) == T::kNonFinite) words[j] &= 0xffffu;
+          }
+          *reinterpret_cast<u32x4*>(stage.v + slot * 16) = words;
+        }
+        __syncthreads();
+      }
+    }
     const bool none = key0 > high || low >= rows.count ||
                       (a.window > 0 && key0 + KEYS - 1 <= low - a.window && key0 >= a.sinks);
     if (none) continue;
@@ -203,6 +265,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
         x[s] = T::mfma(key, q[c], x[s]);
       }
     }
+    // Four reads of K ahead of the products that use them.
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int j = 0; j < kSubtiles * D / 16; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
 
     const bool whole = key0 + KEYS - 1 <= low &&
                        (a.window == 0 || key0 > high - a.window || key0 + KEYS <= a.sinks);
@@ -216,6 +285,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
           x[s][r] = seen ? x[s][r] : -INFINITY;
         }
     }
+    // Keeps the logits in the registers of the product on either way (they would be copied otherwise).
+#pragma unroll
+    for (int s = 0; s < kSubtiles; ++s) asm volatile("" : "+v"(x[s]));
 
     float most = -INFINITY;
 #pragma unroll
@@ -265,62 +337,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
       }
       return words;
     };
-    // A weight of zero times a value that is no finite number would be no number: where rows see different keys, such
-    // values are left out of the product, and added below for the rows that see them.
-    auto strange = [](const u32x4& words) {
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        found |= (words[j] & T::kNonFinite) == T::kNonFinite || (words[j] >> 16 & T::kNonFinite) == T::kNonFinite;
-      return found;
-    };
-    bool finite = true;
-    if (!whole) {
-      bool found = false;
-#pragma unroll 2
-      for (int j = 0; j < KEYS * kPieces / 64; ++j)
-        found |= strange(*reinterpret_cast<const u32x4*>(stage.v + (j * 64 + lane) * 16));
-      finite = __ballot(found) == 0ull;
-    }
 #pragma unroll
     for (int block = 0; block < 2 * kSubtiles; ++block)
 #pragma unroll
-      for (int k = 0; k < kDims; ++k) {
-        u32x4 words = value(block, k);
-        if (!finite)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if ((words[j] & T::kNonFinite) == T::kNonFinite) words[j] &= 0xffff0000u;
-            if ((words[j] >> 16 & T::kNonFinite) == T::kNonFinite) words[j] &= 0xffffu;
-          }
-        o[k] = T::mfma(bits_as<vec>(words), weights[block], o[k]);
-      }
-    if (!finite) {
-#pragma unroll 1
-      for (int j = 0; j < KEYS * kPieces / 64; ++j) {
-        const u32x4 words = *reinterpret_cast<const u32x4*>(stage.v + (j * 64 + lane) * 16);
-        unsigned long long left = __ballot(strange(words));
-        while (left != 0ull) {
-          const int from = __builtin_ctzll(left), slot = j * 64 + from, row = slot / kPieces;
-          left &= left - 1;
-          const int key = key0 + row;
-          const bool seen = key <= position && (a.window == 0 || key > position - a.window || key < a.sinks);
-#pragma unroll 1
-          for (int e = 0; e < 8; ++e) {
-            const unsigned word = e < 4 ? (e < 2 ? words[0] : words[1]) : (e < 6 ? words[2] : words[3]);
-            const unsigned bits = __builtin_amdgcn_readlane((int)word, from) >> (16 * (e & 1)) & 0xffffu;
-            if ((bits & T::kNonFinite) != T::kNonFinite) continue;
-            const float number = (bits & 0x7fffu) != T::kNonFinite ? NAN : bits >> 15 ? -INFINITY : INFINITY;
-            const int dim = ((slot % kPieces) ^ v_swizzle<D>(row)) * 8 + e;
-#pragma unroll
-            for (int k = 0; k < kDims; ++k)
-#pragma unroll
-              for (int r = 0; r < 16; ++r)
-                if (seen && 32 * k + 8 * (r / 4) + 4 * half + r % 4 == dim) o[k][r] += number;
-          }
-        }
-      }
-    }
+      for (int k = 0; k < kDims; ++k) o[k] = T::mfma(bits_as<vec>(value(block, k)), weights[block], o[k]);
   }
 
   l += __shfl_xor(l, 32);

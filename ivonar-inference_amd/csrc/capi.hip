@@ -597,7 +597,8 @@ hipError_t ivonar_window_attention(hipStream_t stream, const void* q, const void
   for (long long stride : strides)
     if ((stride & 7) != 0) return hipErrorInvalidValue;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return hipErrorInvalidValue;
-  if (k_token_stride < 0 || k_token_stride >= 1 << 23 || v_token_stride < 0 || v_token_stride >= 1 << 23)
+  // A row past a tile's last one has to start past its buffer.
+  if (k_token_stride < head_dim || k_token_stride >= 1 << 23 || v_token_stride < head_dim || v_token_stride >= 1 << 23)
     return hipErrorInvalidValue;
   const WindowAttentionArgs a{q,
                               k,

@@ -253,7 +253,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor | None = N
     if rows == 0:
         return out
     if ((q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 or (q_row | q_head | k_row | k_head | v_row | v_head) & 7
-            or k_row >= 1 << 23 or v_row >= 1 << 23):
+            or not dim <= k_row < 1 << 23 or not dim <= v_row < 1 << 23):
         q, k, v = (x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
         (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
     _run("ivonar_window_attention", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], q_row, q_head,
