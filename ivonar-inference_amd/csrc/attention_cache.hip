@@ -170,7 +170,8 @@ template <int D, bool STREAM>
 __device__ __forceinline__ void load_tile(const uint8_t* base, unsigned to, int lane) {
   const v4u buffer = wide_buffer(base, cache_tile_bytes(D));
 #pragma unroll
-  for (int j = 0; j < Stage<D>::kCodeLoads; ++j) dma<16, STREAM>(buffer, to + j * 1024, lane * 16, j * 1024);
+  for (int j = 0; j < Stage<D>::kCodeLoads; j += 2)
+    dma_pair<STREAM>(buffer, to + j * 1024, 1024, lane * 16, lane * 16, j * 1024, 1024);
 #pragma unroll
   for (int j = 0; j < Stage<D>::kScaleLoads; ++j)
     dma<4, STREAM>(buffer, to + 32 * D + j * 256, lane * 4, 32 * D + j * 256);

@@ -120,7 +120,7 @@ struct Stage {
 };
 
 template <typename T, int D, int KEYS>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void window_attention_kernel(Params p) {
   constexpr int kPieces = D / 8, kSubtiles = KEYS / 32, kDims = D / 32, kLoads = KEYS * kPieces / kThreads;
   typedef typename T::vec vec;
   const WindowAttentionArgs& a = p.a;
@@ -162,17 +162,26 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void window_attention_k
     k_at[j] = row * (int)a.k_strides.token * 2 + (piece ^ k_swizzle<D>(row + j * kStep)) * 16;
     v_at[j] = row * (int)a.v_strides.token * 2 + (piece ^ v_swizzle<D>(row + j * kStep)) * 16;
   }
+  // The next tile to load: its first key, and the addresses and sizes of its rows.
+  int next_key = tile_of(0) * KEYS;
+  const uint16_t *k_next = k0 + next_key * a.k_strides.token, *v_next = v0 + next_key * a.v_strides.token;
+  const int k_row = (int)a.k_strides.token * 2, v_row = (int)a.v_strides.token * 2;
   auto load_tile = [&](int i, int stage) {
-    const int key0 = tile_of(i) * KEYS;
-    const int count = min(KEYS, rows.count - key0);
-    const v4u k_buffer = wide_buffer(k0 + key0 * a.k_strides.token, ((count - 1) * a.k_strides.token + D) * 2);
-    const v4u v_buffer = wide_buffer(v0 + key0 * a.v_strides.token, ((count - 1) * a.v_strides.token + D) * 2);
+    const int before = min(KEYS, rows.count - next_key) - 1;
+    const v4u k_buffer = wide_buffer(k_next, before * k_row + D * 2);
+    const v4u v_buffer = wide_buffer(v_next, before * v_row + D * 2);
+    const unsigned to = lds_address(&stages[stage]) + wave * 1024;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j)
-      dma16(k_buffer, lds_address(stages[stage].k + (j * kThreads + wave * 64) * 16), k_at[j % kPlaces], j * k_step);
+    for (int j = 0; j < kLoads; j += 2)
+      dma_pair<false>(k_buffer, to + j * kThreads * 16, kThreads * 16, k_at[0], k_at[kPlaces - 1], j * k_step, k_step);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j)
-      dma16(v_buffer, lds_address(stages[stage].v + (j * kThreads + wave * 64) * 16), v_at[j % kPlaces], j * v_step);
+    for (int j = 0; j < kLoads; j += 2)
+      dma_pair<false>(v_buffer, to + KEYS * D * 2 + j * kThreads * 16, kThreads * 16, v_at[0], v_at[kPlaces - 1],
+                      j * v_step, v_step);
+    const int keys = i + 1 == sink_tiles ? window_tile * KEYS - next_key : KEYS;
+    next_key += keys;
+    k_next += keys * a.k_strides.token;
+    v_next += keys * a.v_strides.token;
   };
 
   load_tile(0, 0);

@@ -61,6 +61,24 @@ __device__ __forceinline__ void dma(v4u buffer, unsigned lds_base, int voffset, 
 #undef IVO_DMA
 }
 
+// Two pieces of 16 bytes per lane from one buffer, `lds_step` and `step` bytes apart in LDS and in memory.
+template <bool STREAM>
+__device__ __forceinline__ void dma_pair(v4u buffer, unsigned lds_base, int lds_step, int voffset0, int voffset1,
+                                         int soffset, int step) {
+  int saved;
+#define IVO_DMA(HINT)                                                                                               \
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, %6 offen" HINT " lds\n\t" \
+               "s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, %7 offen" HINT " lds\n\t"                \
+               "s_mov_b32 m0, %0"                                                                                   \
+               : "=&s"(saved)                                                                                       \
+               : "s"(lds_base), "s"(lds_base + lds_step), "v"(voffset0), "v"(voffset1), "s"(buffer), "s"(soffset),  \
+                 "s"(soffset + step)                                                                                \
+               : "memory")
+  if constexpr (STREAM) IVO_DMA(" nt");
+  if constexpr (!STREAM) IVO_DMA("");
+#undef IVO_DMA
+}
+
 // Waits until at most N of the wave's loads are under way.  A direct load counts until its bytes are in LDS, so the
 // wave itself may read them then; other waves need a barrier as well (direct_load_sync).
 template <int N>
