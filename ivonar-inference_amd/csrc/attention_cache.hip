@@ -284,7 +284,6 @@ __device__ __forceinline__ void clear_rows(const Params& p, int head) {
 
 // Blocks of 4 waves per CU that the registers leave room for (waves per SIMD).
 constexpr int occupancy(int D, int R, int NT) {
-  if (R == 64) return D == 64 && NT == 1 ? 2 : 1;
   if (R == 8 && D == 128) return NT == 1 ? 3 : 2;
   if (R <= 16) return D == 64 ? (NT == 3 ? 3 : 4) : D == 128 ? (NT == 3 ? 2 : 3) : NT == 3 ? 1 : 2;
   return D == 256 || (D == 128 && NT == 3) ? 1 : D == 64 && NT == 1 ? 3 : 2;
@@ -846,19 +845,19 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
 
 constexpr int kUnitsOnDevice = 256;  // CUs
 constexpr int kLeastTiles = 8;       // least share of a block: two tiles per wave
-constexpr int kChunkBlocks = 512;
+constexpr int kChunkBlocks = 384;
 // Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.
 constexpr long long kStreamBytes = 128LL << 20;
 // Row tiles and heads, and their key tiles, at which each goes to one block as a whole.
 constexpr int kWholeUnits = 512, kWholeTiles = 64;
 
-// Rows of a row tile: 8, or a multiple of 16 as the sequences' rows fill on average, within the registers.
+// Rows of a row tile: 8, 16 or 32 as the sequences' rows fill on average, within the registers.  64 rows convert a
+// tile's codes for twice the products, but leave room for one wave per SIMD instead of two: 512 queries over 8702
+// keys, 32/8 heads of 128, took 139 us with them and take 117 (300 over 3000, 16/4 heads: 58 and 44).
 int tile_rows(const CacheAttentionArgs& a) {
   const long long rows = (long long)a.rows * (a.heads / a.kv_heads) / (a.sequences > 0 ? a.sequences : 1);
   if (a.head_dim == 256) return rows <= 16 || a.dtype != kBfloat16 ? 16 : 32;
-  if (rows <= 8) return 8;
-  if (rows <= 16) return 16;
-  return rows <= 32 || a.dtype == kFloat32 ? 32 : 64;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
 }
 
 Params plan(const CacheAttentionArgs& a) {
@@ -923,8 +922,6 @@ hipError_t run_rows(hipStream_t stream, const Params& p) {
   if constexpr (D < 256) {
     if (rows == 8) return run<D, In, 8, NT>(stream, p);
     if (rows == 32) return run<D, In, 32, NT>(stream, p);
-    if constexpr (NT < 3)
-      if (rows == 64) return run<D, In, 64, NT>(stream, p);
   } else if constexpr (NT == 1) {
     if (rows == 32) return run<D, In, 32, NT>(stream, p);
   }
