@@ -28,9 +28,12 @@ holds what is left of the prompt, since a tile's 194 dependent launches (24
 layers) cost little more at many tokens than at few (3.4 us each at 32, 4.4 at
 128, 5.9 at 256, 11 at 1024).
 
-The mixers (recurrent scan, latent attention) are not part of this path: the
-output projection reads the V third of the entry projection's output instead
-of a mixer's output.  Greedy tokens are written on the device into a ring of
+The reference's mixers (recurrent scan, latent attention) are not part of this path: without ``attention``
+the output projection reads the V third of the entry projection's output instead
+of a mixer's output.  With ``attention`` (an ``AttentionConfig``) the thirds are the queries, keys and values
+of causal self-attention, with a sliding window and sinks if it has them: a decode step writes its token's keys and
+values into a 4-bit cache and attends to the cache; a prompt's first tile attends to its own keys and values as they
+are, in bfloat16, and later tiles to the cache.  Greedy tokens are written on the device into a ring of
 ``burst`` slots, so a burst of decode steps runs as one HIP graph replay with
 a single read-back, as the reference's burst graphs do (``kernel_decoder.py:694-735``).
 """
@@ -39,10 +42,12 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from functools import partial
 
 import numpy as np
 import torch
 
+from . import attention as attn
 from . import runtime
 from .matrix import Matrix, _lanes_for
 from .quantization import TernaryLinear
@@ -74,6 +79,67 @@ def _linear(layer) -> TernaryLinear:
 
 
 @dataclass
+class AttentionConfig:
+    """Self-attention between the entry and the output projection: `heads` heads (hidden / heads one of
+    attention.HEAD_DIMS), the last `window` tokens (0: all) and the first `sinks` visible, a cache of `capacity`
+    tokens."""
+
+    heads: int
+    window: int = 0
+    sinks: int = 0
+    capacity: int = 4096
+    page_size: int = 64
+
+
+class _Attention:
+    """The caches of a decoder's layers and the buffers that its attention calls read and write."""
+
+    def __init__(self, config: AttentionConfig, hidden: int, layers: int, longest: int, device: torch.device) -> None:
+        if config.heads <= 0 or hidden % config.heads or hidden // config.heads not in attn.HEAD_DIMS:
+            raise KernelError(f"{config.heads} heads do not divide {hidden} into one of {attn.HEAD_DIMS}")
+        if config.capacity <= 0:
+            raise KernelError("the cache needs room for at least one token")
+        self.config, self.shape = config, (config.heads, hidden // config.heads)
+        pages = -(-config.capacity // config.page_size)
+        self.pages = [attn.cache_pages(pages, *self.shape, config.page_size, device) for _ in range(layers)]
+        self.table = torch.arange(pages, dtype=torch.int32, device=device).reshape(1, pages)
+        # decode: the tokens before the step's and with it; a prompt's tile: the same, and the rows before and after it
+        self.step_index = torch.tensor([0, 1], dtype=torch.int32, device=device)
+        self.tile_index = torch.zeros(4, dtype=torch.int32, device=device)
+        self.mixed = torch.zeros(hidden, dtype=torch.float32, device=device)
+        self.mixed_tile = torch.zeros(longest, hidden, dtype=torch.float32, device=device)
+        self.half_tile = torch.zeros(longest, 3 * hidden, dtype=torch.bfloat16, device=device)
+        self.half_out = torch.zeros(longest, hidden, dtype=torch.bfloat16, device=device)
+        self.tokens = 0  # in the cache
+
+    def _thirds(self, rows: torch.Tensor):
+        return rows.unflatten(1, (3, *self.shape)).unbind(1)
+
+    def _cached(self, layer: int, rows: torch.Tensor, past, lengths, offsets, out: torch.Tensor) -> None:
+        q, k, v = self._thirds(rows)
+        attn.cache_write(self.pages[layer], k, v, self.table, past, offsets)
+        attn.cache_attention(q, self.pages[layer], self.table, lengths, offsets, self.config.window, self.config.sinks,
+                             max_length=self.config.capacity, out=out.unflatten(1, self.shape))
+
+    def step(self, layer: int, mixer_in: torch.Tensor) -> None:
+        self._cached(layer, mixer_in.unsqueeze(0), self.step_index[:1], self.step_index[1:], None,
+                     self.mixed.unsqueeze(0))
+
+    def tile(self, layer: int, mixer_in: torch.Tensor, first: bool) -> None:
+        rows, index = mixer_in.shape[0], self.tile_index
+        if not first:
+            self._cached(layer, mixer_in, index[:1], index[1:2], index[2:], self.mixed_tile[:rows])
+            return
+        _, k, v = self._thirds(mixer_in)
+        attn.cache_write(self.pages[layer], k, v, self.table, index[:1], index[2:])
+        half, out = self.half_tile[:rows], self.half_out[:rows]
+        half.copy_(mixer_in)
+        attn.window_attention(*self._thirds(half), index[2:], self.config.window, self.config.sinks,
+                              out=out.unflatten(1, self.shape))
+        self.mixed_tile[:rows].copy_(out)
+
+
+@dataclass
 class _LayerOps:
     entry: Matrix
     out: Matrix
@@ -98,7 +164,7 @@ class _TorchOp:
 
 class StackDecoder:
     def __init__(self, weights: LinearStackWeights, device: str | torch.device = "cuda", burst: int = BURST,
-                 sampling: bool = False, max_top_k: int = 256) -> None:
+                 sampling: bool = False, max_top_k: int = 256, attention: AttentionConfig | None = None) -> None:
         device = torch.device(device)
         if device.type != "cuda":
             raise KernelError("the ternary decoder needs a ROCm device")
@@ -146,6 +212,7 @@ class StackDecoder:
         self.q8_tile = torch.zeros(longest, max_chunks * CHUNK, dtype=torch.int8, device=device)
         self.xsum_tile = torch.zeros(longest, max_chunks, dtype=torch.int32, device=device)
         self.scale_tile = torch.zeros(longest, **f32)
+        self.attention = None if attention is None else _Attention(attention, hidden, len(self.layers), longest, device)
         # The head is one GEMV with the RMSNorm prologue fused (the reference runs quantize_norm and
         # gemv_prequant_store, kernel_decoder.py:265-267; the logits are the same bits either way).
         self._head = [self._gemv("gemv_norm_store", self.token_matrix, self.residual, self.final_norm, self.logits,
@@ -153,9 +220,12 @@ class StackDecoder:
         layers = self._build_layers()
         self._steps = [self._build_step(slot, layers) for slot in range(self.burst)]
         self._tiles = self._build_tiles()
+        self._later_tiles = self._tiles if self.attention is None else self._build_tiles(first=False)
         self._first = self._head + self._select(self.burst - 1)  # after the last tile
         self._graph: torch.cuda.CUDAGraph | None = None
-        self._tile_graph: dict[int, torch.cuda.CUDAGraph] | None = None  # one per tile size
+        # one per tile size, of a prompt's first tile and (the same without attention) of its later ones
+        self._tile_graph: dict[int, torch.cuda.CUDAGraph] | None = None
+        self._later_tile_graph: dict[int, torch.cuda.CUDAGraph] | None = None
         self.position = 0
 
     # ------------------------------------------------------------------ launch builders
@@ -232,10 +302,12 @@ class StackDecoder:
         config = self.config
         hidden = config.hidden
         launches = []
-        values = self.mixer_in.narrow(0, 2 * hidden, hidden)
-        for ops in self.layers:
+        values = self.mixer_in.narrow(0, 2 * hidden, hidden) if self.attention is None else self.attention.mixed
+        for index, ops in enumerate(self.layers):
             launches.append(self._gemv("gemv_norm_store", ops.entry, self.residual, ops.mixer_norm, self.mixer_in,
                                        eps=config.eps))
+            if self.attention is not None:
+                launches.append(_TorchOp(partial(self.attention.step, index, self.mixer_in)))
             launches.append(self._gemv("gemv_plain_residual", ops.out, values, None, self.residual))
             launches.append(self._gemv("gemv_norm_silu_pair", ops.gate_up, self.residual, ops.ffn_norm,
                                        self.ffn_mid, eps=config.eps))
@@ -250,11 +322,13 @@ class StackDecoder:
         embed = Launch(self.module.kernel("embed_token"), ((hidden + THREADS - 1) // THREADS, 1, 1), (THREADS, 1, 1),
                        [pointer(previous), pointer(token.packed), pointer(token.scales), pointer(self.residual),
                         int32(hidden), int32(token.row_bytes), int32(token.groups)])
-        return [embed, *layers, *self._head, *self._select(slot)]
+        advance = [] if self.attention is None else [_TorchOp(partial(self.attention.step_index.add_, 1))]
+        return [embed, *layers, *advance, *self._head, *self._select(slot)]
 
-    def _build_tiles(self) -> dict[int, list[Launch]]:
+    def _build_tiles(self, first: bool = True) -> dict[int, list[Launch]]:
         """Per tile size: one prefill tile of up to that many tokens, ending with its last valid token's
-        residual in ``self.residual``.  The sizes share every argument but the token count."""
+        residual in ``self.residual``.  The sizes share every argument but the token count.  With attention a
+        prompt's first tile differs from the later ones, which attend to the cache."""
         config = self.config
         hidden, dense, qkv = config.hidden, config.dense, config.qkv
         token = self.token_matrix
@@ -263,11 +337,20 @@ class StackDecoder:
         blocks = (hidden + THREADS - 1) // THREADS
         steps = [lambda tokens: Launch(self.module.kernel("embed_tile"), (blocks, tokens, 1), (THREADS, 1, 1),
                                        [*embed, int32(tokens)])]
-        values = self.mixer_in_tile.narrow(1, 2 * hidden, hidden)
-        for ops in self.layers:
+        attention = self.attention
+        values, stride = self.mixer_in_tile.narrow(1, 2 * hidden, hidden), qkv
+        if attention is not None:
+            values, stride = attention.mixed_tile, hidden
+
+        def attend(index: int):
+            return lambda tokens: _TorchOp(partial(attention.tile, index, self.mixer_in_tile[:tokens], first))
+
+        for index, ops in enumerate(self.layers):
             steps.append(self._quantize_tile(MODE_NORM, self.residual_tile, hidden, hidden, ops.mixer_norm, config.eps))
             steps.append(self._gemm_tile("gemm_tile_store", ops.entry, self.mixer_in_tile, qkv))
-            steps.append(self._quantize_tile(MODE_PLAIN, values, hidden, qkv))
+            if attention is not None:
+                steps.append(attend(index))
+            steps.append(self._quantize_tile(MODE_PLAIN, values, hidden, stride))
             steps.append(self._gemm_tile("gemm_tile_residual", ops.out, self.residual_tile, hidden))
             steps.append(self._quantize_tile(MODE_NORM, self.residual_tile, hidden, hidden, ops.ffn_norm, config.eps))
             steps.append(self._gemm_tile("gemm_tile_silu_pair", ops.gate_up, self.ffn_tile, dense))
@@ -296,6 +379,10 @@ class StackDecoder:
             raise ValueError("the prompt must not be empty")
         if int(ids.min()) < 0 or int(ids.max()) >= self.config.vocab:
             raise IndexError(f"token id is out of range for vocab_size={self.config.vocab}")
+        attention = self.attention
+        if attention is not None:
+            attention.tokens = 0
+            self._reserve(length)
         host, start = self._tile_host, 0
         while start < length:
             count = min(length - start, TILES[-1])
@@ -304,18 +391,32 @@ class StackDecoder:
             host[1:1 + count] = ids[start:start + count]
             host[1 + count:1 + tokens] = 0
             self.tile_input[:1 + tokens].copy_(host[:1 + tokens])
-            if self._tile_graph is not None:
-                self._tile_graph[tokens].replay()  # one replay per tile (kernel_decoder.py:444-447)
+            if attention is not None:
+                attention.tile_index.copy_(torch.tensor([start, start + count, 0, count], dtype=torch.int32))
+            if self._tile_graph is not None:  # one replay per tile (kernel_decoder.py:444-447)
+                (self._later_tile_graph if start else self._tile_graph)[tokens].replay()
             else:
-                self._run(self._tiles[tokens])
+                self._run((self._later_tiles if start else self._tiles)[tokens])
             start += count
+        if attention is not None:
+            attention.step_index.copy_(torch.tensor([length, length + 1], dtype=torch.int32))
         self._run(self._first)
         self.position = 0
         return self.logits
 
+    def _reserve(self, count: int) -> None:
+        """Counts `count` tokens into the cache, which must have room for them."""
+        attention = self.attention
+        if attention is None:
+            return
+        if attention.tokens + count > attention.config.capacity:
+            raise ValueError(f"the cache holds {attention.config.capacity} tokens, not {attention.tokens + count}")
+        attention.tokens += count
+
     @torch.no_grad()
     def step(self) -> None:
         """One eager greedy step: consumes the last token, appends the next one to the ring."""
+        self._reserve(1)
         self._run(self._steps[self.position % self.burst])
         self.position += 1
 
@@ -331,6 +432,8 @@ class StackDecoder:
             raise KernelError("capture at a burst boundary")
         saved = self.history.clone()
         seen = None if self.sampler is None else self.sampler.seen.clone()
+        # The warm-up's tokens go behind the cache's, which overwrites them later.
+        index = None if self.attention is None else self.attention.step_index.clone()
         stream = torch.cuda.Stream(device=self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(stream):
@@ -341,6 +444,8 @@ class StackDecoder:
         self.history.copy_(saved)
         if seen is not None:
             self.sampler.seen.copy_(seen)
+        if index is not None:
+            self.attention.step_index.copy_(index)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             for slot in range(self.burst):
@@ -350,19 +455,23 @@ class StackDecoder:
         if seen is not None:
             self.sampler.seen.copy_(seen)
         self._graph = graph
-        self._tile_graph = self._capture_tiles(stream)
+        self._tile_graph = self._later_tile_graph = self._capture_tiles(stream, self._tiles)
+        if self._later_tiles is not self._tiles:
+            self._later_tile_graph = self._capture_tiles(stream, self._later_tiles)
         return True
 
-    def _capture_tiles(self, stream: torch.cuda.Stream) -> dict[int, torch.cuda.CUDAGraph]:
+    def _capture_tiles(self, stream: torch.cuda.Stream, tiles: dict[int, list]) -> dict[int, torch.cuda.CUDAGraph]:
         residual, valid = self.residual.clone(), self.tile_valid.clone()
         self.tile_valid.fill_(TILE)
+        if self.attention is not None:
+            self.attention.tile_index.zero_()  # no rows: the warm-up leaves the cache as it is
         stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(stream):
-            self._run(self._tiles[TILE])
+            self._run(tiles[TILE])
         torch.cuda.current_stream(self.device).wait_stream(stream)
         torch.cuda.synchronize(self.device)
         graphs = {}
-        for tokens, launches in self._tiles.items():
+        for tokens, launches in tiles.items():
             graphs[tokens] = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graphs[tokens], stream=stream):
                 self._run(launches)
@@ -378,6 +487,7 @@ class StackDecoder:
         tokens: list[int] = []
         sampling = self.sampler is not None
         while count - len(tokens) >= self.burst and self._graph is not None and self.position % self.burst == 0:
+            self._reserve(self.burst)
             self._graph.replay()
             self.position += self.burst
             tokens.extend(self.history.tolist())
@@ -397,6 +507,9 @@ class StackDecoder:
         self.history.zero_()
         if self.sampler is not None:
             self.sampler.seen.zero_()
+        if self.attention is not None:
+            self.attention.tokens = 0
+            self.attention.step_index.copy_(torch.tensor([0, 1], dtype=torch.int32))
 
     @torch.no_grad()
     def self_check(self) -> None:
