@@ -44,7 +44,7 @@ extern "C" {
  * quantize itself: NORM and ATTN rows, unaligned PLAIN rows, rows above
  * 32768 inputs), the 16 MB of fp32 wave chains of a K-sliced token GEMM
  * (1..16 tokens whose q8 rows exceed LDS) with its per-group arrival counts,
- * and the argmax's block count.
+ * the cache attention's arrival counts and the argmax's block count.
  * Besides it, every stream that makes such a call outside graph capture
  * gets a scratch of its own (about 17 MB, kept until the process ends) on
  * its first call, so eager calls on different streams never share one; a
@@ -53,8 +53,9 @@ extern "C" {
  * whatever thread calls.  Call once per device outside graph capture;
  * replaces the reference's compile_module set-up step
  * (kernels/runtime.py:301-324).  Calls with the device current.  Calling it
- * again clears the arrival counts (argmax, K-sliced token GEMV) of every
- * scratch of the device, with no call of the device in flight. */
+ * again clears the arrival counts (argmax, K-sliced token GEMV, cache
+ * attention) of every scratch of the device, with no call of the device in
+ * flight. */
 hipError_t ivonar_init(int device);
 
 /* Process-wide values the reference passes as -D defines to NVRTC
@@ -282,7 +283,9 @@ hipError_t ivonar_cache_read(hipStream_t stream, const uint8_t* pages, int page_
  * (0: none) only the last `window` of them and the first `sinks` of the sequence.  A row that sees nothing is 0, and
  * so are rows of no sequence.  scale > 0 multiplies q . k.  max_length: about the longest length; it sets how the keys
  * are shared between blocks, not the result's validity.  work: ivonar_cache_attention_work bytes (same arguments; the
- * sizes alone decide, offsets is only tested for NULL; -1 for sizes that the call refuses), 16-byte aligned. */
+ * sizes alone decide, offsets is only tested for NULL; -1 for sizes that the call refuses), 16-byte aligned; calls
+ * that may overlap need one each.  Where several blocks share a row's keys they count each other in the stream's
+ * scratch (see ivonar_init, with the same concurrency rule as the GEMV's). */
 long long ivonar_cache_attention_work(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
                                       int sequences, int rows, int window, int sinks, int max_length);
 hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, long long q_token_stride,

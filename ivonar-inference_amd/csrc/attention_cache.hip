@@ -16,8 +16,10 @@
 // into two or, for fp32 rows, three: a single term of P would leave errors of 2^-8 of sum p |v|, as much as the
 // rounding of a bf16 result that does not cancel.
 //
-// The waves of a block take the tiles of its share of the keys in turn and add their results through LDS; few rows
-// and many keys are split over several blocks, whose results (unscaled sums, m, sum) a second kernel adds.
+// The waves of a block take the tiles of its share of the keys in turn and add their results through LDS.  The keys of
+// all sequences are dealt out evenly to as many blocks as the device holds; where that cuts a row tile's keys, the last
+// of its blocks to end adds the parts (unscaled sums, m, sum).  Row tiles of long chunks, of which there are many more,
+// are split at equal lengths if at all, and a second kernel adds their parts.
 #include "buffer_ops.hpp"
 #include "cache_layout.hpp"
 #include "ternary_device.hpp"
@@ -38,7 +40,8 @@ struct Params {
   int blocks;    // of each head
   float scale;   // log2(e) * scale
   bool aligned;  // q's rows start on 16 bytes
-  bool stream;   // the cache is read past the caches that outlive the call
+  bool stream;   // the cache is loaded past the memory-side cache
+  unsigned* counters;  // of dealt out row tiles, by their first block: the parts that have arrived
 };
 
 // A row tile of a sequence and the key tiles that its rows see: [0, sink_tiles) and [window_tile, ..), at least one.
@@ -118,8 +121,9 @@ __device__ __forceinline__ bool span_of(const Params& p, int slot, Span& s) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The key tiles of all sequences in a row: sequence by sequence, its row tiles in order.  A block takes `share` neighbouring ones of them for one head, so that blocks end together whatever the
-// lengths are, and the heads' blocks, which start together, read the heads' parts of a page at about the same time.
+// The key tiles of all sequences in a row: sequence by sequence, its row tiles in order.  A block takes `share`
+// neighbouring ones of them for one head, so that blocks end together whatever the lengths are, and the heads' blocks,
+// which start together, read the heads' parts of a page at about the same time.
 template <int R>
 __device__ __forceinline__ long long tiles_of(const Params& p, int sequence) {
   if (sequence >= p.a.sequences) return 0;
@@ -193,8 +197,8 @@ __device__ __forceinline__ void read_words(const unsigned char* at, unsigned* to
   }
 }
 
-// A lane's keys and values of a tile in LDS.  Of up to 8 rows (NARROW) lane (n, b) takes half a row of key 16 (b / 2) + n,
-// else a quarter of the rows of keys n and 16 + n.
+// A lane's keys and values of a tile in LDS.  Of up to 8 rows (NARROW) lane (n, b) takes half a row of key
+// 16 (b / 2) + n, else a quarter of the rows of keys n and 16 + n.
 template <int D, bool NARROW>
 __device__ __forceinline__ void read_tile(const unsigned char* base, int lane, Tile<D>& t) {
   constexpr int W = D / 32;
@@ -284,7 +288,7 @@ __device__ __forceinline__ void clear_rows(const Params& p, int head) {
 
 // Blocks of 4 waves per CU that the registers leave room for (waves per SIMD).
 constexpr int occupancy(int D, int R, int NT) {
-  if (R == 8 && D == 128) return NT == 1 ? 3 : 2;
+  if (R == 8) return D == 128 ? (NT == 1 ? 3 : 2) : NT == 1 ? 4 : 3;
   if (R <= 16) return D == 64 ? (NT == 3 ? 3 : 4) : D == 128 ? (NT == 3 ? 2 : 3) : NT == 3 ? 1 : 2;
   return D == 256 || (D == 128 && NT == 3) ? 1 : D == 64 && NT == 1 ? 3 : 2;
 }
@@ -308,17 +312,19 @@ __device__ __forceinline__ long long tiles_up_to(const Params& p, int base) {
 // A run of key tiles of one row tile: tiles begin .. of the row tile at row `start` of the sequence.
 struct Run {
   int sequence, start, begin;
+  long long at;  // the run's first tile among all of them
 };
 
 // Where a share of all key tiles begins, and how many tiles it has.
 template <int R>
-__device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run, long long& left) {
+__device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run, long long& left, long long& share) {
   const CacheAttentionArgs& a = p.a;
   long long sum = tiles_up_to<R>(p, 0);
   const long long all = a.sequences <= 64 ? uniform(__shfl(sum, 63)) : tiles_before<R>(p, a.sequences);
-  const long long share = share_of(p, all);
+  share = share_of(p, all);
   long long at = block * share;
   if (at >= all) return false;
+  run.at = at;
   left = min(share, all - at);
   int base = 0;
   for (;;) {
@@ -343,6 +349,97 @@ __device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run
   }
 }
 
+// Adds the parts of a row (sums relative to a part's maximum, and the maximum and sum of the weights): a thread takes
+// four dims and every `groups`-th part of them, in their order, several on their way at a time.  `first`, then `second`
+// and from there on `step` apart: the parts' numbers.
+struct RowSum {
+  float4 sum;
+  float top, total;
+};
+__device__ __forceinline__ void add_scaled(RowSum& to, const float4& v, float factor) {
+  to.sum.x += v.x * factor;
+  to.sum.y += v.y * factor;
+  to.sum.z += v.z * factor;
+  to.sum.w += v.w * factor;
+}
+template <int D, int R>
+__device__ __forceinline__ RowSum add_row(int line, int lane, int groups, int group, const float* work, long long first,
+                                          long long second, int step, int parts) {
+  constexpr int kPart = R * (D + 2), kAtOnce = 8;
+  RowSum to{float4{0.0f, 0.0f, 0.0f, 0.0f}, kNoKey, 0.0f};
+  for (int base = group; base < parts; base += groups * kAtOnce) {
+    float tops[kAtOnce], weights[kAtOnce];
+    float2 low[kAtOnce], high[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = min(base + k * groups, parts - 1);
+      const float* from = work + (i == 0 ? first : second + (long long)(i - 1) * step) * kPart;
+      const unsigned long long* values = reinterpret_cast<const unsigned long long*>(from + line * D + lane * 4);
+      tops[k] = load_device(from + R * D + 2 * line);
+      weights[k] = load_device(from + R * D + 2 * line + 1);
+      low[k] = bits_as<float2>(load_device(values));
+      high[k] = bits_as<float2>(load_device(values + 1));
+    }
+    float top = to.top;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, tops[k]);
+    const float before = __builtin_amdgcn_exp2f(to.top - top);
+    to = RowSum{float4{to.sum.x * before, to.sum.y * before, to.sum.z * before, to.sum.w * before}, top,
+                to.total * before};
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (base + k * groups >= parts) break;
+      const float factor = __builtin_amdgcn_exp2f(tops[k] - top);
+      to.total += weights[k] * factor;
+      add_scaled(to, float4{low[k].x, low[k].y, high[k].x, high[k].y}, factor);
+    }
+  }
+  return to;
+}
+template <int D, typename In>
+__device__ __forceinline__ void store_row(const Params& p, const Span& s, int head, int line, int lane,
+                                          const RowSum& from) {
+  const float inverse = from.total == 0.0f ? 0.0f : 1.0f / from.total;
+  const float4 sum = from.sum;
+  const int row = s.start + line, token = row / p.group, h = row - token * p.group;
+  In* to = static_cast<In*>(p.a.out) + ((long long)(s.row0 + token) * p.a.heads + head * p.group + h) * D + lane * 4;
+  store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
+}
+
+// All rows of a row tile by one block: D / 4 threads per row and group of parts.  room: 6 floats per thread.
+template <int D, typename In, int R>
+__device__ __forceinline__ void add_parts(const Params& p, const Span& s, int head, const float* work, long long first,
+                                          long long second, int step, int parts, float* room) {
+  constexpr int kLanes = D / 4, kTeams = kThreads / kLanes;
+  const int lane = threadIdx.x % kLanes, team = (int)threadIdx.x / kLanes;
+  const int rows = min(R, s.rows - s.start);
+  // Teams per row, a power of two, as many as parts can use.
+  int groups = 1;
+  while (groups * 2 * rows <= kTeams && groups * 2 <= parts) groups *= 2;
+  float4* sums = reinterpret_cast<float4*>(room);
+  float2* stats = reinterpret_cast<float2*>(room + 4 * kThreads);
+  for (int base = 0; base < rows; base += kTeams / groups) {
+    const int line = min(base + team / groups, rows - 1), group = team % groups;
+    const RowSum mine = add_row<D, R>(line, lane, groups, group, work, first, second, step, parts);
+    __syncthreads();
+    sums[threadIdx.x] = mine.sum;
+    stats[threadIdx.x] = float2{mine.top, mine.total};
+    __syncthreads();
+    if (group == 0 && base + team / groups < rows) {
+      float top = mine.top;
+      for (int k = 1; k < groups; ++k) top = fmaxf(top, stats[threadIdx.x + k * kLanes].x);
+      RowSum all{float4{0.0f, 0.0f, 0.0f, 0.0f}, top, 0.0f};
+      for (int k = 0; k < groups; ++k) {
+        const float2 part = stats[threadIdx.x + k * kLanes];
+        const float factor = __builtin_amdgcn_exp2f(part.x - top);
+        all.total += part.y * factor;
+        add_scaled(all, sums[threadIdx.x + k * kLanes], factor);
+      }
+      store_row<D, In>(p, s, head, line, lane, all);
+    }
+  }
+}
+
 template <int D, typename In, int R, int NT, bool STREAM>
 __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention_kernel(Params p) {
   constexpr bool kNarrow = R == 8;
@@ -360,12 +457,13 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
   Room& room = *reinterpret_cast<Room*>(room_bytes);
   auto& sums = room.sums;
   __shared__ float stats[2][kWaves][16 * RT];
+  __shared__ unsigned arrived;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool shared = p.splits == 0;
 
   // The block's runs of tiles: one, or as many as its share of all tiles has; and where the first one's result goes.
   Run run;
-  long long left = 0;
+  long long left = 0, share = 0;
   long long part;
   const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
   if (shared) {
@@ -373,7 +471,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
       clear_rows<D, In>(p, head);
       return;
     }
-    if (!share_begin<R>(p, unit, run, left)) return;
+    if (!share_begin<R>(p, unit, run, left, share)) return;
     part = 2LL * unit * a.kv_heads + head;
   } else {
     const int split = unit % p.splits, slot = unit / p.splits;
@@ -429,8 +527,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
     if (i < end) page = page_of(min(i + (kStages - 1) * kWaves, last));
     int stage = 0;
     // q as the B operand.  Row n of row tile rt, dims 8 (b W + c) + j; of up to 8 rows, row n % 8 and dims
-    // (b % 2) D / 2 + 8 c + j, where the keys b / 2 = n / 8, and zero elsewhere: columns 0 .. 7 of the product are then the
-    // rows with the tile's first 16 keys, columns 8 .. 15 with its others, so that every lane has logits of its own.
+    // (b % 2) D / 2 + 8 c + j, where the keys b / 2 = n / 8, and zero elsewhere: columns 0 .. 7 of the product are then
+    // the rows with the tile's first 16 keys, columns 8 .. 15 with its others, so that every lane has logits of its own.
     bf16x8 q[RT][NT][kChunks];
     int position[RT];
 #pragma unroll
@@ -473,7 +571,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
         wait_loads<0>();
       // The stage of the tile before this one, which has been used, takes the next tile.
       if (i + (kStages - 1) * kWaves <= last) {
-        there |= (unsigned)load(i + (kStages - 1) * kWaves, page, stage == 0 ? kStages - 1 : stage - 1) << (kStages - 1);
+        const int free = stage == 0 ? kStages - 1 : stage - 1;
+        there |= (unsigned)load(i + (kStages - 1) * kWaves, page, free) << (kStages - 1);
         page = page_of(min(i + kStages * kWaves, last));
       }
       Tile<D> t;
@@ -505,7 +604,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
         f32x4 upper = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // of up to 8 rows, a second chain of products
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          const float scale = kNarrow ? scale_operand(t.k_scale[c / 4], 0) : scale_operand(t.k_scale[W == 8 ? c / 4 : 0], h);
+          const float scale =
+              kNarrow ? scale_operand(t.k_scale[c / 4], 0) : scale_operand(t.k_scale[W == 8 ? c / 4 : 0], h);
           u32x4 words;
 #pragma unroll
           for (int j = 0; j < 4; ++j) words[j] = convert(t.k[h * W + c], scale, j);
@@ -578,7 +678,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
       }
 
       // The weights as the B operand: row n, keys 4 b + r and 16 + 4 b + r in elements r and 4 + r.  Of up to 8 rows,
-      // columns 0 .. 7 take the first terms of a row's weights and columns 8 .. 15 the second ones, for all of its keys.
+      // columns 0 .. 7 take the first terms of a row's weights and columns 8 .. 15 the second ones, for all of its
+      // keys.
       constexpr int kOperands = kNarrow ? NP / 2 + NP % 2 : NP;
       bf16x8 weights[RT][kOperands];
 #pragma unroll
@@ -642,7 +743,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
 #pragma unroll
           for (int z = 0; z < kOperands; ++z) {
             o[2 * w][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value0, weights[rt][z], o[2 * w][rt], 0, 0, 0);
-            o[2 * w + 1][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value1, weights[rt][z], o[2 * w + 1][rt], 0, 0, 0);
+            o[2 * w + 1][rt] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(value1, weights[rt][z], o[2 * w + 1][rt], 0, 0, 0);
           }
       }
 
@@ -701,7 +803,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
 #pragma unroll
         for (int k = 0; k < kTiles; k += 4)
           *reinterpret_cast<float4*>(&sums[wave][n][kTiles * (4 * b + r) + k]) =
-              float4{o[k][rt][r] * factor, o[k + 1][rt][r] * factor, o[k + 2][rt][r] * factor, o[k + 3][rt][r] * factor};
+              float4{o[k][rt][r] * factor, o[k + 1][rt][r] * factor, o[k + 2][rt][r] * factor,
+                     o[k + 3][rt][r] * factor};
       __syncthreads();
       for (int at = thread; at < kLines * D / 4; at += kThreads) {
         const int line = at / (D / 4), column = at % (D / 4) * 4;
@@ -735,15 +838,38 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
           In* to = static_cast<In*>(a.out) + ((long long)(s.row0 + token) * a.heads + head * p.group + h) * D + column;
           store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
         } else {
-          *reinterpret_cast<float4*>(sums_out + (rt * 16 + line) * D + column) = sum;
+          float* to = sums_out + (rt * 16 + line) * D + column;
+          store_device(to, sum.x);
+          store_device(to + 1, sum.y);
+          store_device(to + 2, sum.z);
+          store_device(to + 3, sum.w);
           if (column == 0) {
-            stats_out[2 * (rt * 16 + line)] = top;
-            stats_out[2 * (rt * 16 + line) + 1] = total;
+            store_device(stats_out + 2 * (rt * 16 + line), top);
+            store_device(stats_out + 2 * (rt * 16 + line) + 1, total);
           }
         }
       }
     }
 
+    if (shared && !all) {
+      // The last part of a row tile to arrive adds them all, by the hand-over of store_device (ternary_device.hpp):
+      // nobody waits for anybody.
+      const long long first = uniform(run.at) - begin;  // the row tile's first tile among all
+      const long long first_block = first / share;
+      const int parts = (int)((first + s.total - 1) / share - first_block) + 1;
+      unsigned* counter = p.counters + first_block * a.kv_heads + head;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (arrived == (unsigned)parts - 1) {
+        if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const long long first_part = (2 * first_block + (first == first_block * share ? 0 : 1)) * a.kv_heads + head;
+        const long long second_part = 2 * (first_block + 1) * a.kv_heads + head;
+        add_parts<D, In, R>(p, s, head, a.work, first_part, second_part, 2 * a.kv_heads, parts, &sums[0][0][0]);
+      }
+    }
+    run.at += end - begin;
     left -= end - begin;
     if (left <= 0) return;
     // The next run starts with the first tile of the next row tile or sequence.
@@ -760,87 +886,27 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
   }
 }
 
-// Adds the parts of a row: THREADS threads per row (query token and head), four dims each, so that several parts are
-// read at a time; every thread adds its parts in their order, and the threads' sums are added in theirs.
-template <int D, typename In, int R, int THREADS>
+// Adds the parts of split row tiles: a wave per row (query token and head).
+template <int D, typename In, int R>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
-  constexpr int kLanes = D / 4, kRowsPerBlock = kThreads / THREADS, kAtOnce = THREADS / kLanes, kPart = R * (D + 2);
   const CacheAttentionArgs& a = p.a;
-  __shared__ float4 sums[kThreads];
-  __shared__ float totals[kThreads];
-  const int thread = threadIdx.x % THREADS;
-  const int group_of = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
-  const long long id = (long long)blockIdx.x * kRowsPerBlock + group_of;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long id = (long long)blockIdx.x * kWaves + wave;
   const int row = (int)(id / a.heads), h = (int)(id % a.heads);
   int sequence = 0, index = 0;
-  const bool live = row < a.rows && find_sequence(a.offsets, a.sequences, row, row, sequence, index);
-  bool merging = false;
-  float top = kNoKey, total = 0.0f;
-  float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (live) {
-    const int head = h / p.group, line = index * p.group + h % p.group;
-    int row0;
-    const int queries = rows_of(a, sequence, row0), length = a.lengths[sequence];
-    const Span s = make_span<R>(p, sequence, row0, queries, length, line / R * R);
-    // The parts of this row tile and head are part 0 and then those `step` apart from `second` on.
-    int parts, step;
-    long long part0, second;
-    if (p.splits > 0) {
-      const int first_slot = a.offsets == nullptr ? sequence * ((p.group + R - 1) / R)
-                                                  : (int)((long long)row0 * p.group / R) + sequence;
-      parts = min(p.splits, (s.total + p.chunk - 1) / p.chunk);
-      part0 = (long long)(first_slot + line / R) * p.splits * a.kv_heads + head;
-      second = part0 + a.kv_heads;
-      step = a.kv_heads;
-    } else {
-      const long long share = share_of(p, tiles_before<R>(p, a.sequences));
-      long long begin = tiles_before<R>(p, sequence);
-      for (int start = 0; start < s.start; start += R)
-        begin += make_span<R>(p, sequence, row0, queries, length, start).total;
-      const long long first_block = begin / share;
-      parts = (int)((begin + s.total - 1) / share - first_block) + 1;
-      part0 = (2 * first_block + (begin % share == 0 ? 0 : 1)) * a.kv_heads + head;
-      second = 2 * (first_block + 1) * a.kv_heads + head;
-      step = 2 * a.kv_heads;
-    }
-    merging = parts > 1;  // a single part went to its place at once
-    if (merging) {
-      const float* from = a.work;
-      auto part_of = [&](int i) { return (i == 0 ? part0 : second + (long long)(i - 1) * step) * kPart; };
-      const float* stats = from + R * D + 2 * (line % R);
-      const float* values = from + (line % R) * D + thread % kLanes * 4;
-      for (int i = threadIdx.x & 63; i < parts; i += 64) top = fmaxf(top, stats[part_of(i)]);
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-#pragma unroll 4
-      for (int i = thread / kLanes; i < parts; i += kAtOnce) {
-        const long long at = part_of(i);
-        const float factor = __builtin_amdgcn_exp2f(stats[at] - top);
-        const float4 v = *reinterpret_cast<const float4*>(values + at);
-        total += stats[at + 1] * factor;
-        sum.x += v.x * factor;
-        sum.y += v.y * factor;
-        sum.z += v.z * factor;
-        sum.w += v.w * factor;
-      }
-    }
-  }
-  sums[threadIdx.x] = sum;
-  totals[threadIdx.x] = total;
-  __syncthreads();
-  if (!merging || thread >= kLanes) return;
-#pragma unroll
-  for (int k = 1; k < kAtOnce; ++k) {
-    const float4 v = sums[threadIdx.x + k * kLanes];
-    total += totals[threadIdx.x + k * kLanes];
-    sum.x += v.x;
-    sum.y += v.y;
-    sum.z += v.z;
-    sum.w += v.w;
-  }
-  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-  In* to = static_cast<In*>(a.out) + ((long long)row * a.heads + h) * D + thread * 4;
-  store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
+  if (row >= a.rows || !find_sequence(a.offsets, a.sequences, row, row, sequence, index)) return;
+  const int head = h / p.group, line = index * p.group + h % p.group;
+  int row0;
+  const int queries = rows_of(a, sequence, row0), length = a.lengths[sequence];
+  const Span s = make_span<R>(p, sequence, row0, queries, length, line / R * R);
+  const int parts = min(p.splits, (s.total + p.chunk - 1) / p.chunk);
+  if (parts <= 1) return;  // a single part went to its place at once
+  const int first_slot = a.offsets == nullptr ? sequence * ((p.group + R - 1) / R)
+                                              : (int)((long long)row0 * p.group / R) + sequence;
+  const long long first = (long long)(first_slot + line / R) * p.splits * a.kv_heads + head;
+  const int lane = threadIdx.x % (D / 4);
+  const RowSum sum = add_row<D, R>(line % R, lane, 1, 0, a.work, first, first + a.kv_heads, a.kv_heads, parts);
+  if ((threadIdx.x & 63) < D / 4) store_row<D, In>(p, s, head, line % R, lane, sum);
 }
 
 constexpr int kUnitsOnDevice = 256;  // CUs
@@ -861,9 +927,10 @@ int tile_rows(const CacheAttentionArgs& a) {
 }
 
 Params plan(const CacheAttentionArgs& a) {
-  Params p{a, a.heads / a.kv_heads, 0, 1, 0, 0, 1.44269504088896340736f * a.scale, false, false};
+  Params p{a, a.heads / a.kv_heads, 0, 1, 0, 0, 1.44269504088896340736f * a.scale, false, false, nullptr};
   const int size = a.dtype == kFloat32 ? 4 : 2;
-  p.aligned = (((uintptr_t)a.q | (uintptr_t)(a.q_strides.token * size) | (uintptr_t)(a.q_strides.head * size)) & 15u) == 0;
+  p.aligned =
+      (((uintptr_t)a.q | (uintptr_t)(a.q_strides.token * size) | (uintptr_t)(a.q_strides.head * size)) & 15u) == 0;
   const int R = tile_rows(a);
   const long long rows = (long long)a.rows * p.group;
   p.slots = (int)(a.offsets == nullptr ? (long long)a.sequences * ((p.group + R - 1) / R) : rows / R + a.sequences);
@@ -873,6 +940,7 @@ Params plan(const CacheAttentionArgs& a) {
   const long long tiles = max(1LL, (keys + kCacheTile - 1) / kCacheTile);
   const long long units = (rows / R + (rows % R > 0 || a.offsets == nullptr ? 1 : 0)) * a.kv_heads;
   const int terms = a.dtype == kFloat32 ? 3 : a.dtype == kFloat16 ? 2 : 1;
+  static_assert(4 * kUnitsOnDevice <= kAttentionCounters, "a counter per block");
   const int resident = kUnitsOnDevice * occupancy(a.head_dim, R, terms);
   const long long few = (long long)max(a.sequences, 1) * 4;
   const long long live = max((long long)a.sequences * a.kv_heads, units);
@@ -894,7 +962,8 @@ Params plan(const CacheAttentionArgs& a) {
 template <int D, typename In, int R, int NT>
 hipError_t run(hipStream_t stream, const Params& p) {
   const bool clears = p.a.offsets != nullptr;  // rows of no sequence
-  const long long blocks = ((long long)(p.splits == 0 ? p.blocks : p.slots * p.splits) + (clears ? max(p.splits, 1) : 0)) * p.a.kv_heads;
+  const long long units = p.splits == 0 ? (long long)p.blocks : (long long)p.slots * p.splits;
+  const long long blocks = (units + (clears ? max(p.splits, 1) : 0)) * p.a.kv_heads;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   if (R <= 16 && p.stream)
     hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, R <= 16>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
@@ -902,16 +971,10 @@ hipError_t run(hipStream_t stream, const Params& p) {
   else
     hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
                        p);
-  if (p.splits != 1) {
-    const long long rows = (long long)p.a.rows * p.a.heads;
-    // A whole block per row where rows may have many parts.
-    const bool wide = p.splits > 16 || (p.splits == 0 && p.blocks > 16 * rows / p.a.heads);
-    const long long merges = wide ? rows : (rows + kWaves - 1) / kWaves;
+  if (p.splits > 1) {
+    const long long merges = ((long long)p.a.rows * p.a.heads + kWaves - 1) / kWaves;
     if (merges > 0x7fffffffLL) return hipErrorInvalidValue;
-    if (wide)
-      hipLaunchKernelGGL((merge_kernel<D, In, R, kThreads>), dim3((unsigned)merges), dim3(kThreads), 0, stream, p);
-    else
-      hipLaunchKernelGGL((merge_kernel<D, In, R, 64>), dim3((unsigned)merges), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((merge_kernel<D, In, R>), dim3((unsigned)merges), dim3(kThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
@@ -946,7 +1009,13 @@ long long cache_attention_work(const CacheAttentionArgs& a) {
 
 hipError_t launch_cache_attention(hipStream_t stream, const CacheAttentionArgs& a) {
   if (a.rows == 0) return hipSuccess;
-  const Params p = plan(a);
+  Params p = plan(a);
+  if (p.splits == 0) {
+    Scratch* scratch = nullptr;
+    const hipError_t status = scratch_for_stream(stream, &scratch);
+    if (status != hipSuccess) return status;
+    p.counters = scratch->sync + kAttentionCounterWord;
+  }
   if (a.head_dim == 64) return run_types<64>(stream, p);
   if (a.head_dim == 128) return run_types<128>(stream, p);
   return run_types<256>(stream, p);

@@ -47,8 +47,8 @@ hipError_t allocate_scratch(Scratch& s) {
   if (status == hipSuccess) status = hipMalloc(&xsum, (size_t)kScratchChunks * sizeof(int32_t));
   if (status == hipSuccess) status = hipMalloc(&scale, 256);
   if (status == hipSuccess) status = hipMalloc(&partials, (size_t)kTokenPartialFloats * sizeof(float));
-  if (status == hipSuccess) status = hipMalloc(&sync, kSyncBytes);
-  if (status == hipSuccess) status = hipMemset(sync, 0, kSyncBytes);  // the argmax's block count starts at zero
+  if (status == hipSuccess) status = hipMalloc(&sync, kSyncAllBytes);
+  if (status == hipSuccess) status = hipMemset(sync, 0, kSyncAllBytes);  // the argmax's block count starts at zero
   if (status != hipSuccess) {
     if (q8) (void)hipFree(q8);
     if (xsum) (void)hipFree(xsum);
@@ -205,11 +205,11 @@ hipError_t init_device(int device) {
   status = allocate_scratch(g_scratch[device]);
   // The argmax's block count is zero between launches; clearing it here
   // recovers a scratch that overlapping graph replays left set.
-  if (status == hipSuccess) status = hipMemset(g_scratch[device].sync, 0, kSyncBytes);
+  if (status == hipSuccess) status = hipMemset(g_scratch[device].sync, 0, kSyncAllBytes);
   for (auto it = g_stream_scratch.lower_bound({device, 0}); status == hipSuccess && it != g_stream_scratch.end() &&
                                                              it->first.first == device;
        ++it)
-    status = hipMemset(it->second.sync, 0, kSyncBytes);
+    status = hipMemset(it->second.sync, 0, kSyncAllBytes);
   if (current != device) (void)hipSetDevice(current);
   return status;
 }

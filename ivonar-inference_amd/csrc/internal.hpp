@@ -35,8 +35,9 @@ struct Scratch {
   float* scale = nullptr;
   int capacity_chunks = 0;
   float* token_partials = nullptr;  // fp32 wave partials of the K-sliced token GEMV
-  // Counters that start and end every launch at zero (kSyncBytes): the
-  // argmax's block count and the sliced token GEMV's tile-group arrivals.
+  // Counters that start and end every launch at zero (kSyncAllBytes): the
+  // argmax's block count, the sliced token GEMV's tile-group arrivals and the
+  // cache attention's.
   unsigned* sync = nullptr;
 };
 constexpr int kSyncBytes = 4096;
@@ -46,6 +47,10 @@ constexpr int kArgmaxCountWord = kSyncBytes / 4 - 32;
 // region's words 0 .. kTokenFinishCounters - 1.
 constexpr int kTokenFinishCounters = kArgmaxCountWord;
 static_assert(kTokenFinishCounters == 992, "the default of Defines::token_finish_groups");
+// Behind them, arrival counters of the cache attention's row tiles, as many as blocks share keys at a time.
+constexpr int kAttentionCounterWord = kSyncBytes / 4;
+constexpr int kAttentionCounters = 1024;
+constexpr int kSyncAllBytes = kSyncBytes + kAttentionCounters * 4;
 // Capacity of Scratch::token_partials (floats; 16 MB per device).
 constexpr long long kTokenPartialFloats = 4LL << 20;
 hipError_t scratch_for_stream(hipStream_t stream, Scratch** out);
