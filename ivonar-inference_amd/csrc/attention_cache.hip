@@ -352,6 +352,12 @@ __device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run
 // Adds the parts of a row (sums relative to a part's maximum, and the maximum and sum of the weights): a thread takes
 // four dims and every `groups`-th part of them, in their order, several on their way at a time.  `first`, then `second`
 // and from there on `step` apart: the parts' numbers.
+constexpr int kDeviceScope = 16;  // SC1, the scope bit of store_device and load_device, of the wide buffer forms
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_buffer(float* work) {
+  return __builtin_amdgcn_make_buffer_rsrc(work, 0, 0x7fffffff, 0x00020000);
+}
 struct RowSum {
   float4 sum;
   float top, total;
@@ -363,35 +369,38 @@ __device__ __forceinline__ void add_scaled(RowSum& to, const float4& v, float fa
   to.sum.w += v.w * factor;
 }
 template <int D, int R>
-__device__ __forceinline__ RowSum add_row(int line, int lane, int groups, int group, const float* work, long long first,
-                                          long long second, int step, int parts) {
+__device__ __forceinline__ RowSum add_row(int line, int lane, int groups, int group, __amdgpu_buffer_rsrc_t work,
+                                          long long first, long long second, int step, int parts) {
   constexpr int kPart = R * (D + 2), kAtOnce = 8;
   RowSum to{float4{0.0f, 0.0f, 0.0f, 0.0f}, kNoKey, 0.0f};
   for (int base = group; base < parts; base += groups * kAtOnce) {
-    float tops[kAtOnce], weights[kAtOnce];
-    float2 low[kAtOnce], high[kAtOnce];
+    float2 stats[kAtOnce];
+    float4 values[kAtOnce];
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       const int i = min(base + k * groups, parts - 1);
-      const float* from = work + (i == 0 ? first : second + (long long)(i - 1) * step) * kPart;
-      const unsigned long long* values = reinterpret_cast<const unsigned long long*>(from + line * D + lane * 4);
-      tops[k] = load_device(from + R * D + 2 * line);
-      weights[k] = load_device(from + R * D + 2 * line + 1);
-      low[k] = bits_as<float2>(load_device(values));
-      high[k] = bits_as<float2>(load_device(values + 1));
+      const int at = (int)(i == 0 ? first : second + (i - 1) * step) * kPart * 4;
+      stats[k] = bits_as<float2>(
+          (u32x2)__builtin_amdgcn_raw_buffer_load_b64(work, at + (R * D + 2 * line) * 4, 0, kDeviceScope));
+      values[k] = bits_as<float4>(
+          (u32x4)__builtin_amdgcn_raw_buffer_load_b128(work, at + (line * D + lane * 4) * 4, 0, kDeviceScope));
     }
     float top = to.top;
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, tops[k]);
+    for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, stats[k].x);
     const float before = __builtin_amdgcn_exp2f(to.top - top);
     to = RowSum{float4{to.sum.x * before, to.sum.y * before, to.sum.z * before, to.sum.w * before}, top,
                 to.total * before};
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      if (base + k * groups >= parts) break;
-      const float factor = __builtin_amdgcn_exp2f(tops[k] - top);
-      to.total += weights[k] * factor;
-      add_scaled(to, float4{low[k].x, low[k].y, high[k].x, high[k].y}, factor);
+      // Without a branch, behind which the compiler would load each part by itself.
+      const bool live = base + k * groups < parts;
+      const float factor = __builtin_amdgcn_exp2f(stats[k].x - top);
+      to.total += live ? stats[k].y * factor : 0.0f;
+      to.sum.x += live ? values[k].x * factor : 0.0f;
+      to.sum.y += live ? values[k].y * factor : 0.0f;
+      to.sum.z += live ? values[k].z * factor : 0.0f;
+      to.sum.w += live ? values[k].w * factor : 0.0f;
     }
   }
   return to;
@@ -408,8 +417,8 @@ __device__ __forceinline__ void store_row(const Params& p, const Span& s, int he
 
 // All rows of a row tile by one block: D / 4 threads per row and group of parts.  room: 6 floats per thread.
 template <int D, typename In, int R>
-__device__ __forceinline__ void add_parts(const Params& p, const Span& s, int head, const float* work, long long first,
-                                          long long second, int step, int parts, float* room) {
+__device__ __forceinline__ void add_parts(const Params& p, const Span& s, int head, __amdgpu_buffer_rsrc_t work,
+                                          long long first, long long second, int step, int parts, float* room) {
   constexpr int kLanes = D / 4, kTeams = kThreads / kLanes;
   const int lane = threadIdx.x % kLanes, team = (int)threadIdx.x / kLanes;
   const int rows = min(R, s.rows - s.start);
@@ -788,8 +797,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
     }
     __syncthreads();
     constexpr int kLines = kNarrow ? 8 : 16;
-    float* sums_out = a.work + part * (R * (D + 2));
-    float* stats_out = sums_out + R * D;
+    const int at_part = (int)part * (R * (D + 2)) * 4;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float highest = kNoKey;
@@ -838,15 +846,11 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
           In* to = static_cast<In*>(a.out) + ((long long)(s.row0 + token) * a.heads + head * p.group + h) * D + column;
           store4(to, float4{sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse});
         } else {
-          float* to = sums_out + (rt * 16 + line) * D + column;
-          store_device(to, sum.x);
-          store_device(to + 1, sum.y);
-          store_device(to + 2, sum.z);
-          store_device(to + 3, sum.w);
-          if (column == 0) {
-            store_device(stats_out + 2 * (rt * 16 + line), top);
-            store_device(stats_out + 2 * (rt * 16 + line) + 1, total);
-          }
+          __builtin_amdgcn_raw_buffer_store_b128(bits_as<u32x4>(sum), parts_buffer(a.work),
+                                                 at_part + ((rt * 16 + line) * D + column) * 4, 0, kDeviceScope);
+          if (column == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(bits_as<u32x2>(float2{top, total}), parts_buffer(a.work),
+                                                  at_part + (R * D + 2 * (rt * 16 + line)) * 4, 0, kDeviceScope);
         }
       }
     }
@@ -857,7 +861,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
       const long long first = uniform(run.at) - begin;  // the row tile's first tile among all
       const long long first_block = first / share;
       const int parts = (int)((first + s.total - 1) / share - first_block) + 1;
-      unsigned* counter = p.counters + first_block * a.kv_heads + head;
+      unsigned* counter = p.counters + (first_block * a.kv_heads + head) * kAttentionCounterStep;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -866,7 +870,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
         if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const long long first_part = (2 * first_block + (first == first_block * share ? 0 : 1)) * a.kv_heads + head;
         const long long second_part = 2 * (first_block + 1) * a.kv_heads + head;
-        add_parts<D, In, R>(p, s, head, a.work, first_part, second_part, 2 * a.kv_heads, parts, &sums[0][0][0]);
+        add_parts<D, In, R>(p, s, head, parts_buffer(a.work), first_part, second_part, 2 * a.kv_heads, parts, &sums[0][0][0]);
       }
     }
     run.at += end - begin;
@@ -905,17 +909,24 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
                                               : (int)((long long)row0 * p.group / R) + sequence;
   const long long first = (long long)(first_slot + line / R) * p.splits * a.kv_heads + head;
   const int lane = threadIdx.x % (D / 4);
-  const RowSum sum = add_row<D, R>(line % R, lane, 1, 0, a.work, first, first + a.kv_heads, a.kv_heads, parts);
+  const RowSum sum = add_row<D, R>(line % R, lane, 1, 0, parts_buffer(a.work), first, first + a.kv_heads, a.kv_heads, parts);
   if ((threadIdx.x & 63) < D / 4) store_row<D, In>(p, s, head, line % R, lane, sum);
 }
 
 constexpr int kUnitsOnDevice = 256;  // CUs
-constexpr int kLeastTiles = 8;       // least share of a block: two tiles per wave
+// Blocks that a call's chunks are split into at least, where their row tiles and heads are fewer.
 constexpr int kChunkBlocks = 384;
-// Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.
+// Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.  Loads alone took
+// 64 us for 313 MB with it and 71 without; 22.6 us for 71 MB with it and 18 without.
 constexpr long long kStreamBytes = 128LL << 20;
-// Row tiles and heads, and their key tiles, at which each goes to one block as a whole.
-constexpr int kWholeUnits = 512, kWholeTiles = 64;
+// A block's share of dealt out tiles: a 32nd of a sequence, since a row's parts are read by one block, 32 of them in two
+// turns, but from 8 tiles on (two per wave) and up to 64 (more leave the device half empty).  One sequence, 32/8 heads of
+// 128: 8000 tokens 11.9 us with 8 tiles and 13.4 with 16; 32000 tokens 17.5 with 31, 22.7 with 11; 131000 tokens 35.8
+// with 64, 39.2 with 48 and 37.7 with 43 (as many as fill the device).
+constexpr int kLeastTiles = 8, kMostTiles = 64, kParts = 32;
+// Row tiles and heads, and their key tiles, up to which each is left to one block: handing over the parts costs 5 us.
+// 64 sequences of 4 heads of 64, 36 tiles: 14.5 us so, 25 dealt out; 60 tiles: 17.3 and 22.7.
+constexpr int kWholeUnits = 128, kWholeTiles = 64;
 
 // Rows of a row tile: 8, 16 or 32 as the sequences' rows fill on average, within the registers.  64 rows convert a
 // tile's codes for twice the products, but leave room for one wave per SIMD instead of two: 512 queries over 8702
@@ -945,14 +956,14 @@ Params plan(const CacheAttentionArgs& a) {
   const long long few = (long long)max(a.sequences, 1) * 4;
   const long long live = max((long long)a.sequences * a.kv_heads, units);
   p.stream = live * tiles * cache_tile_bytes(a.head_dim) > kStreamBytes;
-  const bool dealt = rows / R <= few && a.sequences <= 4096 && (tiles > kWholeTiles || live < kWholeUnits) &&
-                     tiles > kLeastTiles;
+  const bool whole = tiles <= kLeastTiles || (tiles <= kWholeTiles && live >= kWholeUnits);
+  const bool dealt = rows / R <= few && a.sequences <= 4096 && !whole;
   if (dealt) {
     p.splits = 0;
-    p.chunk = kLeastTiles;
-    p.blocks = (int)max(1LL, min((long long)resident, (live * tiles + kLeastTiles - 1) / kLeastTiles) / a.kv_heads);
+    p.chunk = (int)max((long long)kLeastTiles, min((long long)kMostTiles, tiles / kParts));
+    p.blocks = (int)max(1LL, min((long long)resident, (live * tiles + p.chunk - 1) / p.chunk) / a.kv_heads);
   } else {
-    const long long wanted = max(1LL, kChunkBlocks / max(1LL, live));
+    const long long wanted = whole ? 1 : max(1LL, kChunkBlocks / max(1LL, live));
     p.chunk = (int)max((long long)kLeastTiles, (tiles + wanted - 1) / wanted);
     p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
   }

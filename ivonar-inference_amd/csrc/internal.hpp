@@ -47,10 +47,11 @@ constexpr int kArgmaxCountWord = kSyncBytes / 4 - 32;
 // region's words 0 .. kTokenFinishCounters - 1.
 constexpr int kTokenFinishCounters = kArgmaxCountWord;
 static_assert(kTokenFinishCounters == 992, "the default of Defines::token_finish_groups");
-// Behind them, arrival counters of the cache attention's row tiles, as many as blocks share keys at a time.
+// Behind them, arrival counters of the cache attention's row tiles, as many as blocks share keys at a time, each in
+// memory lines of its own: the device's counts in one line wait for each other.
 constexpr int kAttentionCounterWord = kSyncBytes / 4;
-constexpr int kAttentionCounters = 1024;
-constexpr int kSyncAllBytes = kSyncBytes + kAttentionCounters * 4;
+constexpr int kAttentionCounters = 1024, kAttentionCounterStep = 64;
+constexpr int kSyncAllBytes = kSyncBytes + kAttentionCounters * kAttentionCounterStep * 4;
 // Capacity of Scratch::token_partials (floats; 16 MB per device).
 constexpr long long kTokenPartialFloats = 4LL << 20;
 hipError_t scratch_for_stream(hipStream_t stream, Scratch** out);
