@@ -9,9 +9,10 @@
 //   S^T [key][row]: A = K (converted from 4 bits with its scales in registers, exact in bf16), B = q;
 //   P = 2^(x - m), which in the MFMA's result layout is already the B operand of
 //   O^T [dim][row] += A = V (converted, then pairs of tokens brought together with v_perm), B = P.
-// Nothing of the cache passes through LDS, no register crosses lanes in the loop besides the maxima, and those only
-// when some value exceeds the running m by a factor of 2^8 (the exponentials stay below 2^8 until then, which fp32
-// and bf16 hold as precisely as values below one).
+// A wave's tiles come straight from memory into a ring of its own in LDS, two or three of them on their way while one
+// is used, so no barrier stands in the loop.  No register crosses lanes in it besides the maxima, and those only when
+// some value exceeds the running m by a factor of 2^8 (the exponentials stay below 2^8 until then, which fp32 and bf16
+// hold as precisely as values below one).
 // q and P are bf16 operands; q in fp16 is split into two bf16 terms and q in fp32 into three (all their bits), and P
 // into two or, for fp32 rows, three: a single term of P would leave errors of 2^-8 of sum p |v|, as much as the
 // rounding of a bf16 result that does not cancel.
@@ -20,6 +21,13 @@
 // all sequences are dealt out evenly to as many blocks as the device holds; where that cuts a row tile's keys, the last
 // of its blocks to end adds the parts (unscaled sums, m, sum).  Row tiles of long chunks, of which there are many more,
 // are split at equal lengths if at all, and a second kernel adds their parts.
+//
+// Measured (MI355X, in graphs).  One token per sequence, bound by the cache's bytes: 64 sequences of about 8000 tokens,
+// 32/8 heads of 128, bf16: 66 us, 4.8 TB/s (a stream of the same 313 MB reads at 6.5; loads alone took 64); one of
+// 131000, fp16: 36.5 us, 3.9 TB/s (142 MB more take 23 us more: the rest is filling the device and adding the parts);
+// 128 with a window of 1024, 16/4 heads of 64: 15 us, 2.4 TB/s; one of 37, fp32: 6.4 us, a chain of loads.  Chunks,
+// bound by the vector units, which convert the codes and the weights next to the matrix units' work: 512 rows over 8702
+// tokens, 32/8 heads of 128, bf16: 119 us, 600 TFLOP/s (900 counting both terms of P).
 #include "buffer_ops.hpp"
 #include "cache_layout.hpp"
 #include "ternary_device.hpp"
@@ -537,7 +545,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
     int stage = 0;
     // q as the B operand.  Row n of row tile rt, dims 8 (b W + c) + j; of up to 8 rows, row n % 8 and dims
     // (b % 2) D / 2 + 8 c + j, where the keys b / 2 = n / 8, and zero elsewhere: columns 0 .. 7 of the product are then
-    // the rows with the tile's first 16 keys, columns 8 .. 15 with its others, so that every lane has logits of its own.
+    // the rows with the tile's first 16 keys, columns 8 .. 15 with its others, so every lane has logits of its own.
     bf16x8 q[RT][NT][kChunks];
     int position[RT];
 #pragma unroll
@@ -870,7 +878,8 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
         if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const long long first_part = (2 * first_block + (first == first_block * share ? 0 : 1)) * a.kv_heads + head;
         const long long second_part = 2 * (first_block + 1) * a.kv_heads + head;
-        add_parts<D, In, R>(p, s, head, parts_buffer(a.work), first_part, second_part, 2 * a.kv_heads, parts, &sums[0][0][0]);
+        add_parts<D, In, R>(p, s, head, parts_buffer(a.work), first_part, second_part, 2 * a.kv_heads, parts,
+                            &sums[0][0][0]);
       }
     }
     run.at += end - begin;
@@ -909,20 +918,21 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
                                               : (int)((long long)row0 * p.group / R) + sequence;
   const long long first = (long long)(first_slot + line / R) * p.splits * a.kv_heads + head;
   const int lane = threadIdx.x % (D / 4);
-  const RowSum sum = add_row<D, R>(line % R, lane, 1, 0, parts_buffer(a.work), first, first + a.kv_heads, a.kv_heads, parts);
+  const RowSum sum =
+      add_row<D, R>(line % R, lane, 1, 0, parts_buffer(a.work), first, first + a.kv_heads, a.kv_heads, parts);
   if ((threadIdx.x & 63) < D / 4) store_row<D, In>(p, s, head, line % R, lane, sum);
 }
 
 constexpr int kUnitsOnDevice = 256;  // CUs
 // Blocks that a call's chunks are split into at least, where their row tiles and heads are fewer.
 constexpr int kChunkBlocks = 384;
-// Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.  Loads alone took
-// 64 us for 313 MB with it and 71 without; 22.6 us for 71 MB with it and 18 without.
+// Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.  Loads alone
+// took 64 us for 313 MB with it and 71 without; 22.6 us for 71 MB with it and 18 without.
 constexpr long long kStreamBytes = 128LL << 20;
-// A block's share of dealt out tiles: a 32nd of a sequence, since a row's parts are read by one block, 32 of them in two
-// turns, but from 8 tiles on (two per wave) and up to 64 (more leave the device half empty).  One sequence, 32/8 heads of
-// 128: 8000 tokens 11.9 us with 8 tiles and 13.4 with 16; 32000 tokens 17.5 with 31, 22.7 with 11; 131000 tokens 35.8
-// with 64, 39.2 with 48 and 37.7 with 43 (as many as fill the device).
+// A block's share of dealt out tiles: a 32nd of a sequence, since a row's parts are read by one block, 32 of them in
+// two turns, but from 8 tiles on (two per wave) and up to 64 (more leave the device half empty).  One sequence, 32/8
+// heads of 128: 8000 tokens 11.9 us with 8 tiles and 13.4 with 16; 32000 tokens 17.5 with 31, 22.7 with 11; 131000
+// tokens 35.8 with 64, 39.2 with 48 and 37.7 with 43 (as many as fill the device).
 constexpr int kLeastTiles = 8, kMostTiles = 64, kParts = 32;
 // Row tiles and heads, and their key tiles, up to which each is left to one block: handing over the parts costs 5 us.
 // 64 sequences of 4 heads of 64, 36 tiles: 14.5 us so, 25 dealt out; 60 tiles: 17.3 and 22.7.
@@ -977,8 +987,8 @@ hipError_t run(hipStream_t stream, const Params& p) {
   const long long blocks = (units + (clears ? max(p.splits, 1) : 0)) * p.a.kv_heads;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   if (R <= 16 && p.stream)
-    hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, R <= 16>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
-                       p);
+    hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, R <= 16>), dim3((unsigned)blocks), dim3(kThreads), 0,
+                       stream, p);
   else
     hipLaunchKernelGGL((cache_attention_kernel<D, In, R, NT, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
                        p);
