@@ -92,6 +92,37 @@ def test_shared_axis(cuda, rng, length, max_length):
     case.run(rng, 4, "bfloat16", queries=[3, 2], max_length=max_length, window=2000, sinks=70)
 
 
+@pytest.mark.parametrize("dim,heads,dtype", [(64, 4, "bfloat16"), (64, 3, "float32"), (128, 4, "float16"),
+                                             (256, 2, "bfloat16")])
+@pytest.mark.parametrize("max_length", [600, 1 << 16])
+def test_many_sequences(cuda, rng, dim, heads, dtype, max_length):
+    """More sequences than lanes, most short and one long: blocks that end one row tile, take whole ones and begin
+    another, or one block for each, by the length that the caller announces."""
+    lengths = [int(n) for n in rng.integers(0, 500, 150)]
+    lengths[3], lengths[70], lengths[149] = 2600, 0, 33
+    case = Case(cuda, rng, lengths, 1, dim, page=32)
+    case.run(rng, heads, dtype, max_length=max_length)
+    queries = [int(n) for n in rng.integers(0, 4, 150)]
+    queries[3], queries[60] = 40, 0
+    case.run(rng, heads, dtype, queries=queries, max_length=max_length)
+
+
+@pytest.mark.parametrize("rows", [8, 12, 30])
+def test_row_tiles_that_share_blocks(cuda, rng, rows):
+    """Row tiles of 8, 16 and 32 rows of few sequences, whose keys begin and end inside blocks."""
+    case = Case(cuda, rng, [1200, 900, 2100], 2, 64)
+    case.run(rng, 2, "bfloat16", queries=[rows, rows - 5, rows + 3], max_length=4000)
+    case.run(rng, 2, "float32", queries=[rows, 0, rows + 9], max_length=4000, window=700, sinks=40)
+
+
+@pytest.mark.parametrize("dim,heads,dtype", [(64, 2, "float32"), (128, 2, "bfloat16"), (256, 1, "float16")])
+def test_long_chunks(cuda, rng, dim, heads, dtype):
+    """Many row tiles, each of whose keys are split at equal lengths."""
+    case = Case(cuda, rng, [3000, 700], 1, dim)
+    case.run(rng, heads, dtype, queries=[611, 10])
+    case.run(rng, heads, dtype, queries=[400, 300], window=1500, sinks=5)
+
+
 def test_more_queries_than_tokens(cuda, rng):
     """Rows before the sequence's first position see nothing and are zero."""
     case = Case(cuda, rng, [3, 0], 1, 64)
