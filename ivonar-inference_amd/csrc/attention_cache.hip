@@ -17,10 +17,10 @@
 // into two or, for fp32 rows, three: a single term of P would leave errors of 2^-8 of sum p |v|, as much as the
 // rounding of a bf16 result that does not cancel.
 //
-// The waves of a block take the tiles of its share of the keys in turn and add their results through LDS.  The keys of
-// all sequences are dealt out evenly to as many blocks as the device holds; where that cuts a row tile's keys, the last
-// of its blocks to end adds the parts (unscaled sums, m, sum).  Row tiles of long chunks, of which there are many more,
-// are split at equal lengths if at all, and a second kernel adds their parts.
+// The waves of a block take the tiles of its share of the keys in turn and add their results through LDS.  Up to 8 rows
+// per sequence: the keys of all sequences are dealt out evenly to as many blocks as the device holds; where that cuts a
+// row tile's keys, the last of its blocks to end adds the parts (unscaled sums, m, sum).  More rows: row tiles are
+// split at equal lengths where there are too few of them, and a second kernel adds their parts.
 //
 // Measured (MI355X, in graphs).  One token per sequence, bound by the cache's bytes: 64 sequences of about 8000 tokens,
 // 32/8 heads of 128, bf16: 66 us, 4.8 TB/s (a stream of the same 313 MB reads at 6.5; loads alone took 64); one of
@@ -924,8 +924,13 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Params p) {
 }
 
 constexpr int kUnitsOnDevice = 256;  // CUs
-// Blocks that a call's chunks are split into at least, where their row tiles and heads are fewer.
-constexpr int kChunkBlocks = 384;
+// Blocks that the row tiles and heads of chunks are split into: as many as the device holds at two per CU.  32/8 heads
+// of 128, 9000 tokens: 16 queries 21.3 us and 27.6 with 768 blocks; 64 queries 29, 34 with 768 and 33 with 384.
+constexpr int kChunkBlocks = 512;
+// Rows per sequence up to which keys are dealt out: the parts of more rows are too much for one block to add.  32/8
+// heads of 128: 4 queries over 2000 tokens 12.4 us dealt out, 10.9 split at equal lengths with a second launch; one
+// query over 9000 12.4 and 17.3.
+constexpr int kFewRows = 8;
 // Cached bytes of a call from which on they are loaded past the memory-side cache: half of its 256 MB.  Loads alone
 // took 64 us for 313 MB with it and 71 without; 22.6 us for 71 MB with it and 18 without.
 constexpr long long kStreamBytes = 128LL << 20;
@@ -934,7 +939,8 @@ constexpr long long kStreamBytes = 128LL << 20;
 // heads of 128: 8000 tokens 11.9 us with 8 tiles and 13.4 with 16; 32000 tokens 17.5 with 31, 22.7 with 11; 131000
 // tokens 35.8 with 64, 39.2 with 48 and 37.7 with 43 (as many as fill the device).
 constexpr int kLeastTiles = 8, kMostTiles = 64, kParts = 32;
-// Row tiles and heads, and their key tiles, up to which each is left to one block: handing over the parts costs 5 us.
+// From so many row tiles and heads on, each with at most so many key tiles is left to one block: handing over the parts
+// costs 5 us.
 // 64 sequences of 4 heads of 64, 36 tiles: 14.5 us so, 25 dealt out; 60 tiles: 17.3 and 22.7.
 constexpr int kWholeUnits = 128, kWholeTiles = 64;
 
@@ -963,11 +969,10 @@ Params plan(const CacheAttentionArgs& a) {
   const int terms = a.dtype == kFloat32 ? 3 : a.dtype == kFloat16 ? 2 : 1;
   static_assert(4 * kUnitsOnDevice <= kAttentionCounters, "a counter per block");
   const int resident = kUnitsOnDevice * occupancy(a.head_dim, R, terms);
-  const long long few = (long long)max(a.sequences, 1) * 4;
   const long long live = max((long long)a.sequences * a.kv_heads, units);
   p.stream = live * tiles * cache_tile_bytes(a.head_dim) > kStreamBytes;
   const bool whole = tiles <= kLeastTiles || (tiles <= kWholeTiles && live >= kWholeUnits);
-  const bool dealt = rows / R <= few && a.sequences <= 4096 && !whole;
+  const bool dealt = rows <= (long long)a.sequences * kFewRows && a.sequences <= 4096 && !whole;
   if (dealt) {
     p.splits = 0;
     p.chunk = (int)max((long long)kLeastTiles, min((long long)kMostTiles, tiles / kParts));
