@@ -476,7 +476,9 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
   __shared__ float stats[2][kWaves][16 * RT];
   __shared__ unsigned arrived;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool shared = p.splits == 0;
+  // Keys are dealt out for up to kFewRows rows, which take the smallest row tiles of their head size.
+  constexpr bool kDealt = R == 8 || (D == 256 && R == 16);
+  const bool shared = kDealt && p.splits == 0;
 
   // The block's runs of tiles: one, or as many as its share of all tiles has; and where the first one's result goes.
   Run run;
