@@ -44,7 +44,7 @@ struct Params {
 
 struct F16 {
   typedef f16x8 vec;
-  static constexpr unsigned kNonFinite = 0x7c00u;
+  static constexpr unsigned kNonFinite = 0x7c00u, kOne = 0x3c00u;
   __device__ static f32x16 mfma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -52,7 +52,7 @@ struct F16 {
 };
 struct B16 {
   typedef bf16x8 vec;
-  static constexpr unsigned kNonFinite = 0x7f80u;
+  static constexpr unsigned kNonFinite = 0x7f80u, kOne = 0x3f80u;
   __device__ static f32x16 mfma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -118,6 +118,17 @@ __device__ __forceinline__ bool strange(const u32x4& words) {
   for (int j = 0; j < 4; ++j)
     found |= (words[j] & T::kNonFinite) == T::kNonFinite || (words[j] >> 16 & T::kNonFinite) == T::kNonFinite;
   return found;
+}
+// Of two values, a one where one is infinite with this sign or no number, and a zero elsewhere.
+template <typename T>
+__device__ __forceinline__ unsigned flags_of(unsigned word, unsigned sign) {
+  unsigned flags = 0;
+#pragma unroll
+  for (int shift = 0; shift < 32; shift += 16) {
+    const unsigned bits = word >> shift & 0xffffu, size = bits & 0x7fffu;
+    if (size > T::kNonFinite || (size == T::kNonFinite && bits >> 15 == sign)) flags |= T::kOne << shift;
+  }
+  return flags;
 }
 __device__ __forceinline__ u32x4 piece_of(const unsigned char* rows, int slot) {
   return *reinterpret_cast<const u32x4*>(rows + slot * 16);
@@ -214,6 +225,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
   float m = kNoKey, l = 0.0f;
+  bool cleared = false;  // some value that is no finite number was left out
+  bool searched = true;  // every tile was searched for them
 
   for (int i = 0; i < tiles; ++i) {
     const int key0 = tile_of(i) * KEYS;
@@ -221,7 +234,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
     direct_load_sync();  // this tile has arrived, and nobody reads the other buffer any more
     if (i + 1 < tiles) load_tile(i + 1, (i + 1) & 1);
     // A weight of zero times a value that is no finite number would be no number.  Where rows see different keys, such
-    // values go to the sums of the rows that see them here, and become zeros in LDS.
+    // values become zeros in LDS; the sums of the rows that see them are set at the end.
     const bool edge = key0 + KEYS - 1 > rows.start ||
                       (a.window > 0 && key0 <= last - a.window && key0 + KEYS > a.sinks);
     if (edge) {
@@ -229,31 +242,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) found |= strange<T>(piece_of(stage.v, j * kThreads + (int)threadIdx.x));
       if (__syncthreads_or(found)) {
-#pragma unroll 1
-        for (int slot = lane; slot < KEYS * kPieces; slot += 64) {
-          const u32x4 words = piece_of(stage.v, slot);
-          unsigned long long left = __ballot(strange<T>(words));
-          while (left != 0ull) {
-            const int from = __builtin_ctzll(left), at = slot - lane + from, row = at / kPieces;
-            left &= left - 1;
-            const int key = key0 + row;
-            const bool seen = key <= position && (a.window == 0 || key > position - a.window || key < a.sinks);
-#pragma unroll 1
-            for (int e = 0; e < 8; ++e) {
-              const unsigned word = e < 4 ? (e < 2 ? words[0] : words[1]) : (e < 6 ? words[2] : words[3]);
-              const unsigned bits = __builtin_amdgcn_readlane((int)word, from) >> (16 * (e & 1)) & 0xffffu;
-              if ((bits & T::kNonFinite) != T::kNonFinite) continue;
-              const float number = (bits & 0x7fffu) != T::kNonFinite ? NAN : bits >> 15 ? -INFINITY : INFINITY;
-              const int dim = ((at % kPieces) ^ v_swizzle<D>(row)) * 8 + e;
-#pragma unroll
-              for (int k = 0; k < kDims; ++k)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  if (seen && 32 * k + 8 * (r / 4) + 4 * half + r % 4 == dim) o[k][r] += number;
-            }
-          }
-        }
-        __syncthreads();
+        cleared = true;
 #pragma unroll 1
         for (int slot = threadIdx.x; slot < KEYS * kPieces; slot += kThreads) {
           u32x4 words = piece_of(stage.v, slot);
@@ -266,6 +255,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
         }
         __syncthreads();
       }
+    } else {
+      searched = false;
     }
     const bool none = key0 > high || low >= rows.count ||
                       (a.window > 0 && key0 + KEYS - 1 <= low - a.window && key0 >= a.sinks);
@@ -363,15 +354,69 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
   }
 
   l += __shfl_xor(l, 32);
-  if (position >= rows.count) return;
-  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* to = static_cast<uint16_t*>(a.out) + ((long long)(rows.begin + position) * a.heads + head) * D + 4 * half;
+  auto store = [&]() {
+    if (position >= rows.count) return;
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* to = static_cast<uint16_t*>(a.out) + ((long long)(rows.begin + position) * a.heads + head) * D + 4 * half;
 #pragma unroll
-  for (int k = 0; k < kDims; ++k)
+    for (int k = 0; k < kDims; ++k)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *reinterpret_cast<u32x2*>(to + 32 * k + 2 * r) = u32x2{T::pack(o[k][r] * inverse, o[k][r + 1] * inverse),
-                                                             T::pack(o[k][r + 2] * inverse, o[k][r + 3] * inverse)};
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<u32x2*>(to + 32 * k + 2 * r) = u32x2{T::pack(o[k][r] * inverse, o[k][r + 1] * inverse),
+                                                               T::pack(o[k][r + 2] * inverse, o[k][r + 3] * inverse)};
+  };
+  store();
+
+  // A row that sees a value that is no finite number gets the infinity, or no number, as its sum.  Such values have
+  // been left out, or an infinity met a weight too small for its type in a tile that was not searched: then a row whose
+  // logits are numbers has a sum that is none.  In either case the wave goes through its values once more, straight
+  // from memory, and stores its rows again (tested before the stores, or by all waves with a barrier, any long prompt
+  // takes 2 to 4 % longer).
+  bool odd = false;
+  if (!searched) {
+    float zero[4] = {};
+#pragma unroll
+    for (int k = 0; k < kDims; ++k)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) zero[r & 3] = fmaf(o[k][r], 0.0f, zero[r & 3]);
+    odd = !((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f) && l < INFINITY;
+  }
+  if (low <= high && (cleared || __ballot(odd) != 0ull)) {
+#pragma unroll
+    for (int k = 0; k < kDims; ++k) {
+      // How many infinities of either sign each row sees per dim: the products of their flags and the visibility.
+      f32x16 count[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) count[0][r] = count[1][r] = 0.0f;
+#pragma unroll 1
+      for (int step = 0; step < tiles * (KEYS / 16); ++step) {
+        const int key0 = tile_of(step / (KEYS / 16)) * KEYS + step % (KEYS / 16) * 16 + 4 * half;
+        u32x4 seen, flags[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          seen[j] = 0;
+          unsigned word = 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = key0 + 8 * (j / 2) + 2 * (j % 2) + e;
+            word |= (unsigned)v0[min(key, rows.count - 1) * a.v_strides.token + 32 * k + n] << (16 * e);
+            if (key <= position && (a.window == 0 || key > position - a.window || key < a.sinks))
+              seen[j] |= T::kOne << (16 * e);
+          }
+#pragma unroll
+          for (unsigned sign = 0; sign < 2; ++sign) flags[sign][j] = flags_of<T>(word, sign);
+        }
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign)
+          count[sign] = T::mfma(bits_as<vec>(flags[sign]), bits_as<vec>(seen), count[sign]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (count[0][r] > 0.0f || count[1][r] > 0.0f)
+          o[k][r] = count[1][r] == 0.0f ? INFINITY : count[0][r] == 0.0f ? -INFINITY : NAN;
+    }
+    store();
+  }
 }
 
 template <typename T>

@@ -224,3 +224,30 @@ def test_refusals(cuda, rng):
                 dict(strides=(256, 64, 1 << 23, 64, 128, 64)), dict(strides=(256, 64, 128, 64, -128, 64)),
                 dict(heads=3), dict(sequences=2), dict(scale=0.0)):
         assert call(**bad) != 0
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("spread", [1.0, 3.0, 40.0])
+def test_infinities_at_any_key(cuda, rng, dtype, dim, spread):
+    """An infinite value that a row sees makes its sum infinite, in whichever of the row's tiles the key lies and however
+    small its weight is; every other number is what it is without them."""
+    from ivonar_amd import attention
+
+    q, k, v = _inputs(cuda, rng, 340, 2, 1, dim, dtype)
+    q *= spread  # how far the weights are apart
+    bad = [(0, 1, np.inf), (2, 2, -np.inf), (3, 3, np.inf), (70, dim - 1, -np.inf), (200, 40, np.inf),
+           (290, 1, np.inf), (300, 2, np.inf), (310, 9, np.nan)]
+    clean_v = v.clone()
+    for row, column, value in bad:
+        v[row, 0, column] = value
+        clean_v[row, 0, column] = 0
+    for window, sinks in ((0, 0), (40, 0), (100, 2)):
+        expected = attention.window_attention(q, k, clean_v, None, window, sinks).float().cpu().numpy()
+        for i in range(340):
+            seen = A.visible(i, 340, window, sinks)
+            for row, column, value in bad:
+                if seen[row]:
+                    expected[i, :, column] += value
+        out = attention.window_attention(q, k, v, None, window, sinks).float().cpu().numpy()
+        np.testing.assert_array_equal(out, expected, err_msg=f"window {window}, sinks {sinks}")
