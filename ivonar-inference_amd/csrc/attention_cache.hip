@@ -38,6 +38,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr float kNoKey = -3.0e38f;  // running maximum before any key
 constexpr float kGrowth = 8.0f;
+constexpr float kFar = 0x1p24f;  // from here on a maximum, x * scale, may be rounded by one and more
 
 struct Params {
   CacheAttentionArgs a;
@@ -47,6 +48,7 @@ struct Params {
   int chunk;     // key tiles of a split, or the least that a block takes of all
   int blocks;    // of each head
   float scale;   // log2(e) * scale
+  float inverse;
   bool aligned;  // q's rows start on 16 bytes
   bool stream;   // the cache is loaded past the memory-side cache
   unsigned* counters;  // of dealt out row tiles, by their first block: the parts that have arrived
@@ -574,6 +576,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
 
     f32x4 o[kTiles][RT];
     float m[RT], l[RT];
+    bool far = false;  // some row's maximum is
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       m[rt] = kNoKey;
@@ -683,6 +686,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
         grows |= most[rt] > m[rt] + kGrowth;
       }
       if (__ballot(grows) != 0ull) {
+        bool some = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           // Only the rows that grow: a row's rounding does not depend on its neighbours.
@@ -690,9 +694,26 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
           const float raised = highest > m[rt] + kGrowth ? highest : m[rt];
           const float factor = __builtin_amdgcn_exp2f(m[rt] - raised);
           m[rt] = raised;
+          some |= fabsf(raised) >= kFar && raised > kNoKey;
           l[rt] *= factor;
 #pragma unroll
           for (int k = 0; k < kTiles; ++k) o[k][rt] *= factor;
+        }
+        far = __ballot(some) != 0ull;
+      }
+      // x * scale - m in one rounding, unless the rounding of m alone counts; then x becomes what the difference of the
+      // two rounded numbers is.  (Costs common logits up to 1 %.)
+      float shift[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) shift[rt] = m[rt];
+      if (__builtin_expect(far, 0)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const bool mine = fabsf(m[rt]) >= kFar && m[rt] > kNoKey;
+#pragma unroll
+          for (int e = 0; e < 4 * kHalves; ++e)
+            x[e / 4][rt][e & 3] = mine ? (x[e / 4][rt][e & 3] * p.scale - m[rt]) * p.inverse : x[e / 4][rt][e & 3];
+          shift[rt] = mine ? 0.0f : m[rt];
         }
       }
 
@@ -710,7 +731,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
           __bf16 terms[2][NP];
 #pragma unroll
           for (int f = 0; f < 2; ++f) {
-            const float w = __builtin_amdgcn_exp2f(fmaf(x[e / 4][rt][(e + f) & 3], p.scale, -m[rt]));
+            const float w = __builtin_amdgcn_exp2f(fmaf(x[e / 4][rt][(e + f) & 3], p.scale, -shift[rt]));
             sum += w;
             split_terms<NP>(w, terms[f]);
           }
@@ -956,7 +977,8 @@ int tile_rows(const CacheAttentionArgs& a) {
 }
 
 Params plan(const CacheAttentionArgs& a) {
-  Params p{a, a.heads / a.kv_heads, 0, 1, 0, 0, 1.44269504088896340736f * a.scale, false, false, nullptr};
+  Params p{a, a.heads / a.kv_heads, 0, 1, 0, 0, 1.44269504088896340736f * a.scale, 0.0f, false, false, nullptr};
+  p.inverse = 1.0f / p.scale;
   const int size = a.dtype == kFloat32 ? 4 : 2;
   p.aligned =
       (((uintptr_t)a.q | (uintptr_t)(a.q_strides.token * size) | (uintptr_t)(a.q_strides.head * size)) & 15u) == 0;

@@ -34,12 +34,14 @@ constexpr int kWaveRows = 32;
 constexpr int kRows = kWaves * kWaveRows;
 constexpr float kNoKey = -3.0e38f;  // running maximum before any key
 constexpr float kGrowth = 8.0f;
+constexpr float kFar = 0x1p24f;  // from here on a maximum, x * scale, may be rounded by one and more
 
 struct Params {
   WindowAttentionArgs a;
   int group;
   int slots;    // row tiles of all sequences (an upper bound)
   float scale;  // log2(e) * scale
+  float inverse;
 };
 
 struct F16 {
@@ -225,6 +227,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
   float m = kNoKey, l = 0.0f;
+  bool far = false;      // some row's maximum is
   bool cleared = false;  // some value that is no finite number was left out
   bool searched = true;  // every tile was searched for them
 
@@ -311,9 +314,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
       const float raised = highest > m + kGrowth ? highest : m;
       const float factor = __builtin_amdgcn_exp2f(m - raised);
       m = raised;
+      far = __ballot(fabsf(m) >= kFar && m > kNoKey) != 0ull;
       l *= factor;
 #pragma unroll
       for (int k = 0; k < kDims; ++k) o[k] *= factor;
+    }
+
+    // x * scale - m in one rounding, unless the rounding of m alone counts; then x becomes what the difference of the
+    // two rounded numbers is.  (Costs common logits up to 1 %.)
+    float shift = m;
+    if (far) {
+      const bool mine = fabsf(m) >= kFar && m > kNoKey;
+#pragma unroll
+      for (int s = 0; s < kSubtiles; ++s)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[s][r] = mine ? (x[s][r] * p.scale - m) * p.inverse : x[s][r];
+      shift = mine ? 0.0f : m;
     }
 
     vec weights[2 * kSubtiles];
@@ -324,8 +340,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : D == 128 ? 2 : 3) void win
         u32x4 words;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float u = __builtin_amdgcn_exp2f(fmaf(x[s][8 * b + 2 * j], p.scale, -m));
-          const float w = __builtin_amdgcn_exp2f(fmaf(x[s][8 * b + 2 * j + 1], p.scale, -m));
+          const float u = __builtin_amdgcn_exp2f(fmaf(x[s][8 * b + 2 * j], p.scale, -shift));
+          const float w = __builtin_amdgcn_exp2f(fmaf(x[s][8 * b + 2 * j + 1], p.scale, -shift));
           l += u + w;
           words[j] = T::pack(u, w);
         }
@@ -433,7 +449,8 @@ void run(hipStream_t stream, const Params& p, unsigned blocks) {
 
 hipError_t launch_window_attention(hipStream_t stream, const WindowAttentionArgs& a) {
   if (a.rows == 0) return hipSuccess;
-  Params p{a, a.heads / a.kv_heads, 0, 1.44269504088896340736f * a.scale};
+  Params p{a, a.heads / a.kv_heads, 0, 1.44269504088896340736f * a.scale, 0.0f};
+  p.inverse = 1.0f / p.scale;
   p.slots = a.offsets == nullptr ? (a.rows + kRows - 1) / kRows : a.rows / kRows + a.sequences;
   const long long blocks = (long long)(p.slots + (a.offsets != nullptr ? 1 : 0)) * a.heads;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;

@@ -346,3 +346,42 @@ def test_refusals(cuda, rng):
     for bad in ((None, need), (work.data_ptr(), need - 1), (work.data_ptr() + 4, need), (work.data_ptr(), need, -1.0),
                 (work.data_ptr(), need, 0.1, -1)):
         assert call(*bad) != 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_logits_past_the_integers(cuda, rng, dtype, dim):
+    """Logits so large that fp32 holds them in steps of far more than one: the largest takes all the weight, and rows
+    next to such a row come out as they do without it."""
+    import torch
+    from ivonar_amd import attention
+
+    case = Case(cuda, rng, [400], 1, dim)
+    k = np.zeros((400, 1, dim), np.float32)
+    k[:, 0, 0] = rng.choice([0.0, 0.5, 1.0, -0.5], 400)
+    for token, value in ((5, 1.5), (130, 4.0), (360, 6.0), (381, 8.0), (60, -1.0), (200, -6.0), (370, -12.0)):
+        k[token] = value
+    v = rng.standard_normal((400, 1, dim)).astype(np.float32)
+    attention.cache_write(case.pages, torch.from_numpy(k).to(cuda), torch.from_numpy(v).to(cuda), case.table,
+                          _ints(cuda, [0]), _ints(cuda, [0, 400]))
+    key, value = A.stored(k)[:, 0, 0], A.stored(v)[:, 0]
+    lengths = _ints(cuda, [400])
+    for count in (1, 3, 8, 50):  # row tiles of every size
+        q = torch.zeros(count, 2, dim, device=cuda, dtype=getattr(torch, dtype))
+        q[:, 0, 0], q[:, 1, 0] = 2.0 ** 15, -2.0 ** 15
+        offsets = _ints(cuda, [0, count])
+        for scale in (2.0 ** 10, 2.0 ** 16, 2.0 ** 30):  # logits from 2^25 to 2^49
+            out = attention.cache_attention(q, case.pages, case.table, lengths, offsets, scale=scale)
+            out = out.double().cpu().numpy()
+            for i in range(count):
+                last = 400 - count + i
+                for head, best in enumerate((key[:last + 1].argmax(), key[:last + 1].argmin())):
+                    expected = torch.from_numpy(value[best]).to(q.dtype).double().numpy()
+                    assert np.array_equal(out[i, head], expected), (count, scale, i, head)
+        q = torch.randn(count, 2, dim, device=cuda).mul_(2.0 ** -10).to(q.dtype)
+        q[::2, 1] = 0
+        q[::2, 1, 0] = 2.0 ** 15
+        out = attention.cache_attention(q, case.pages, case.table, lengths, offsets, scale=2.0 ** 10)
+        q[::2, 1] = 0
+        without = attention.cache_attention(q, case.pages, case.table, lengths, offsets, scale=2.0 ** 10)
+        assert torch.equal(out[:, 0], without[:, 0]) and torch.equal(out[1::2], without[1::2])

@@ -230,8 +230,8 @@ def test_refusals(cuda, rng):
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("spread", [1.0, 3.0, 40.0])
 def test_infinities_at_any_key(cuda, rng, dtype, dim, spread):
-    """An infinite value that a row sees makes its sum infinite, in whichever of the row's tiles the key lies and however
-    small its weight is; every other number is what it is without them."""
+    """An infinite value that a row sees makes its sum infinite, in whichever of the row's tiles the key lies and
+    however small its weight is; every other number is what it is without them."""
     from ivonar_amd import attention
 
     q, k, v = _inputs(cuda, rng, 340, 2, 1, dim, dtype)
@@ -251,3 +251,33 @@ def test_infinities_at_any_key(cuda, rng, dtype, dim, spread):
                     expected[i, :, column] += value
         out = attention.window_attention(q, k, v, None, window, sinks).float().cpu().numpy()
         np.testing.assert_array_equal(out, expected, err_msg=f"window {window}, sinks {sinks}")
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_logits_past_the_integers(cuda, rng, dtype, dim):
+    """Logits so large that fp32 holds them in steps of far more than one: the largest takes all the weight, and rows
+    next to such a row come out as they do without it."""
+    import torch
+    from ivonar_amd import attention
+
+    q, k, v = _inputs(cuda, rng, 200, 2, 1, dim, dtype)
+    order = rng.permutation(200)
+    k[:, 0, 0] = torch.from_numpy(order.astype(np.float32)).to(k)
+    large = q.clone()
+    large[1::3] = 0
+    large[1::3, 0, 0], large[1::3, 1, 0] = 2.0 ** 15, -2.0 ** 15
+    for window, sinks in ((0, 0), (50, 4)):
+        for scale in (2.0 ** 10, 2.0 ** 16, 2.0 ** 30):  # logits from 2^25 to 2^52
+            out = attention.window_attention(large, k, v, None, window, sinks, scale)
+            for i in range(1, 200, 3):
+                keys = np.flatnonzero(A.visible(i, 200, window, sinks))
+                for head, best in enumerate((keys[order[keys].argmax()], keys[order[keys].argmin()])):
+                    assert torch.equal(out[i, head], v[best, 0]), (scale, i, head)
+        # the other rows' logits are common ones: as if there were no large ones
+        small = q * 2.0 ** -10
+        small[1::3] = large[1::3]
+        others = np.flatnonzero(np.arange(200) % 3 != 1)
+        out = attention.window_attention(small, k, v, None, window, sinks, 2.0 ** 10)
+        small[1::3] = 0
+        assert torch.equal(out[others], attention.window_attention(small, k, v, None, window, sinks, 2.0 ** 10)[others])
