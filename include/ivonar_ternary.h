@@ -260,8 +260,8 @@ hipError_t sample_token(hipStream_t stream, const float* logits, const float* bo
  * pages: [page_count, kv_heads, page_tiles, 34 * head_dim] bytes, 16-byte aligned; page_tiles (tiles of 32 tokens
  * per page) a power of two; head_dim 64, 128 or 256.  A value is 4-bit floating point (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
  * their negatives); 32 neighbouring values of a row share a power-of-two scale byte.  table: [sequences, table_width]
- * page numbers, at most 2^30 tokens per sequence; an entry outside 0 .. page_count - 1 is no page: nothing is written
- * there, 0 is read, and attention does not see its tokens.  offsets: [sequences + 1] rows before each sequence, not
+ * page numbers, at most 2^30 tokens per sequence; an entry outside 0 .. page_count - 1 is no page, and so is every
+ * position past the table: nothing is written there, 0 is read, and attention does not see its tokens.  offsets: [sequences + 1] rows before each sequence, not
  * decreasing, or NULL for one row per sequence (rows == sequences).  dtype: 0 fp32, 1 fp16, 2 bfloat16.  Strides are
  * in elements; a head's dims lie side by side.  All index arrays are int32 on the device and are not read by the host.
  *

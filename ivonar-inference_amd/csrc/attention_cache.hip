@@ -76,14 +76,14 @@ __device__ __forceinline__ Span make_span(const Params& p, int sequence, int row
   s.row0 = row0;
   s.rows = queries * p.group;
   s.start = start;
-  // The table's capacity is at most 2^30 tokens, so positions less the window stay within 32 bits.
-  const int capacity = (a.table_width << a.page_shift) * kCacheTile;
-  s.first = min(max(length, 0), capacity) - queries;
+  // Rows, the window and the table's tokens are at most 2^30, so positions less any of them stay within 32 bits.
+  s.first = max(length, 0) - queries;
   s.low = s.first + start / p.group;
   s.high = s.first + (min(start + R, s.rows) - 1) / p.group;
-  const int end_tile = s.high < 0 ? 0 : s.high / kCacheTile + 1;
+  // Rows may lie past the table, which has no page for what they see there.
+  const int end_tile = s.high < 0 ? 0 : min(s.high / kCacheTile + 1, a.table_width << a.page_shift);
   s.window_tile = a.window == 0 || s.low < a.window ? 0 : (s.low - a.window + 1) / kCacheTile;
-  s.window_tile = min(s.window_tile, end_tile);
+  s.window_tile = min(s.window_tile, max(end_tile - 1, 0));
   s.sink_tiles = a.window == 0 ? 0 : min(a.sinks <= 0 ? 0 : (a.sinks - 1) / kCacheTile + 1, s.window_tile);
   s.total = max(1, s.sink_tiles + end_tile - s.window_tile);
   return s;
@@ -702,7 +702,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
         far = __ballot(some) != 0ull;
       }
       // x * scale - m in one rounding, unless the rounding of m alone counts; then x becomes what the difference of the
-      // two rounded numbers is.  (Costs common logits up to 1 %.)
+      // two rounded numbers is.  (Costs common logits 1 to 2 %.)
       float shift[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) shift[rt] = m[rt];

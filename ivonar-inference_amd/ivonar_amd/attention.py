@@ -18,8 +18,8 @@ that 32 neighbouring values of a head's row share: 4.25 bits per value.  A block
 infinity reads back as NaN.
 
 ``table`` [sequences, width] (int32) holds each sequence's page numbers in order; an entry outside the pages (-1, for
-instance) is no page: nothing is written there, zeros are read, and attention does not see its tokens, so pages
-before a window may be handed back.  ``offsets`` (int32 [sequences + 1]) are the rows before each sequence in a ragged
+instance) is no page, and so is every position past the table: nothing is written there, zeros are read, and attention
+does not see its tokens, so pages before a window may be handed back.  ``offsets`` (int32 [sequences + 1]) are the rows before each sequence in a ragged
 batch; None stands for one row per sequence.  Rows past the last sequence's (padding) are not written to the cache,
 and are zero in the results.  Index tensors stay on the device: no call reads them on the host, allocates more than
 its results and a workspace, or synchronises, so all of them can be captured into a graph.

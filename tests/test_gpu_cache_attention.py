@@ -385,3 +385,23 @@ def test_logits_past_the_integers(cuda, rng, dtype, dim):
         q[::2, 1] = 0
         without = attention.cache_attention(q, case.pages, case.table, lengths, offsets, scale=2.0 ** 10)
         assert torch.equal(out[:, 0], without[:, 0]) and torch.equal(out[1::2], without[1::2])
+
+
+@pytest.mark.parametrize("length,window,sinks", [(80, 0, 0), (80, 20, 3), (65, 1, 0), (5000, 64, 0), (5000, 64, 70),
+                                                 (2 ** 31 - 1, 2 ** 30, 5), (2 ** 31 - 1, 0, 0)])
+def test_lengths_past_the_table(cuda, rng, length, window, sinks):
+    """Positions past the table have no page: the rows keep their positions, and see what the table holds of them."""
+    import torch
+    from ivonar_amd import attention
+
+    case = Case(cuda, rng, [2048], 2, 64, page=32)
+    for width in (2, 64):
+        table = case.table[:, :width].contiguous()
+        keys = 32 * width
+        for count in (1, 5, 40):
+            q = torch.randn(count, 4, 64, device=cuda)
+            out = attention.cache_attention(q, case.pages, table, _ints(cuda, [length]), _ints(cuda, [0, count]), window,
+                                            sinks).cpu().numpy()
+            seen = min(keys, length)
+            result = A.attend(q.cpu().numpy(), case.k[0][:seen], case.v[0][:seen], length - count, window, sinks)
+            A.check(out, *result, "float32", keys, 64, f"{count} rows over {keys} tokens")
