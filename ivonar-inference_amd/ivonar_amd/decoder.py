@@ -380,9 +380,7 @@ class StackDecoder:
         if int(ids.min()) < 0 or int(ids.max()) >= self.config.vocab:
             raise IndexError(f"token id is out of range for vocab_size={self.config.vocab}")
         attention = self.attention
-        if attention is not None:
-            attention.tokens = 0
-            self._reserve(length)
+        self._reserve(length, held=0)
         host, start = self._tile_host, 0
         while start < length:
             count = min(length - start, TILES[-1])
@@ -404,14 +402,16 @@ class StackDecoder:
         self.position = 0
         return self.logits
 
-    def _reserve(self, count: int) -> None:
-        """Counts `count` tokens into the cache, which must have room for them."""
+    def _reserve(self, count: int, held: int | None = None) -> None:
+        """Counts `count` tokens into the cache behind `held` (default: all that it has); it must have room for them,
+        and stays as it is if it has not."""
         attention = self.attention
         if attention is None:
             return
-        if attention.tokens + count > attention.config.capacity:
-            raise ValueError(f"the cache holds {attention.config.capacity} tokens, not {attention.tokens + count}")
-        attention.tokens += count
+        total = count + (attention.tokens if held is None else held)
+        if total > attention.config.capacity:
+            raise ValueError(f"the cache holds {attention.config.capacity} tokens, not {total}")
+        attention.tokens = total
 
     @torch.no_grad()
     def step(self) -> None:

@@ -124,3 +124,16 @@ def test_refusals(cuda):
         decoder.step()
     assert decoder.attention.tokens == 40
     decoder.prefill(prompt_ids(STACK.vocab, 40))  # a new prompt starts anew
+
+
+def test_refused_prompt_leaves_the_sequence_as_it_is(cuda):
+    decoder = _decoder(cuda, capacity=40)
+    decoder.generate(prompt_ids(STACK.vocab, 36), 3)
+    with pytest.raises(ValueError):
+        decoder.prefill(prompt_ids(STACK.vocab, 41))
+    assert decoder.attention.tokens == 38 == int(decoder.attention.step_index[0])
+    decoder.step()
+    decoder.step()
+    with pytest.raises(ValueError):
+        decoder.step()
+    assert decoder.attention.tokens == 40 == int(decoder.attention.step_index[0])
