@@ -405,13 +405,15 @@ class StackDecoder:
     def _reserve(self, count: int, held: int | None = None) -> None:
         """Counts `count` tokens into the cache behind `held` (default: all that it has); it must have room for them,
         and stays as it is if it has not."""
-        attention = self.attention
-        if attention is None:
-            return
-        total = count + (attention.tokens if held is None else held)
-        if total > attention.config.capacity:
-            raise ValueError(f"the cache holds {attention.config.capacity} tokens, not {total}")
-        attention.tokens = total
+        if self.attention is not None:
+            total = count + (self.attention.tokens if held is None else held)
+            self._require_room(total)
+            self.attention.tokens = total
+
+    def _require_room(self, total: int) -> None:
+        capacity = self.attention.config.capacity
+        if total > capacity:
+            raise ValueError(f"the cache holds {capacity} tokens, not {total}")
 
     @torch.no_grad()
     def step(self) -> None:
@@ -483,7 +485,10 @@ class StackDecoder:
     @torch.no_grad()
     def advance_many(self, count: int) -> list[int]:
         """``count`` greedy tokens after the last one produced: whole bursts replay the graph with one
-        read-back each (kernel_decoder.py:722-735); the rest run eagerly."""
+        read-back each (kernel_decoder.py:722-735); the rest run eagerly.  With attention the cache must have room
+        for all of them, or none is run."""
+        if self.attention is not None:
+            self._require_room(self.attention.tokens + count)
         tokens: list[int] = []
         sampling = self.sampler is not None
         while count - len(tokens) >= self.burst and self._graph is not None and self.position % self.burst == 0:

@@ -137,3 +137,24 @@ def test_refused_prompt_leaves_the_sequence_as_it_is(cuda):
     with pytest.raises(ValueError):
         decoder.step()
     assert decoder.attention.tokens == 40 == int(decoder.attention.step_index[0])
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_many_steps_are_refused_as_a_whole(cuda, captured):
+    """No token is lost where the cache has room for some of a call's steps only."""
+    prompt = prompt_ids(STACK.vocab, 20)
+    expected = _decoder(cuda).generate(prompt, 21)
+    decoder = _decoder(cuda, capacity=40)
+    decoder.prefill(prompt)
+    if captured:
+        decoder.capture()
+    first = int(decoder.history[decoder.burst - 1])
+    with pytest.raises(ValueError):
+        decoder.advance_many(21)
+    assert decoder.attention.tokens == 20 == int(decoder.attention.step_index[0])
+    assert [first] + decoder.advance_many(20) == expected
+    with pytest.raises(ValueError):
+        decoder.advance_many(1)
+    with pytest.raises(ValueError):
+        decoder.generate(prompt, 22)
+    assert decoder.generate(prompt, 21) == expected
