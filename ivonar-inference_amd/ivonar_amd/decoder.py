@@ -521,14 +521,16 @@ class StackDecoder:
         """Runs one prompt through the prefill tiles and through single decode steps and requires both to
         agree (kernel_decoder.py:524-549), so a GPU the kernels do not run correctly on fails while loading.
 
-        The prompt has TILE + TILE // 2 + 1 random ids in [2, vocab): prefill() takes it whole (the GEMMs of
-        a 64-token tile), then the first id alone, after which every further id is written into the ring slot the
-        next step reads and one step consumes it (the GEMVs).  Both end with the logits of the prompt's last
-        id; they must be finite, not all zero, and within a relative norm of SELF_CHECK_TOLERANCE, and the
-        token the last step selected must lie in the vocabulary.  The decoder is reset afterwards.  Raises
-        KernelError."""
+        The prompt has TILE + TILE // 2 + 1 random ids in [2, vocab), or as many as an attention cache holds:
+        prefill() takes it whole (the GEMMs of a 64-token tile), then the first id alone, after which every further
+        id is written into the ring slot the next step reads and one step consumes it (the GEMVs).  Both end with
+        the logits of the prompt's last id; they must be finite, not all zero, and within a relative norm of
+        SELF_CHECK_TOLERANCE, and the token the last step selected must lie in the vocabulary.  The decoder is reset
+        afterwards.  Raises KernelError."""
         vocab = int(self.config.vocab)
         length = TILE + TILE // 2 + 1
+        if self.attention is not None:
+            length = min(length, self.attention.config.capacity)
         ids = torch.randint(2, max(vocab, 3), (length,), generator=torch.Generator().manual_seed(0)) % vocab
         whole = self.prefill(ids).clone()
         self.prefill(ids[:1])

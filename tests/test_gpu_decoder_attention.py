@@ -158,3 +158,10 @@ def test_many_steps_are_refused_as_a_whole(cuda, captured):
     with pytest.raises(ValueError):
         decoder.generate(prompt, 22)
     assert decoder.generate(prompt, 21) == expected
+
+
+@pytest.mark.parametrize("capacity", [1, 2, 33, 48])
+def test_self_check_of_a_small_cache(cuda, capacity):
+    decoder = _decoder(cuda, capacity=capacity)
+    decoder.self_check()
+    assert decoder.attention.tokens == 0
