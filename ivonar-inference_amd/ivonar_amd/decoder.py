@@ -66,6 +66,9 @@ TILE = 32
 # 1024/4096 took 11.25 ms in 16 tiles of 32 and take 1.5 ms in one of 512.
 TILES = (32, 64, 128, 256, 512, 1024)
 SELF_CHECK_TOLERANCE = 0.25  # kernel_decoder.py:38
+# With attention the steps see keys and values in 4 bits and a prompt's first tile does not: 0.1 to 0.4 of the logits'
+# norm on 220 random stacks of 1 to 32 layers, on right kernels.  Logits that have nothing in common are 1.4 apart.
+SELF_CHECK_CACHED = 1.0
 THREADS = 256
 HEAD_LANES = 4
 CHUNK = 64
@@ -525,8 +528,8 @@ class StackDecoder:
         prefill() takes it whole (the GEMMs of a 64-token tile), then the first id alone, after which every further
         id is written into the ring slot the next step reads and one step consumes it (the GEMVs).  Both end with
         the logits of the prompt's last id; they must be finite, not all zero, and within a relative norm of
-        SELF_CHECK_TOLERANCE, and the token the last step selected must lie in the vocabulary.  The decoder is reset
-        afterwards.  Raises KernelError."""
+        SELF_CHECK_TOLERANCE (SELF_CHECK_CACHED with attention), and the token the last step selected must lie in
+        the vocabulary.  The decoder is reset afterwards.  Raises KernelError."""
         vocab = int(self.config.vocab)
         length = TILE + TILE // 2 + 1
         if self.attention is not None:
@@ -544,7 +547,7 @@ class StackDecoder:
         if not (bool(torch.isfinite(whole).all()) and bool(torch.isfinite(stepped).all())) or scale == 0.0:
             raise KernelError("the ternary kernels produced invalid numbers on this GPU")
         difference = float((whole - stepped).norm()) / scale
-        if difference > SELF_CHECK_TOLERANCE:
+        if difference > (SELF_CHECK_TOLERANCE if self.attention is None else SELF_CHECK_CACHED):
             raise KernelError(f"the ternary kernels disagree with themselves on this GPU ({difference:.1e})")
         if not 0 <= selected < vocab:
             raise KernelError("the ternary sampler returned an invalid token on this GPU")

@@ -165,3 +165,12 @@ def test_self_check_of_a_small_cache(cuda, capacity):
     decoder = _decoder(cuda, capacity=capacity)
     decoder.self_check()
     assert decoder.attention.tokens == 0
+
+
+@pytest.mark.parametrize("layers,dense,seed", [(16, 256, 17), (6, 512, 2)])
+def test_self_check_allows_for_the_cache(cuda, layers, dense, seed):
+    """Stacks whose steps, with keys and values in 4 bits, are further from the prompt's tile than without a cache."""
+    from ivonar_amd.decoder import AttentionConfig, StackDecoder
+
+    weights = decoder_stack(StackConfig(vocab=700, hidden=64, layers=layers, dense=dense), seed=seed)
+    StackDecoder(weights, cuda, attention=AttentionConfig(1)).self_check()
