@@ -86,6 +86,8 @@ def _geometry(pages: Tensor, table: Tensor, what: str) -> tuple[int, int, int, i
     dim = size // 34
     if dim * 34 != size or dim not in HEAD_DIMS or tiles & (tiles - 1) or not (count and heads and tiles):
         raise KernelError(f"{what} needs pages as cache_pages() makes them")
+    if pages.data_ptr() & 15:
+        raise KernelError(f"{what} needs pages that start on 16 bytes")
     shape = table.shape
     if len(shape) != 2 or table.dtype is not torch.int32 or not table.is_contiguous():
         raise KernelError(f"{what} needs a contiguous int32 table [sequences, width]")
@@ -173,6 +175,8 @@ def _output(q: Tensor, out: Tensor | None) -> Tensor:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
         raise KernelError("out must be contiguous and of q's shape and type")
+    if out.data_ptr() & 15:
+        raise KernelError("out must start on 16 bytes")
     return out
 
 

@@ -405,3 +405,22 @@ def test_lengths_past_the_table(cuda, rng, length, window, sinks):
             seen = min(keys, length)
             result = A.attend(q.cpu().numpy(), case.k[0][:seen], case.v[0][:seen], length - count, window, sinks)
             A.check(out, *result, "float32", keys, 64, f"{count} rows over {keys} tokens")
+
+
+def test_misaligned_tensors_are_named(cuda, rng):
+    import torch
+    from ivonar_amd import attention
+    from ivonar_amd.runtime import KernelError
+
+    case = Case(cuda, rng, [50], 2, 64)
+    q, lengths = torch.zeros(1, 4, 64, device=cuda), _ints(cuda, [50])
+    out = torch.empty(4 * 64 + 1, device=cuda)[1:].view(1, 4, 64)
+    with pytest.raises(KernelError, match="out .*16 bytes"):
+        attention.cache_attention(q, case.pages, case.table, lengths, out=out)
+    pages = torch.zeros(case.pages.numel() + 8, dtype=torch.uint8, device=cuda)[8:].view(case.pages.shape)
+    kv = torch.zeros(1, 2, 64, device=cuda)
+    for call in (lambda: attention.cache_attention(q, pages, case.table, lengths),
+                 lambda: attention.cache_write(pages, kv, kv, case.table, lengths),
+                 lambda: attention.cache_read(pages, case.table, lengths, None, 1)):
+        with pytest.raises(KernelError, match="pages .*16 bytes"):
+            call()
