@@ -74,8 +74,9 @@ def bound(out, spread, size, dtype: str, keys: int, dim: int, weight_unit: float
 
     Logits: products of exact operands summed in fp32, dim of them with up to three terms each, then scaled and
     shifted: (3 dim + 8) 2^-24 of `size`, which is a relative error of each weight; the exponential adds 2^-22.
-    Weights: rounded to TERMS[dtype] bf16 terms (8 bits each) for the product with the values, not for their sum.  Sums over the keys:
-    keys + 64 roundings of 2^-24 each, in numerator and denominator.  Last, the rounding to the result's type."""
+    Weights: rounded for the product with the values, not for their sum, with an error of weight_unit; by default what
+    TERMS[dtype] bf16 terms (8 bits each) leave, more than the cache attention's two terms for bfloat16 rows.  Sums over
+    the keys: keys + 64 roundings of 2^-24 each, in numerator and denominator.  Last, the rounding to the result's type."""
     if weight_unit is None:
         weight_unit = max(2.0 ** (-8 * TERMS[dtype] - 1), 2.0 ** -24)
     relative = weight_unit + 2 * ((3 * dim + 8) * 2.0 ** -24 * size + 2.0 ** -22) + 2 * (keys + 64) * 2.0 ** -24
@@ -104,3 +105,14 @@ def place(lengths, page_size: int, rng, spare: int = 3, width: int = 1):
         table[row, :count] = order[start:start + count]
         start += count
     return total, table
+
+
+def cancelling(length: int, dim: int):
+    """(k, v, scale) of keys that the cache holds exactly, for q = (1, 0, ..): every third one has the weight 1 and the
+    others 0.5 + 0.4 / 256, which bfloat16 rounds to 0.5, and values whose weighted sum is small against their size."""
+    third = np.arange(length) % 3 == 2
+    k = np.zeros((length, 1, dim), np.float32)
+    k[third, :, 0] = 1
+    v = np.resize(np.float32([6, -4, 3, 2, -1.5, 1, -0.5, 6]), (length, 1, dim)).copy()
+    v[third] *= -1
+    return k, v, -math.log(0.5 + 0.4 / 256)

@@ -75,3 +75,28 @@ def test_visible_keys(window, sinks):
     for position in range(-2, 9):
         expected = [j for j in range(8) if j <= position and (window == 0 or j > position - window or j < sinks)]
         assert np.flatnonzero(A.visible(position, 8, window, sinks)).tolist() == expected
+
+
+@pytest.mark.parametrize("count", [1, 40])
+def test_bound_notices_a_weight_of_one_term(count):
+    """Weights rounded to one bfloat16 term miss the bound for two by far, and weights of two terms keep it."""
+    k, v, scale = A.cancelling(300, 64)
+    q = np.zeros((count, 2, 64))
+    q[..., 0] = 1
+    out, spread, size = A.attend(q, k, v, 300 - count, scale=scale)
+    limit = A.bound(out, spread, size, "bfloat16", 300, 64, weight_unit=2.0 ** -17)
+
+    def emulated(terms):
+        got = np.zeros_like(out)
+        for i in range(count):
+            keys = 300 - count + i + 1
+            weight = np.exp(scale * (k[:keys, 0, 0].astype(np.float64) - 1))
+            rounded, rest = np.zeros(keys), weight
+            for _ in range(terms):
+                term = torch.from_numpy(rest).bfloat16().double().numpy()
+                rounded, rest = rounded + term, rest - term
+            got[i] = rounded @ v[:keys, 0] / weight.sum()
+        return torch.from_numpy(got).bfloat16().double().numpy()
+
+    assert (np.abs(emulated(1) - out) > 4 * limit).all()
+    assert (np.abs(emulated(2) - out) <= limit).all()

@@ -424,3 +424,30 @@ def test_misaligned_tensors_are_named(cuda, rng):
                  lambda: attention.cache_read(pages, case.table, lengths, None, 1)):
         with pytest.raises(KernelError, match="pages .*16 bytes"):
             call()
+
+
+# The kernel rounds a weight to two bf16 terms for float16 and bfloat16 rows, and to three for float32 ones.
+WEIGHT = {"float32": 2.0 ** -24, "float16": 2.0 ** -17, "bfloat16": 2.0 ** -17}
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("count", [1, 3, 8, 40])
+def test_every_term_of_the_weights(cuda, dtype, dim, count):
+    """Two thirds of the keys have a weight between two bfloat16 numbers, and values that nearly cancel those of the
+    others: the results are much smaller than the values, so that their own rounding does not hide the weights'."""
+    import torch
+    from ivonar_amd import attention
+
+    length = 300
+    k, v, scale = A.cancelling(length, dim)
+    pages = attention.cache_pages(8, 1, dim, 64, cuda)
+    table = torch.arange(8, dtype=torch.int32, device=cuda).reshape(1, 8)
+    attention.cache_write(pages, torch.from_numpy(k).to(cuda), torch.from_numpy(v).to(cuda), table, _ints(cuda, [0]),
+                          _ints(cuda, [0, length]))
+    assert np.array_equal(A.stored(k), k) and np.array_equal(A.stored(v), v)
+    q = torch.zeros(count, 2, dim, device=cuda, dtype=getattr(torch, dtype))
+    q[..., 0] = 1
+    out = attention.cache_attention(q, pages, table, _ints(cuda, [length]), _ints(cuda, [0, count]), scale=scale)
+    result = A.attend(q.float().cpu().numpy(), k, v, length - count, scale=scale)
+    A.check(out.float().cpu().numpy(), *result, dtype, length, dim, weight_unit=WEIGHT[dtype])
