@@ -451,3 +451,51 @@ def test_every_term_of_the_weights(cuda, dtype, dim, count):
     out = attention.cache_attention(q, pages, table, _ints(cuda, [length]), _ints(cuda, [0, count]), scale=scale)
     result = A.attend(q.float().cpu().numpy(), k, v, length - count, scale=scale)
     A.check(out.float().cpu().numpy(), *result, dtype, length, dim, weight_unit=WEIGHT[dtype])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("count", [30, 4])
+def test_no_number_with_half_queries(cuda, rng, dim, count):
+    """As above for float16 queries, in row tiles of both kinds."""
+    import torch
+    from ivonar_amd import attention
+
+    case = Case(cuda, rng, [90], 1, dim)
+    key, value = np.zeros((1, 1, dim), np.float32), np.zeros((1, 1, dim), np.float32)
+    value[0, 0, 40] = -np.inf
+    attention.cache_write(case.pages, torch.from_numpy(key).to(cuda), torch.from_numpy(value).to(cuda), case.table,
+                          _ints(cuda, [70]))
+    key[0, 0, 0] = np.nan
+    attention.cache_write(case.pages, torch.from_numpy(key).to(cuda), torch.zeros_like(torch.from_numpy(value)).to(cuda),
+                          case.table, _ints(cuda, [88]))
+    case.k[0][70], case.v[0][88] = 0, 0
+    missing = np.zeros(90, bool)
+    missing[[70, 88]] = True
+    q, out = case.run(rng, 2, "float16", queries=[count], check=False)
+    got, rows = out.float().cpu().numpy(), q.float().cpu().numpy()
+    for i in range(count):
+        position = 90 - count + i
+        if position >= 88:
+            assert np.isnan(got[i]).all()
+        elif position >= 70:
+            assert np.isnan(got[i, :, 32:64]).all()
+            assert np.isfinite(got[i, :, :32]).all() and np.isfinite(got[i, :, 64:]).all()
+        else:
+            result = A.attend(rows[i:i + 1], case.k[0], case.v[0], position, missing=missing)
+            A.check(got[i:i + 1], *result, "float16", 90, dim, f"row {i}")
+
+
+def test_results_past_2_to_31_elements(cuda):
+    import torch
+    from ivonar_amd import attention
+
+    rows, heads, dim = 131200, 64, 256
+    pages = attention.cache_pages(2, 1, dim, 32, cuda)
+    table = torch.arange(rows, device=cuda).remainder_(2).to(torch.int32).unsqueeze(1)
+    v = torch.tensor([6.0, -3.0], device=cuda).reshape(2, 1, 1).expand(2, 1, dim).contiguous()
+    attention.cache_write(pages, v, v, table[:2].contiguous(), _ints(cuda, [0, 0]))
+    q = torch.zeros(rows, heads, dim, dtype=torch.bfloat16, device=cuda)
+    out = attention.cache_attention(q, pages, table, torch.ones(rows, dtype=torch.int32, device=cuda))
+    expected = v.bfloat16()
+    for start in range(0, rows, 8200):
+        assert torch.equal(out[start:start + 8200], expected.repeat(4100, heads, 1))

@@ -293,3 +293,16 @@ def test_misaligned_output_is_named(cuda, rng):
     out = torch.empty(10 * 4 * 64 + 4, dtype=torch.float16, device=cuda)[4:].view(10, 4, 64)
     with pytest.raises(KernelError, match="out .*16 bytes"):
         attention.window_attention(q, k, v, out=out)
+
+
+def test_results_past_2_to_31_elements(cuda):
+    import torch
+    from ivonar_amd import attention
+
+    rows, heads, dim = 131200, 64, 256
+    q = torch.zeros(rows, heads, dim, dtype=torch.bfloat16, device=cuda)
+    v = torch.randn(rows, 1, dim, device=cuda).bfloat16()
+    out = attention.window_attention(q, v, v, window=1)  # every row sees itself
+    for start in range(0, rows, 8200):
+        part = slice(start, start + 8200)
+        assert torch.equal(out[part], v[part].expand(8200, heads, dim))
