@@ -49,7 +49,9 @@ extern "C" {
  * gets a scratch of its own (about 17 MB, kept until the process ends) on
  * its first call, so eager calls on different streams never share one; a
  * call under capture uses its stream's scratch if it has one, else the
- * device's.  The null stream and hipStreamPerThread each use one scratch,
+ * device's.  Graphs that share a scratch, or a graph and an eager call on its
+ * scratch's stream, must not run at the same time: results are undefined.
+ * The null stream and hipStreamPerThread each use one scratch,
  * whatever thread calls.  Call once per device outside graph capture;
  * replaces the reference's compile_module set-up step
  * (kernels/runtime.py:301-324).  Calls with the device current.  Calling it
@@ -261,9 +263,10 @@ hipError_t sample_token(hipStream_t stream, const float* logits, const float* bo
  * per page) a power of two; head_dim 64, 128 or 256.  A value is 4-bit floating point (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
  * their negatives); 32 neighbouring values of a row share a power-of-two scale byte.  table: [sequences, table_width]
  * page numbers, at most 2^30 tokens per sequence; an entry outside 0 .. page_count - 1 is no page, and so is every
- * position past the table: nothing is written there, 0 is read, and attention does not see its tokens.  offsets: [sequences + 1] rows before each sequence, not
- * decreasing, or NULL for one row per sequence (rows == sequences).  dtype: 0 fp32, 1 fp16, 2 bfloat16.  Strides are
- * in elements; a head's dims lie side by side.  All index arrays are int32 on the device and are not read by the host.
+ * position past the table: nothing is written there, 0 is read, and attention does not see its tokens.  offsets:
+ * [sequences + 1] rows before each sequence, not decreasing, or NULL for one row per sequence (rows == sequences).
+ * dtype: 0 fp32, 1 fp16, 2 bfloat16.  Strides are in elements; a head's dims lie side by side.  All index arrays are
+ * int32 on the device and are not read by the host.
  *
  * ivonar_cache_write: row r of sequence b becomes position past[b] + r - offsets[b]; a negative past[b] writes
  * nothing.  A block of 32 values with a NaN or an infinity reads back as NaN. */

@@ -9,10 +9,10 @@
 //   S^T [key][row]: A = K (converted from 4 bits with its scales in registers, exact in bf16), B = q;
 //   P = 2^(x - m), which in the MFMA's result layout is already the B operand of
 //   O^T [dim][row] += A = V (converted, then pairs of tokens brought together with v_perm), B = P.
-// A wave's tiles come straight from memory into a ring of its own in LDS, two or three of them on their way while one
-// is used, so no barrier stands in the loop.  No register crosses lanes in it besides the maxima, and those only when
-// some value exceeds the running m by a factor of 2^8 (the exponentials stay below 2^8 until then, which fp32 and bf16
-// hold as precisely as values below one).
+// A wave's tiles come straight from memory into a ring of its own in LDS, three of them (64 dims), two (128) or one
+// (256) on their way while one is used, so no barrier stands in the loop.  No register crosses lanes in it besides the
+// maxima, and those only when some value exceeds the running m by a factor of 2^8 (the exponentials stay below 2^8
+// until then, which fp32 and bf16 hold as precisely as values below one).
 // q and P are bf16 operands; q in fp16 is split into two bf16 terms and q in fp32 into three (all their bits), and P
 // into two or, for fp32 rows, three: a single term of P would leave errors of 2^-8 of sum p |v|, as much as the
 // rounding of a bf16 result that does not cancel.
@@ -188,7 +188,7 @@ __device__ __forceinline__ void load_tile(const uint8_t* base, unsigned to, int 
     dma_pair<STREAM>(buffer, to + j * 1024, 1024, lane * 16, lane * 16, j * 1024, 1024);
 #pragma unroll
   for (int j = 0; j < Stage<D>::kScaleLoads; ++j)
-    dma<4, STREAM>(buffer, to + 32 * D + j * 256, lane * 4, 32 * D + j * 256);
+    dma4<STREAM>(buffer, to + 32 * D + j * 256, lane * 4, 32 * D + j * 256);
 }
 
 template <int N>
@@ -286,7 +286,7 @@ __device__ __forceinline__ void clear_rows(const Params& p, int head) {
   const CacheAttentionArgs& a = p.a;
   const int begin = a.sequences > 0 ? max(a.offsets[0], 0) : 0;
   const int end = a.sequences > 0 ? a.offsets[a.sequences] : 0;
-  In* out = static_cast<In*>(const_cast<void*>(static_cast<const void*>(a.out)));
+  In* out = static_cast<In*>(a.out);
   const int width = p.group * D;
   for (int row = 0; row < a.rows; ++row) {
     if (row == begin) row = max(end, begin);
@@ -363,8 +363,6 @@ __device__ __forceinline__ bool share_begin(const Params& p, int block, Run& run
 // four dims and every `groups`-th part of them, in their order, several on their way at a time.  `first`, then `second`
 // and from there on `step` apart: the parts' numbers.
 constexpr int kDeviceScope = 16;  // SC1, the scope bit of store_device and load_device, of the wide buffer forms
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t parts_buffer(float* work) {
   return __builtin_amdgcn_make_buffer_rsrc(work, 0, 0x7fffffff, 0x00020000);
 }
@@ -461,6 +459,7 @@ __device__ __forceinline__ void add_parts(const Params& p, const Span& s, int he
 
 template <int D, typename In, int R, int NT, bool STREAM>
 __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention_kernel(Params p) {
+  static_assert(R != 8 || D < 256, "up to 8 rows, a lane has two scales of K at most");
   constexpr bool kNarrow = R == 8;
   constexpr int RT = kNarrow ? 1 : R / 16, kHalves = kNarrow ? 1 : 2;
   constexpr int W = D / 32, kChunks = kNarrow ? 2 * W : W, kTiles = D / 16, kPad = D + 4;
@@ -582,7 +581,7 @@ __global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void cache_attention
       m[rt] = kNoKey;
       l[rt] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) o[i][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int k = 0; k < kTiles; ++k) o[k][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
     for (; i < end; i += kWaves) {

@@ -44,20 +44,18 @@ __device__ __forceinline__ void dma16(v4u buffer, unsigned lds_base, int voffset
       : "memory");
 }
 
-// The same for pieces of BYTES (16 or 4) per lane, past the memory-side cache with STREAM.
-template <int BYTES, bool STREAM>
-__device__ __forceinline__ void dma(v4u buffer, unsigned lds_base, int voffset, int soffset) {
+// The same for pieces of 4 bytes per lane, past the memory-side cache with STREAM.
+template <bool STREAM>
+__device__ __forceinline__ void dma4(v4u buffer, unsigned lds_base, int voffset, int soffset) {
   int saved;
-#define IVO_DMA(LOAD)                                                              \
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t" LOAD "\n\t" \
-               "s_mov_b32 m0, %0"                                                  \
-               : "=&s"(saved)                                                      \
-               : "s"(lds_base), "v"(voffset), "s"(buffer), "s"(soffset)            \
+#define IVO_DMA(HINT)                                                                      \
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"                     \
+               "buffer_load_dword %2, %3, %4 offen" HINT " lds\n\ts_mov_b32 m0, %0"        \
+               : "=&s"(saved)                                                              \
+               : "s"(lds_base), "v"(voffset), "s"(buffer), "s"(soffset)                    \
                : "memory")
-  if constexpr (BYTES == 16 && STREAM) IVO_DMA("buffer_load_dwordx4 %2, %3, %4 offen nt lds");
-  if constexpr (BYTES == 16 && !STREAM) IVO_DMA("buffer_load_dwordx4 %2, %3, %4 offen lds");
-  if constexpr (BYTES == 4 && STREAM) IVO_DMA("buffer_load_dword %2, %3, %4 offen nt lds");
-  if constexpr (BYTES == 4 && !STREAM) IVO_DMA("buffer_load_dword %2, %3, %4 offen lds");
+  if constexpr (STREAM) IVO_DMA(" nt");
+  if constexpr (!STREAM) IVO_DMA("");
 #undef IVO_DMA
 }
 

@@ -19,10 +19,16 @@ infinity reads back as NaN.
 
 ``table`` [sequences, width] (int32) holds each sequence's page numbers in order; an entry outside the pages (-1, for
 instance) is no page, and so is every position past the table: nothing is written there, zeros are read, and attention
-does not see its tokens, so pages before a window may be handed back.  ``offsets`` (int32 [sequences + 1]) are the rows before each sequence in a ragged
-batch; None stands for one row per sequence.  Rows past the last sequence's (padding) are not written to the cache,
-and are zero in the results.  Index tensors stay on the device: no call reads them on the host, allocates more than
-its results and a workspace, or synchronises, so all of them can be captured into a graph.
+does not see its tokens, so pages before a window may be handed back.  ``offsets`` (int32 [sequences + 1]) are the
+rows before each sequence in a ragged batch; None stands for one row per sequence.  Rows past the last sequence's
+(padding) are not written to the cache, and are zero in the results.
+
+Index tensors stay on the device: no call reads them on the host, allocates more than its results and a workspace, or
+synchronises, so all of them can be captured into a graph.  Where blocks share a sequence's keys, ``cache_attention``
+counts them in the library's scratch of the stream, and under capture in that of the capture stream if it has made an
+eager call before, else of the device.  So graphs captured on one stream, or an eager call on that stream and a replay
+on another, must not run at the same time: their results would be undefined, and the counts they leave would spoil
+later calls until the library's ``ivonar_init`` clears them.  Eager calls on different streams may overlap.
 """
 
 from __future__ import annotations
