@@ -22,12 +22,13 @@
 // row tile's keys, the last of its blocks to end adds the parts (unscaled sums, m, sum).  More rows: row tiles are
 // split at equal lengths where there are too few of them, and a second kernel adds their parts.
 //
-// Measured (MI355X, in graphs).  One token per sequence, bound by the cache's bytes: 64 sequences of about 8000 tokens,
-// 32/8 heads of 128, bf16: 66 us, 4.8 TB/s (a stream of the same 313 MB reads at 6.5; loads alone took 64); one of
-// 131000, fp16: 36.5 us, 3.9 TB/s (142 MB more take 23 us more: the rest is filling the device and adding the parts);
-// 128 with a window of 1024, 16/4 heads of 64: 15 us, 2.4 TB/s; one of 37, fp32: 6.4 us, a chain of loads.  Chunks,
-// bound by the vector units, which convert the codes and the weights next to the matrix units' work: 512 rows over 8702
-// tokens, 32/8 heads of 128, bf16: 119 us, 600 TFLOP/s (900 counting both terms of P).
+// Measured (MI355X, calls back to back).  One token per sequence, bound by the cache's bytes: 64 sequences of 1000 to
+// 8000 tokens (288000 in all), 32/8 heads of 128, bf16: 67 us, 4.7 TB/s (a stream of the same 313 MB reads at 6.5;
+// loads alone took 64); one of 131000, fp16: 36.5 us, 3.9 TB/s (142 MB more take 23 us more: the rest is filling the
+// device and adding the parts); 128 with a window of 1024, 16/4 heads of 64: 15.2 us, 2.4 TB/s; one of 37, fp32: 6.4 us
+// in a graph, a chain of loads.  Chunks, bound by the vector units, which convert the codes and the weights next to the
+// matrix units' work: 512 rows over 8702 tokens, 32/8 heads of 128, bf16: 120 us, 590 TFLOP/s (890 counting both terms
+// of P); fp16 142 us, fp32 223 us, with more terms of q and P.
 #include "buffer_ops.hpp"
 #include "cache_layout.hpp"
 #include "ternary_device.hpp"

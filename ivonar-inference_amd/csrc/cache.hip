@@ -8,10 +8,10 @@
 // infinity gets the byte 255, which the conversions back turn into NaN.  The division and the rounding are
 // v_cvt_scalef32_pk_fp4_f32, which rounds ties to even and saturates.
 //
-// Both kernels are bound by the rows' bytes: a value costs a handful of instructions.  Measured (MI355X, traced):
-// 8190 tokens of 8 heads of 128, fp32: written in 17.4 us, read back in 15.8 us, 76 MB each, 4.4 and 4.8 TB/s (a copy
-// reaches 5.3); 65000 tokens read as bf16: 61 .. 73 us, 337 MB, 4.6 .. 5.5 TB/s.  A decode step of 64 tokens takes 3.9
-// us for either, a chain of dependent loads (offsets, page, row).
+// Both kernels are bound by the rows' bytes: a value costs a handful of instructions.  Measured (MI355X, medians of
+// traced calls): 8190 tokens of 8 heads of 128, fp32: written in 16 to 19 us, read back in 17 us, 76 MB each, 4.0 to
+// 4.8 and 4.5 TB/s (a copy reaches 5.3); 65000 tokens read as bf16: 70 us, 337 MB, 4.8 TB/s.  A decode step of 64
+// tokens takes 3.9 and 3.7 us, a chain of dependent loads (offsets, page, row).
 #include "cache_layout.hpp"
 #include "ternary_device.hpp"
 

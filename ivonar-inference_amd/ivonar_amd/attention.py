@@ -203,7 +203,8 @@ def cache_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, of
     sequence.  heads is a multiple of the cache's kv_heads: head h reads key/value head h // (heads / kv_heads).  A row
     that sees nothing is zero.  scale (default head_dim ** -0.5) multiplies q . k.  max_length, about the longest
     length, sets how keys are shared between blocks (default: what the table can hold); any value gives the same
-    result up to the order of sums."""
+    result up to the order of sums.  That sharing goes by the average rows of a sequence: single rows over very long
+    sequences and chunks of many rows are faster as two calls than as one."""
     device = _device(q, pages, table, lengths, offsets, out)
     count, kv_heads, tiles, dim, sequences, width = _geometry(pages, table, "cache_attention")
     rows, heads, q_row, q_head = _rows(q, None, dim, "q")
@@ -236,8 +237,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor | None = N
 
     offsets (int32 [sequences + 1]): the rows before each sequence; None: all rows are one sequence.  A row sees its
     sequence's rows up to its own, and with a window (0: none) only the last `window` of them and the first `sinks`
-    of the sequence.  heads is a multiple of kv_heads.  scale (default head_dim ** -0.5) multiplies q . k.  Rows that
-    do not start on 16 bytes are copied first."""
+    of the sequence.  heads is a multiple of kv_heads.  scale (default head_dim ** -0.5) multiplies q . k.  The
+    softmax's weights are rounded to that type for their product with v (their sum is fp32), which adds about as much
+    error as the rounding of the result.  Rows that do not start on 16 bytes are copied first."""
     device = _device(q, k, v, offsets, out)
     rows, heads, q_row, q_head = _rows(q, None, None, "q")
     dim = q.shape[2]

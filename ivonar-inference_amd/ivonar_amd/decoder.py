@@ -28,13 +28,14 @@ holds what is left of the prompt, since a tile's 194 dependent launches (24
 layers) cost little more at many tokens than at few (3.4 us each at 32, 4.4 at
 128, 5.9 at 256, 11 at 1024).
 
-The reference's mixers (recurrent scan, latent attention) are not part of this path: without ``attention``
-the output projection reads the V third of the entry projection's output instead
-of a mixer's output.  With ``attention`` (an ``AttentionConfig``) the thirds are the queries, keys and values
-of causal self-attention, with a sliding window and sinks if it has them: a decode step writes its token's keys and
-values into a 4-bit cache and attends to the cache; a prompt's first tile attends to its own keys and values as they
-are, in bfloat16, and later tiles to the cache.  Greedy tokens are written on the device into a ring of
-``burst`` slots, so a burst of decode steps runs as one HIP graph replay with
+The reference's mixers (recurrent scan, latent attention) are not part of this path: without ``attention`` the
+output projection reads the V third of the entry projection's output instead of a mixer's output. With
+``attention`` (an ``AttentionConfig``) the thirds are the queries, keys and values of causal self-attention,
+with a sliding window and sinks if it has them: a decode step writes its token's keys and values into a 4-bit
+cache and attends to the cache; a prompt's first tile attends to its own keys and values, rounded to bfloat16
+(window_attention takes half types, and bfloat16 has fp32's range; what it drops, 2^-9 of a value, is little
+next to the cache's 4 bits), and later tiles to the cache. Greedy tokens are written on the device into a ring
+of ``burst`` slots, so a burst of decode steps runs as one HIP graph replay with
 a single read-back, as the reference's burst graphs do (``kernel_decoder.py:694-735``).
 """
 
