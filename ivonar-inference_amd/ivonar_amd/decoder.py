@@ -103,8 +103,10 @@ class _Attention:
             raise KernelError(f"{config.heads} heads do not divide {hidden} into one of {attn.HEAD_DIMS}")
         if config.capacity <= 0:
             raise KernelError("the cache needs room for at least one token")
+        if config.window < 0 or config.sinks < 0:
+            raise KernelError("window and sinks must not be negative")
         self.config, self.shape = config, (config.heads, hidden // config.heads)
-        pages = -(-config.capacity // config.page_size)
+        pages = -(-config.capacity // max(1, config.page_size))  # cache_pages refuses other sizes
         self.pages = [attn.cache_pages(pages, *self.shape, config.page_size, device) for _ in range(layers)]
         self.table = torch.arange(pages, dtype=torch.int32, device=device).reshape(1, pages)
         # decode: the tokens before the step's and with it; a prompt's tile: the same, and the rows before and after it

@@ -100,3 +100,13 @@ def test_bound_notices_a_weight_of_one_term(count):
 
     assert (np.abs(emulated(1) - out) > 4 * limit).all()
     assert (np.abs(emulated(2) - out) <= limit).all()
+
+
+@pytest.mark.parametrize("options", [{"page_size": 0}, {"page_size": -64}, {"window": -1}, {"window": 8, "sinks": -1},
+                                     {"heads": 3}, {"capacity": 0}])
+def test_decoder_refuses_what_its_calls_would(options):
+    from ivonar_amd.decoder import AttentionConfig, _Attention
+
+    with pytest.raises(KernelError):
+        _Attention(AttentionConfig(**{"heads": 4, **options}), 256, 1, 32, torch.device("cpu"))
+    _Attention(AttentionConfig(4, window=8, sinks=1), 256, 1, 32, torch.device("cpu"))
