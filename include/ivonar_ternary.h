@@ -280,6 +280,26 @@ hipError_t ivonar_cache_write(hipStream_t stream, const void* k, const void* v, 
 hipError_t ivonar_cache_read(hipStream_t stream, const uint8_t* pages, int page_count, int kv_heads, int page_tiles,
                              int head_dim, const int32_t* table, int table_width, const int32_t* start,
                              const int32_t* offsets, int sequences, int rows, int dtype, void* k, void* v);
+/* The norm of query and key heads and their rotation, in one pass: per head row x of head_dim values,
+ * y = x * rsqrt(mean(x^2) + eps) * norm (norm [head_dim] fp32, NULL: y = x); of the first `rotary` values of y (a
+ * multiple of 16, at most head_dim) pair i, at i and rotary / 2 + i, or interleaved at 2 i and 2 i + 1, is turned by the
+ * row's position times frequencies[i] (fp32 [rotary / 2], radians).  Row r of sequence b is at past[b] + r - offsets[b].
+ * Rows of no sequence are 0 in the results, which may be q and k themselves, but not other rows that overlap them. */
+hipError_t ivonar_rotate(hipStream_t stream, const void* q, const void* k, int dtype, long long q_token_stride,
+                         long long q_head_stride, long long k_token_stride, long long k_head_stride, int heads,
+                         int kv_heads, int head_dim, int rows, const int32_t* past, const int32_t* offsets,
+                         int sequences, const float* frequencies, int rotary, int interleaved, const float* q_norm,
+                         const float* k_norm, float eps, void* q_out, void* k_out, long long q_out_token_stride,
+                         long long q_out_head_stride, long long k_out_token_stride, long long k_out_head_stride);
+/* ivonar_rotate and ivonar_cache_write of its k and of v, in one launch: the same bytes in the cache. */
+hipError_t ivonar_rotate_write(hipStream_t stream, const void* q, const void* k, const void* v, int dtype,
+                               long long q_token_stride, long long q_head_stride, long long k_token_stride,
+                               long long k_head_stride, long long v_token_stride, long long v_head_stride, int heads,
+                               int rows, uint8_t* pages, int page_count, int kv_heads, int page_tiles, int head_dim,
+                               const int32_t* table, int table_width, const int32_t* past, const int32_t* offsets,
+                               int sequences, const float* frequencies, int rotary, int interleaved,
+                               const float* q_norm, const float* k_norm, float eps, void* q_out,
+                               long long q_out_token_stride, long long q_out_head_stride);
 /* out [rows, heads, head_dim] = attention of q's rows over the cached keys and values; heads a multiple of kv_heads
  * (head h reads key/value head h / (heads / kv_heads)).  The rows of sequence b are its last ones: row r is position
  * lengths[b] - (offsets[b + 1] - offsets[b]) + r - offsets[b] and sees the positions up to its own, with a window
@@ -306,6 +326,52 @@ hipError_t ivonar_window_attention(hipStream_t stream, const void* q, const void
                                    long long k_head_stride, long long v_token_stride, long long v_head_stride,
                                    int heads, int kv_heads, int head_dim, int rows, const int32_t* offsets,
                                    int sequences, int window, int sinks, float scale, void* out);
+
+/* ------------------------------------------------------ pages of a cache
+ * A pool: refs [pages] (how many table entries hold each page) and free [(pages + 31) / 32] (bit p % 32 of word p / 32
+ * set where refs[p] is 0).  Tables are as above, page_size a power of two from 32 on.  The free page with the lowest
+ * number is given first.  Everything is on the device; nothing is read by the host.
+ *
+ * ivonar_page_reserve: sequence b gets a page for every slot that its positions lengths[b] .. lengths[b] + counts[b] - 1
+ * are the first to use and that has none, sequence by sequence.  *missing: slots that got none, for want of free pages
+ * or of table entries (they stay as they are). */
+hipError_t ivonar_page_reserve(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
+                               int table_width, const int32_t* lengths, const int32_t* counts, int sequences,
+                               int32_t* missing);
+/* Sequence b gives back the pages of its slots first[b] .. last[b] - 1 (NULL: from the first, to the last), whose
+ * entries become -1; a page that nobody holds any more is free. */
+hipError_t ivonar_page_release(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
+                               int table_width, const int32_t* first, const int32_t* last, int sequences);
+/* out_table [rows, table_width] and out_lengths replace table and lengths: row r goes on from sequence parents[r] (none
+ * outside 0 .. sequences - 1: an empty row).  The first row of a parent takes its whole row over.  Further ones share
+ * its finished pages, and a page that is not full is copied: copies [rows, 2] lists (source, target), then -1, for
+ * ivonar_page_copy.  *missing: rows for whose copy there was no page; they end with their last finished page.  Pages that
+ * no row holds any more are free after the call, not for it.  At most 8192 sequences. */
+hipError_t ivonar_page_fork(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size,
+                            const int32_t* table, int table_width, const int32_t* lengths, int sequences,
+                            const int32_t* parents, int rows, int32_t* out_table, int32_t* out_lengths, int32_t* copies,
+                            int32_t* missing);
+/* Renumbers the held pages 0 .. *live - 1: those from *live on take the free numbers below it, both in order, in refs,
+ * free and table (which has to be the pool's only one).  copies [pages / 2, 2] lists what ivonar_page_copy has to move;
+ * moved [pages] is scratch. */
+hipError_t ivonar_page_compact(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
+                               int table_width, int sequences, int32_t* copies, int32_t* moved, int32_t* live);
+/* Copies page copies[i][0] of page_bytes (a multiple of 16) to page copies[i][1]; rows with a number outside the pages
+ * (-1) are skipped.  No page may be in the list as a source and as a target, or as two targets.  copies on 8 bytes. */
+hipError_t ivonar_page_copy(hipStream_t stream, uint8_t* pages, int page_count, long long page_bytes,
+                            const int32_t* copies, int count);
+
+/* -------------------------------------------------------- scores of tokens
+ * Of every row of logits [rows, vocab] (dtype 0 fp32, 1 fp16, 2 bfloat16; rows row_stride elements apart) divided by
+ * temperature: the log probability of tokens[row] (-inf outside the vocabulary), the entropy in nats, and the `top` (at
+ * most 64 and vocab) largest logits' log probabilities and tokens, falling, of equal logits the lowest token first (NaN
+ * counts as less than all).  A row of -inf has log probabilities of -inf and entropy 0; one with a NaN or +inf has NaN.
+ * work: ivonar_log_probabilities_work bytes (-1 for sizes that the call refuses), 16-byte aligned. */
+long long ivonar_log_probabilities_work(int dtype, int rows, int vocab, int top);
+hipError_t ivonar_log_probabilities(hipStream_t stream, const void* logits, int dtype, long long row_stride, int rows,
+                                    int vocab, const int64_t* tokens, int top, float temperature, float* log_probability,
+                                    float* entropy, float* top_log_probability, int64_t* top_token, void* work,
+                                    long long work_bytes);
 
 /* ------------------------------------------------------ checkpoint checks
  * The packed-buffer tests of the reference loader (loader.py:94-112), on the

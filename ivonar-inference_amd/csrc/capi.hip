@@ -521,6 +521,176 @@ hipError_t ivonar_cache_read(hipStream_t stream, const uint8_t* pages, int page_
   return launch_cache_read(stream, a, head_dim, dtype, k, v);
 }
 
+static bool rotate_sizes(const void* q, const void* k, const void* q_out, int dtype, int heads, int kv_heads, int head_dim,
+                         int rows, const int32_t* past, const int32_t* offsets, int sequences, const float* frequencies,
+                         int rotary) {
+  if (dtype < kFloat32 || dtype > kBfloat16 || heads <= 0 || heads > 65535 || kv_heads <= 0 || kv_heads > 65535)
+    return false;
+  if (!cache_head_dim(head_dim) || rows < 0 || sequences < 0 || (offsets == nullptr && rows != sequences)) return false;
+  if (q == nullptr || k == nullptr || q_out == nullptr || (past == nullptr && sequences > 0)) return false;
+  return rotary > 0 && rotary <= head_dim && rotary % 16 == 0 && frequencies != nullptr;
+}
+
+hipError_t ivonar_rotate(hipStream_t stream, const void* q, const void* k, int dtype, long long q_token_stride,
+                         long long q_head_stride, long long k_token_stride, long long k_head_stride, int heads,
+                         int kv_heads, int head_dim, int rows, const int32_t* past, const int32_t* offsets,
+                         int sequences, const float* frequencies, int rotary, int interleaved, const float* q_norm,
+                         const float* k_norm, float eps, void* q_out, void* k_out, long long q_out_token_stride,
+                         long long q_out_head_stride, long long k_out_token_stride, long long k_out_head_stride) {
+  if (!rotate_sizes(q, k, q_out, dtype, heads, kv_heads, head_dim, rows, past, offsets, sequences, frequencies, rotary) ||
+      k_out == nullptr)
+    return hipErrorInvalidValue;
+  const CacheArgs a{nullptr, nullptr, past, offsets, 0, 0, kv_heads, 0, sequences, rows};
+  const RotateArgs r{q,
+                     k,
+                     nullptr,
+                     q_out,
+                     k_out,
+                     RowStrides{q_token_stride, q_head_stride},
+                     RowStrides{k_token_stride, k_head_stride},
+                     RowStrides{0, 0},
+                     RowStrides{q_out_token_stride, q_out_head_stride},
+                     RowStrides{k_out_token_stride, k_out_head_stride},
+                     q_norm,
+                     k_norm,
+                     frequencies,
+                     heads,
+                     rotary,
+                     interleaved != 0,
+                     eps};
+  return launch_rotate(stream, a, r, head_dim, dtype);
+}
+
+hipError_t ivonar_rotate_write(hipStream_t stream, const void* q, const void* k, const void* v, int dtype,
+                               long long q_token_stride, long long q_head_stride, long long k_token_stride,
+                               long long k_head_stride, long long v_token_stride, long long v_head_stride, int heads,
+                               int rows, uint8_t* pages, int page_count, int kv_heads, int page_tiles, int head_dim,
+                               const int32_t* table, int table_width, const int32_t* past, const int32_t* offsets,
+                               int sequences, const float* frequencies, int rotary, int interleaved,
+                               const float* q_norm, const float* k_norm, float eps, void* q_out,
+                               long long q_out_token_stride, long long q_out_head_stride) {
+  int shift = 0;
+  if (!cache_geometry(pages, page_count, kv_heads, page_tiles, head_dim, table, table_width, sequences, rows, &shift))
+    return hipErrorInvalidValue;
+  if (!rotate_sizes(q, k, q_out, dtype, heads, kv_heads, head_dim, rows, past, offsets, sequences, frequencies, rotary) ||
+      v == nullptr)
+    return hipErrorInvalidValue;
+  const CacheArgs a{pages, table, past, offsets, page_count, shift, kv_heads, table_width, sequences, rows};
+  const RotateArgs r{q,
+                     k,
+                     v,
+                     q_out,
+                     nullptr,
+                     RowStrides{q_token_stride, q_head_stride},
+                     RowStrides{k_token_stride, k_head_stride},
+                     RowStrides{v_token_stride, v_head_stride},
+                     RowStrides{q_out_token_stride, q_out_head_stride},
+                     RowStrides{0, 0},
+                     q_norm,
+                     k_norm,
+                     frequencies,
+                     heads,
+                     rotary,
+                     interleaved != 0,
+                     eps};
+  return launch_rotate(stream, a, r, head_dim, dtype);
+}
+
+// A pool of at most 2^27 pages, and tables of at most 2^31 - 1 entries whose sequences have at most 2^30 tokens.
+static bool pool_sizes(int32_t* refs, int32_t* free, int pages, int page_size, const int32_t* table, int table_width,
+                       int sequences, PoolArgs* pool) {
+  if (refs == nullptr || free == nullptr || pages <= 0 || pages > (1 << 27)) return false;
+  if (page_size < kCacheTile || (page_size & (page_size - 1)) != 0) return false;
+  if ((table == nullptr && sequences > 0) || table_width <= 0 || sequences < 0) return false;
+  if ((long long)table_width * page_size > (1LL << 30) || (long long)table_width * sequences > 0x7fffffffLL) return false;
+  *pool = PoolArgs{refs, free, pages, __builtin_ctz((unsigned)page_size)};
+  return true;
+}
+
+hipError_t ivonar_page_reserve(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
+                               int table_width, const int32_t* lengths, const int32_t* counts, int sequences,
+                               int32_t* missing) {
+  PoolArgs pool{};
+  if (!pool_sizes(refs, free, pages, page_size, table, table_width, sequences, &pool) || missing == nullptr ||
+      ((lengths == nullptr || counts == nullptr) && sequences > 0))
+    return hipErrorInvalidValue;
+  return launch_page_reserve(stream, pool, table, table_width, lengths, counts, sequences, missing);
+}
+
+hipError_t ivonar_page_release(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
+                               int table_width, const int32_t* first, const int32_t* last, int sequences) {
+  PoolArgs pool{};
+  if (!pool_sizes(refs, free, pages, page_size, table, table_width, sequences, &pool)) return hipErrorInvalidValue;
+  return launch_page_release(stream, pool, table, table_width, first, last, sequences);
+}
+
+hipError_t ivonar_page_fork(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size,
+                            const int32_t* table, int table_width, const int32_t* lengths, int sequences,
+                            const int32_t* parents, int rows, int32_t* out_table, int32_t* out_lengths, int32_t* copies,
+                            int32_t* missing) {
+  PoolArgs pool{};
+  if (!pool_sizes(refs, free, pages, page_size, table, table_width, sequences, &pool) || rows < 0 ||
+      sequences > kMaxPoolSequences || (long long)rows * table_width > 0x7fffffffLL || missing == nullptr ||
+      (lengths == nullptr && sequences > 0))
+    return hipErrorInvalidValue;
+  if (rows > 0 && (parents == nullptr || out_table == nullptr || out_lengths == nullptr || copies == nullptr ||
+                   out_table == table || out_lengths == lengths))
+    return hipErrorInvalidValue;
+  return launch_page_fork(stream, pool, ForkArgs{table, lengths, parents, out_table, out_lengths, copies, missing,
+                                                 table_width, sequences, rows});
+}
+
+hipError_t ivonar_page_compact(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
+                               int table_width, int sequences, int32_t* copies, int32_t* moved, int32_t* live) {
+  PoolArgs pool{};
+  if (!pool_sizes(refs, free, pages, page_size, table, table_width, sequences, &pool) || moved == nullptr ||
+      live == nullptr || (copies == nullptr && pages > 1))
+    return hipErrorInvalidValue;
+  return launch_page_compact(stream, pool, table, (long long)table_width * sequences, copies, moved, live);
+}
+
+hipError_t ivonar_page_copy(hipStream_t stream, uint8_t* pages, int page_count, long long page_bytes,
+                            const int32_t* copies, int count) {
+  if (pages == nullptr || !aligned16(pages) || page_count <= 0 || page_bytes <= 0 || (page_bytes & 15) != 0 ||
+      page_bytes > (1LL << 40) || count < 0 || (copies == nullptr && count > 0) || ((uintptr_t)copies & 7u) != 0)
+    return hipErrorInvalidValue;
+  return launch_page_copy(stream, pages, page_count, page_bytes, copies, count);
+}
+
+static bool score_sizes(int dtype, int rows, int vocab, int top) {
+  return dtype >= kFloat32 && dtype <= kBfloat16 && rows >= 0 && vocab > 0 && vocab <= (1 << 30) && top >= 0 &&
+         top <= kMaxScoreTop && top <= vocab;
+}
+
+long long ivonar_log_probabilities_work(int dtype, int rows, int vocab, int top) {
+  if (!score_sizes(dtype, rows, vocab, top)) return -1;
+  ScoreArgs a{};
+  a.dtype = dtype;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.top = top;
+  return score_work(a);
+}
+
+hipError_t ivonar_log_probabilities(hipStream_t stream, const void* logits, int dtype, long long row_stride, int rows,
+                                    int vocab, const int64_t* tokens, int top, float temperature, float* log_probability,
+                                    float* entropy, float* top_log_probability, int64_t* top_token, void* work,
+                                    long long work_bytes) {
+  if (!score_sizes(dtype, rows, vocab, top) || !(temperature > 0.0f) || !isfinite(temperature) ||
+      !isfinite(2.0f / temperature))
+    return hipErrorInvalidValue;
+  if (rows == 0) return hipSuccess;
+  if (logits == nullptr || tokens == nullptr || log_probability == nullptr || entropy == nullptr ||
+      (top > 0 && (top_log_probability == nullptr || top_token == nullptr)) ||
+      ((uintptr_t)logits & (dtype == kFloat32 ? 3u : 1u)) != 0)
+    return hipErrorInvalidValue;
+  const ScoreArgs a{logits,    row_stride, tokens, log_probability, entropy, top_log_probability,
+                    top_token, static_cast<float*>(work), dtype, rows, vocab, top, 1.0f / temperature};
+  const long long need = score_work(a);
+  if (need > 0 && (work == nullptr || !aligned16(work) || work_bytes < need)) return hipErrorInvalidValue;
+  return launch_score(stream, a);
+}
+
 static bool attention_sizes(int dtype, int heads, int kv_heads, int head_dim, int sequences, int rows, int window,
                             int sinks, float scale) {
   return dtype >= kFloat32 && dtype <= kBfloat16 && kv_heads > 0 && kv_heads <= 65535 && heads > 0 &&

@@ -200,6 +200,25 @@ hipError_t launch_sample_token(hipStream_t stream, const float* logits, const fl
                                const float* penalty, const float* inverse_penalty, uint8_t* seen,
                                const int64_t* top_k, const float* uniform, int64_t* token, int64_t* history,
                                int vocab);
+// Log probabilities of given tokens, entropy and the largest logits of rows of logits.
+constexpr int kMaxScoreTop = 64;
+struct ScoreArgs {
+  const void* logits;
+  long long row_stride;
+  const int64_t* tokens;  // [rows]
+  float* log_probability;  // [rows]
+  float* entropy;          // [rows]
+  float* top_log_probability;  // [rows, top]
+  int64_t* top_token;
+  float* work;
+  int dtype;
+  int rows;
+  int vocab;
+  int top;
+  float inverse_temperature;
+};
+long long score_work(const ScoreArgs& a);
+hipError_t launch_score(hipStream_t stream, const ScoreArgs& a);
 // Reserved codes in a packed operand (flag 1), non-finite (2) or non-positive
 // (4) fp16 scales, ORed into flags[0]; packed and scales 16-byte aligned.
 hipError_t launch_validate(hipStream_t stream, const uint8_t* packed, long long packed_bytes, const uint16_t* scales,
@@ -232,6 +251,60 @@ struct RowStrides {
 hipError_t launch_cache_write(hipStream_t stream, const CacheArgs& a, int head_dim, int dtype, const void* k,
                               const void* v, RowStrides ks, RowStrides vs);
 hipError_t launch_cache_read(hipStream_t stream, const CacheArgs& a, int head_dim, int dtype, void* k, void* v);
+
+// Norm and rotation of q's and k's rows; with v, k and v go into the cache instead of k_out.
+struct RotateArgs {
+  const void* q;
+  const void* k;
+  const void* v;  // null: no cache
+  void* q_out;
+  void* k_out;
+  RowStrides q_strides;
+  RowStrides k_strides;
+  RowStrides v_strides;
+  RowStrides q_out_strides;
+  RowStrides k_out_strides;
+  const float* q_norm;  // [head_dim]; null: no norm
+  const float* k_norm;
+  const float* frequencies;  // [rotary / 2] radians per position
+  int heads;
+  int rotary;
+  bool interleaved;
+  float eps;
+  bool aligned = false;  // the rows of q, k and v start on 16 bytes
+  bool out_aligned = false;
+};
+hipError_t launch_rotate(hipStream_t stream, const CacheArgs& a, RotateArgs r, int head_dim, int dtype);
+
+// The pages of a cache: how many table entries hold each, and a bit for each that none holds.
+struct PoolArgs {
+  int* refs;  // [pages]
+  int* free;  // [(pages + 31) / 32]
+  int pages;
+  int page_shift;  // log2 of a page's tokens
+};
+constexpr int kMaxPoolSequences = 8192;
+struct ForkArgs {
+  const int* table;  // [sequences, width]
+  const int* lengths;
+  const int* parents;  // [rows]
+  int* out_table;      // [rows, width]
+  int* out_lengths;
+  int* copies;   // [rows, 2]: source and target pages, then -1
+  int* missing;  // pages that there were none for
+  int width;
+  int sequences;
+  int rows;
+};
+hipError_t launch_page_reserve(hipStream_t stream, const PoolArgs& p, int* table, int width, const int* lengths,
+                               const int* counts, int sequences, int* missing);
+hipError_t launch_page_release(hipStream_t stream, const PoolArgs& p, int* table, int width, const int* first,
+                               const int* last, int sequences);
+hipError_t launch_page_fork(hipStream_t stream, const PoolArgs& p, const ForkArgs& a);
+hipError_t launch_page_compact(hipStream_t stream, const PoolArgs& p, int* table, long long entries, int* copies,
+                               int* moved, int* live);
+hipError_t launch_page_copy(hipStream_t stream, uint8_t* pages, int page_count, long long page_bytes, const int* copies,
+                            int count);
 
 // Attention of q's rows over the 4-bit cache.
 struct CacheAttentionArgs {

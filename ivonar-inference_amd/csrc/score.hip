@@ -1,0 +1,440 @@
+// Log probabilities of given tokens, the entropy, and the likeliest alternatives, of rows of logits, in one pass.
+//
+// For a row x of V logits and a temperature T, with m = max x, z_i = (x_i - m) / T, S = sum e^z_i, U = sum z_i e^z_i:
+//   log p_i = z_i - log S,   H = -sum p_i log p_i = log S - U / S.
+// m, S and U are kept per thread in fp32 and rescaled when a chunk raises m: S' = f S, U' = f (U + d S) for a maximum
+// that rises by -d T, f = e^d.  A logit of -inf has no weight; a row of nothing else has log probabilities of -inf and
+// no entropy.  A NaN or +inf makes all of its row's numbers NaN.
+//
+// The `top` largest logits are found in the same pass.  A logit's key is its value as an ordered number, then its index
+// from the end, so no two keys are alike and ties go to the lowest index; a NaN has the lowest value.  A wave keeps the
+// 64 largest keys that it has met, sorted over its lanes, and a bound below which a key cannot be among the row's top:
+// the top'th of them, or of the first chunk's per-lane maxima, or what another wave of the row has found.  Most chunks
+// hold no logit above the bound, which their maxima tell.  Keys above it go through a buffer in LDS and are sorted and
+// merged 64 at a time.
+//
+// A wave takes 2048 logits at a time, 32 per lane; the next ones are under way while these are used.  Few rows are
+// split between blocks, whose results a second kernel joins.
+#include "internal.hpp"
+#include "ternary_device.hpp"
+
+namespace ivo {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kValues = 32;                 // logits of a lane at a time
+constexpr int kWaveChunk = 64 * kValues;    // and of a wave
+constexpr int kBuffer = 128;                // keys above the bound that a wave holds before it merges 64
+constexpr float kLowest = -3.402823466e38f;
+typedef unsigned long long Key;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+struct Params {
+  ScoreArgs a;
+  float scale;   // log2(e) / T
+  int splits;    // blocks that share a row
+  int row_waves;  // waves of a block that share a row: 1 or kWaves
+};
+
+// What a part of a row leaves: m, S, U (in units of log 2), and its largest keys.
+struct Part {
+  float m, sum, weighted;
+  Key list;  // of 64, this lane's
+};
+constexpr int kPartFloats = 4 + 2 * 64;
+
+template <typename In>
+__device__ __forceinline__ In minus_infinity();
+template <>
+__device__ __forceinline__ float minus_infinity<float>() { return -INFINITY; }
+template <>
+__device__ __forceinline__ Half minus_infinity<Half>() { return Half{0xfc00u}; }
+template <>
+__device__ __forceinline__ Bfloat minus_infinity<Bfloat>() { return Bfloat{0xff80u}; }
+// 16 bytes of logits as fp32.
+template <typename In>
+__device__ __forceinline__ void unpack(const u32x4& words, float* x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(In) == 4) {
+      x[j] = __uint_as_float(words[j]);
+    } else {
+      x[2 * j] = to_float(In{(uint16_t)words[j]});
+      x[2 * j + 1] = to_float(In{(uint16_t)(words[j] >> 16)});
+    }
+  }
+}
+
+__device__ __forceinline__ unsigned ordered(float x) {
+  const unsigned bits = __float_as_uint(x + 0.0f);  // -0 counts as 0
+  const unsigned key = bits ^ ((unsigned)((int)bits >> 31) | 0x80000000u);
+  return x != x ? 0u : key;
+}
+__device__ __forceinline__ float value_of(Key key) {
+  const unsigned high = (unsigned)(key >> 32);
+  if (high == 0u) return NAN;
+  return __uint_as_float(high & 0x80000000u ? high ^ 0x80000000u : ~high);
+}
+__device__ __forceinline__ Key key_of(float x, int index) {
+  return (Key)ordered(x) << 32 | (unsigned)~index;
+}
+
+// The value of lane ^ X.
+template <int X>
+__device__ __forceinline__ unsigned xor_lane(unsigned v) {
+  if constexpr (X == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false);
+  if constexpr (X == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false);
+  if constexpr (X == 4)  // the mirror of eight lanes, then of four
+    return (unsigned)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF,
+                                              false);
+  if constexpr (X == 8) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, false);
+  if constexpr (X == 16) {
+    const auto swapped = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? swapped[0] : swapped[1];
+  }
+  if constexpr (X == 32) {
+    const auto swapped = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? swapped[0] : swapped[1];
+  }
+}
+template <int X>
+__device__ __forceinline__ float xor_lane(float v) { return __uint_as_float(xor_lane<X>(__float_as_uint(v))); }
+
+// Compares with lane ^ X and keeps the larger key or the smaller one.
+template <int X>
+__device__ __forceinline__ Key keep(Key key, bool larger) {
+  const Key other = (Key)xor_lane<X>((unsigned)(key >> 32)) << 32 | xor_lane<X>((unsigned)key);
+  return (other > key) == larger ? other : key;
+}
+// Keys that rise and then fall (or the reverse) over SIZE lanes, sorted: falling where `falling`.
+template <int SIZE>
+__device__ __forceinline__ Key merge_lanes(Key key, bool falling) {
+  if constexpr (SIZE > 1) {
+    key = keep<SIZE / 2>(key, ((threadIdx.x & (SIZE / 2)) == 0) == falling);
+    key = merge_lanes<SIZE / 2>(key, falling);
+  }
+  return key;
+}
+// Sorted over the wave, rising from lane 0 on.
+template <int SIZE = 64>
+__device__ __forceinline__ Key sort_lanes(Key key) {
+  if constexpr (SIZE > 2) key = sort_lanes<SIZE / 2>(key);
+  return merge_lanes<SIZE>(key, SIZE < 64 && (threadIdx.x & SIZE) != 0);
+}
+// The 64 largest of a falling list and a rising one, falling.
+__device__ __forceinline__ Key join(Key falling, Key rising) {
+  return merge_lanes<64>(falling > rising ? falling : rising, true);
+}
+__device__ __forceinline__ Key lane_key(Key key, int lane) {
+  return (Key)(unsigned)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)key, lane);
+}
+
+__device__ __forceinline__ float all_max(float v) {
+  v = fmaxf(v, xor_lane<1>(v));
+  v = fmaxf(v, xor_lane<2>(v));
+  v = fmaxf(v, xor_lane<4>(v));
+  v = fmaxf(v, xor_lane<8>(v));
+  v = fmaxf(v, xor_lane<16>(v));
+  return fmaxf(v, xor_lane<32>(v));
+}
+__device__ __forceinline__ float all_sum(float v) {
+  v += xor_lane<1>(v);
+  v += xor_lane<2>(v);
+  v += xor_lane<4>(v);
+  v += xor_lane<8>(v);
+  v += xor_lane<16>(v);
+  return v + xor_lane<32>(v);
+}
+
+// z no further down than where its weight is zero: zero times the result is zero.
+__device__ __forceinline__ float bounded(float z) { return fmaxf(z, -1000.0f); }
+
+// S and U moved to the maximum `to`.
+__device__ __forceinline__ void raise(float& m, float& sum, float& weighted, float to, float scale) {
+  const float d = bounded((m - to) * scale);
+  const float factor = __builtin_amdgcn_exp2f(d);
+  weighted = fmaf(sum, d, weighted) * factor;
+  sum *= factor;
+  m = to;
+}
+
+// The results of a row, by one wave that holds it whole.
+__device__ __forceinline__ void finish(const Params& p, int row, const Part& part) {
+  const ScoreArgs& a = p.a;
+  const int lane = threadIdx.x & 63;
+  const float log_sum = logf(part.sum);
+  const bool none = part.sum == 0.0f;
+  auto log_probability = [&](float x) { return none ? -INFINITY : (x - part.m) * a.inverse_temperature - log_sum; };
+  if (lane == 0) {
+    const int64_t token = a.tokens[row];
+    float chosen = -INFINITY;
+    if (token >= 0 && token < a.vocab) {
+      const long long at = row * a.row_stride + token;
+      const float x = a.dtype == kFloat32 ? static_cast<const float*>(a.logits)[at]
+                      : a.dtype == kFloat16 ? to_float(static_cast<const Half*>(a.logits)[at])
+                                            : to_float(static_cast<const Bfloat*>(a.logits)[at]);
+      chosen = log_probability(x);
+    }
+    a.log_probability[row] = chosen;
+    a.entropy[row] = none ? 0.0f : log_sum - 0.69314718055994530942f * (part.weighted / part.sum);
+  }
+  if (lane < a.top) {
+    const long long at = (long long)row * a.top + lane;
+    a.top_log_probability[at] = log_probability(value_of(part.list));
+    a.top_token[at] = (int64_t)(int)~(unsigned)part.list;
+  }
+}
+
+template <typename In, bool TOP>
+__global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
+  constexpr int kVec = 16 / sizeof(In), kVectors = kValues / kVec;
+  const ScoreArgs& a = p.a;
+  __shared__ Key buffers[TOP ? kWaves : 1][TOP ? kBuffer : 1];
+  __shared__ Key bounds[kWaves];  // of each row of the block, the best bound so far
+  __shared__ float sums[kWaves][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int sub = wave & (p.row_waves - 1), first_wave = wave - sub;
+  const int split = blockIdx.x % p.splits;
+  const long long row_id = (long long)(blockIdx.x / p.splits) * (kWaves / p.row_waves) + wave / p.row_waves;
+  const bool there = row_id < a.rows;
+  const int row = (int)(there ? row_id : a.rows - 1);
+  if (TOP) {
+    if (threadIdx.x < kWaves) bounds[threadIdx.x] = 0;
+    __syncthreads();
+  }
+
+  // Element e of the row, counted from the 16 bytes that its first logit lies in, is logit e - lead.
+  const In* begin = static_cast<const In*>(a.logits) + row * a.row_stride;
+  const int lead = (int)(((uintptr_t)begin & 15u) / sizeof(In));
+  const In* base = begin - lead;
+  const long long end = (long long)lead + a.vocab;
+  const int chunks = there ? (int)((end + kWaveChunk - 1) / kWaveChunk) : 0;
+  const int step = p.splits * p.row_waves;
+  auto load = [&](int chunk, u32x4 (&to)[kVectors]) {
+    const long long from = (long long)chunk * kWaveChunk;
+    if (from >= lead && from + kWaveChunk <= end) {
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v)
+        to[v] = reinterpret_cast<const u32x4*>(base + from)[v * 64 + lane];
+    } else {
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) {
+        const long long e = from + (v * 64 + lane) * kVec;
+        In values[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          values[j] = minus_infinity<In>();
+          if (e + j >= lead && e + j < end) values[j] = base[e + j];
+        }
+        __builtin_memcpy(&to[v], values, 16);
+      }
+    }
+  };
+
+  float m = kLowest, sum = 0.0f, weighted = 0.0f;
+  Key list = 0, bound = 0;
+  int held = 0;  // keys in the buffer
+  Key* buffer = buffers[TOP ? wave : 0];
+  // Merges the first `count` keys of the buffer into the list.
+  auto merge = [&](int count) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    Key key = buffer[lane];
+    key = lane < count ? key : 0;
+    list = join(list, sort_lanes(key));
+    const Key last = lane_key(list, a.top - 1);
+    bound = last > bound ? last : bound;
+    if (lane == 0) atomicMax(&bounds[first_wave], bound);
+  };
+
+  u32x4 current[kVectors], next[kVectors];
+  int chunk = split * p.row_waves + sub;
+  if (chunk < chunks) load(chunk, current);
+  for (; chunk < chunks; chunk += step) {
+    if (chunk + step < chunks) load(chunk + step, next);
+    float x[kValues];
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) unpack<In>(current[v], x + v * kVec);
+    float most = x[0];
+#pragma unroll
+    for (int j = 1; j < kValues; ++j) most = fmaxf(most, x[j]);
+    if (most > m) raise(m, sum, weighted, most, p.scale);
+    float part_sum[2] = {}, part_weighted[2] = {};
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) {
+      // The difference first: a scaled logit of the type's lowest value may overflow.
+      const float z = (x[j] - m) * p.scale;
+      const float weight = __builtin_amdgcn_exp2f(z);
+      part_sum[j & 1] += weight;
+      part_weighted[j & 1] = fmaf(bounded(z), weight, part_weighted[j & 1]);
+    }
+    sum += part_sum[0] + part_sum[1];
+    weighted += part_weighted[0] + part_weighted[1];
+
+    if constexpr (TOP) {
+      const Key shared = *(volatile Key*)&bounds[first_wave];
+      bound = shared > bound ? shared : bound;
+      const int offset = (int)((long long)chunk * kWaveChunk - lead) + lane * kVec;  // the lane's first logit
+      auto index_of = [&](int j) { return offset + j / kVec * (64 * kVec) + j % kVec; };
+      if (bound == 0) {
+        // Of the lanes' largest keys the top'th is no larger than that of all keys.
+        int best = -1;
+#pragma unroll
+        for (int j = kValues - 1; j >= 0; --j) {
+          const int index = index_of(j);
+          best = x[j] == most && (unsigned)index < (unsigned)a.vocab ? index : best;
+        }
+        const Key key = sort_lanes(best >= 0 ? key_of(most, best) : 0);
+        const Key last = lane_key(key, 64 - a.top);
+        bound = last > 0 ? last - 1 : 0;
+      }
+      const float least = value_of(bound);  // NaN: none yet
+      if (__ballot(!(most < least)) != 0ull) {
+        unsigned above = 0;  // bit j: logit j may be
+#pragma unroll
+        for (int j = 0; j < kValues; ++j) above |= !(x[j] < least) ? 1u << j : 0u;
+        while (__ballot(above != 0u) != 0ull) {
+          bool add = false;
+          Key key = 0;
+          if (above != 0u) {
+            const int j = __builtin_ctz(above);
+            above &= above - 1u;
+            const int index = index_of(j);
+            if ((unsigned)index < (unsigned)a.vocab) {
+              key = key_of(to_float(begin[index]), index);
+              add = key > bound;
+            }
+          }
+          const unsigned long long adds = __ballot(add);
+          if (add) buffer[held + __popcll(adds & ((1ull << lane) - 1ull))] = key;
+          held += __popcll(adds);
+          if (held >= 64) {
+            merge(64);
+            const Key rest = buffer[64 + lane];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            buffer[lane] = rest;
+            held -= 64;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) current[v] = next[v];
+  }
+  if (TOP && held > 0) merge(held);
+
+  Part part;
+  part.m = all_max(m);
+  raise(m, sum, weighted, part.m, p.scale);
+  part.sum = all_sum(sum);
+  part.weighted = all_sum(weighted);
+  part.list = list;
+  if (p.row_waves > 1) {
+    if (lane == 0) {
+      sums[wave][0] = part.m;
+      sums[wave][1] = part.sum;
+      sums[wave][2] = part.weighted;
+    }
+    if (TOP) buffer[lane] = list;
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      float other_m = sums[w][0], other_sum = sums[w][1], other_weighted = sums[w][2];
+      const float top = fmaxf(part.m, other_m);
+      raise(part.m, part.sum, part.weighted, top, p.scale);
+      raise(other_m, other_sum, other_weighted, top, p.scale);
+      part.sum += other_sum;
+      part.weighted += other_weighted;
+      if (TOP) part.list = join(part.list, buffers[TOP ? w : 0][TOP ? 63 - lane : 0]);
+    }
+  }
+  if (!there) return;
+  if (p.splits == 1) {
+    finish(p, row, part);
+  } else {
+    float* to = a.work + ((long long)row * p.splits + split) * kPartFloats;
+    if (lane == 0) *reinterpret_cast<float4*>(to) = float4{part.m, part.sum, part.weighted, 0.0f};
+    if (TOP) reinterpret_cast<Key*>(to + 4)[lane] = part.list;
+  }
+}
+
+// Joins the parts of split rows, a wave per row.
+__global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
+  const int lane = threadIdx.x & 63;
+  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+  if (row >= p.a.rows) return;
+  const float* from = p.a.work + (long long)row * p.splits * kPartFloats;
+  Part part;
+  part.m = kLowest;
+  part.sum = part.weighted = 0.0f;
+  part.list = 0;
+  for (int i = lane; i < p.splits; i += 64) {
+    float4 other = *reinterpret_cast<const float4*>(from + (long long)i * kPartFloats);
+    const float top = fmaxf(part.m, other.x);
+    raise(part.m, part.sum, part.weighted, top, p.scale);
+    raise(other.x, other.y, other.z, top, p.scale);
+    part.sum += other.y;
+    part.weighted += other.z;
+  }
+  const float top = all_max(part.m);
+  raise(part.m, part.sum, part.weighted, top, p.scale);
+  part.sum = all_sum(part.sum);
+  part.weighted = all_sum(part.weighted);
+  if (p.a.top > 0)
+    for (int i = 0; i < p.splits; ++i)
+      part.list = join(part.list, reinterpret_cast<const Key*>(from + (long long)i * kPartFloats + 4)[63 - lane]);
+  finish(p, row, part);
+}
+
+// Blocks that few rows are split into.
+constexpr long long kWanted = 1024;
+// Rows of up to this many chunks get a wave each.
+constexpr int kWaveRowChunks = 2;
+
+Params plan(const ScoreArgs& a) {
+  Params p{a, 1.44269504088896340736f * a.inverse_temperature, 1, kWaves};
+  const long long chunks = ((long long)a.vocab + 7 + kWaveChunk - 1) / kWaveChunk;
+  if (chunks <= kWaveRowChunks && a.rows >= kWanted) {
+    p.row_waves = 1;
+    return p;
+  }
+  const long long wanted = (kWanted + a.rows - 1) / (a.rows > 0 ? a.rows : 1);
+  const long long most = (chunks + kWaves - 1) / kWaves;
+  p.splits = (int)(wanted < most ? wanted : most);
+  return p;
+}
+
+template <typename In>
+void run(hipStream_t stream, const Params& p, unsigned blocks) {
+  if (p.a.top > 0)
+    hipLaunchKernelGGL((score_kernel<In, true>), dim3(blocks), dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((score_kernel<In, false>), dim3(blocks), dim3(kThreads), 0, stream, p);
+}
+
+}  // namespace
+
+long long score_work(const ScoreArgs& a) {
+  const Params p = plan(a);
+  return p.splits == 1 ? 0 : (long long)a.rows * p.splits * kPartFloats * 4;
+}
+
+hipError_t launch_score(hipStream_t stream, const ScoreArgs& a) {
+  if (a.rows == 0) return hipSuccess;
+  const Params p = plan(a);
+  const int block_rows = kWaves / p.row_waves;
+  const long long blocks = ((long long)a.rows + block_rows - 1) / block_rows * p.splits;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (a.dtype == kFloat32)
+    run<float>(stream, p, (unsigned)blocks);
+  else if (a.dtype == kFloat16)
+    run<Half>(stream, p, (unsigned)blocks);
+  else
+    run<Bfloat>(stream, p, (unsigned)blocks);
+  if (p.splits > 1)
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((a.rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace ivo

@@ -7,6 +7,10 @@ The reference keeps fp16 keys and values and attends to them in ``attention_step
   [pages, kv_heads, page_size / 32, 34 * head_dim];
 * ``cache_write(pages, k, v, table, past, offsets)``: new tokens' keys and values, quantised as they are written;
 * ``cache_read(pages, table, start, offsets, rows, dtype)`` -> (k, v): stretches of the sequences as tensors;
+* ``rotate(q, k, past, frequencies, offsets, ..)`` -> (q, k): the RMS norm of every query and key head and its rotation
+  by the token's position; ``rotate_write(pages, q, k, v, table, past, frequencies, ..)`` -> q: the same, with the new
+  keys and values written into the cache, as ``cache_write`` after it would, in one launch;
+  ``rotary_frequencies(rotary, base)``: the usual frequencies;
 * ``cache_attention(q, pages, table, lengths, offsets, window, sinks)``: the last rows of each sequence (one token
   while decoding, several for a chunk of a prompt) over all of its cached tokens, or over a sliding window and the
   first few (sinks);
@@ -78,6 +82,9 @@ def _device(first: Tensor, *others: Tensor | None) -> int:
 
 
 def _run(name: str, index: int, *args) -> None:
+    if index != torch._C._cuda_getDevice():  # a launch goes to the current device
+        with torch.cuda.device(index):
+            return _run(name, index, *args)
     status = getattr(library(), name)(_raw_stream(index), *args)
     if status != 0:
         check(status, name)
@@ -164,6 +171,100 @@ def cache_read(pages: Tensor, table: Tensor, start: Tensor | None, offsets: Tens
         _run("ivonar_cache_read", device, pages.data_ptr(), count, heads, tiles, dim, table.data_ptr(), width,
              _address(start), _address(offsets), sequences, rows, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
     return k, v
+
+
+def rotary_frequencies(rotary: int, base: float = 10000.0, factor: float = 1.0,
+                       device: torch.device | str = "cuda") -> Tensor:
+    """base ** (-2 i / rotary) / factor radians per position for i = 0 .. rotary / 2 - 1, in fp32; a factor above one
+    stretches the positions."""
+    if rotary <= 0 or rotary % 16:
+        raise KernelError(f"rotary {rotary} is not a positive multiple of 16")
+    if not (base > 0 and math.isfinite(base) and factor > 0 and math.isfinite(factor)):
+        raise KernelError("base and factor must be positive and finite")
+    pair = torch.arange(rotary // 2, dtype=torch.float64)
+    return (base ** (-2.0 * pair / rotary) / factor).float().to(device)
+
+
+def _turns(q: Tensor, k: Tensor, past: Tensor, frequencies: Tensor, offsets: Tensor | None, q_norm: Tensor | None,
+           k_norm: Tensor | None, eps: float, kv_heads: int | None = None, dim: int | None = None):
+    """Checks what rotate and rotate_write share; (rows, heads, kv_heads, head_dim, sequences, q's strides, k's strides,
+    rotary)."""
+    rows, heads, q_row, q_head = _rows(q, None, dim, "q")
+    dim = q.shape[2]
+    if dim not in HEAD_DIMS:
+        raise KernelError(f"head_dim {dim} is not one of {HEAD_DIMS}")
+    k_rows, kv_heads, k_row, k_head = _rows(k, kv_heads, dim, "k")
+    if k_rows != rows or k.dtype is not q.dtype:
+        raise KernelError("q and k must have the same rows and type")
+    if not 0 < heads <= 65535 or not 0 < kv_heads <= 65535:
+        raise KernelError(f"{heads} and {kv_heads} heads are not 1 to 65535")
+    sequences = past.shape[0] if past.dim() == 1 else -1
+    _index(past, max(sequences, 0), "past")
+    _offsets(offsets, sequences, rows)
+    rotary = 2 * frequencies.shape[0] if frequencies.dim() == 1 else 0
+    if frequencies.dtype is not torch.float32 or not frequencies.is_contiguous() or not 0 < rotary <= dim or rotary % 16:
+        raise KernelError(f"frequencies must be contiguous float32 [rotary / 2], rotary a multiple of 16 up to {dim}")
+    for norm, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if norm is not None and (norm.dtype is not torch.float32 or norm.shape != (dim,) or not norm.is_contiguous()):
+            raise KernelError(f"{name} must be contiguous float32 [{dim}]")
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise KernelError("eps must not be negative")
+    return rows, heads, kv_heads, dim, sequences, (q_row, q_head), (k_row, k_head), rotary
+
+
+def _like(x: Tensor, out: Tensor | None, what: str) -> Tensor:
+    """A contiguous result of x's shape and type, or `out` if it is of them, with any row and head stride."""
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    if out.shape != x.shape or out.dtype is not x.dtype or out.stride(2) != 1:
+        raise KernelError(f"{what} must be of the input's shape and type, with a head's values side by side")
+    return out
+
+
+def rotate(q: Tensor, k: Tensor, past: Tensor, frequencies: Tensor, offsets: Tensor | None = None,
+           q_norm: Tensor | None = None, k_norm: Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+           out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
+    """(q, k) [rows, heads, head_dim] and [rows, kv_heads, head_dim] (fp32, fp16 or bfloat16, any row and head stride)
+    with every head normed and rotated, in their type.
+
+    A head's values x become x * rsqrt(mean(x ** 2) + eps) * norm (fp32 [head_dim]; None: x as it is).  Then of its
+    first 2 * len(frequencies) values, pair i (i and len(frequencies) + i, or interleaved 2 i and 2 i + 1) is turned by
+    position * frequencies[i] radians: (a, b) -> (a cos - b sin, b cos + a sin).  Row r of sequence b is at position
+    past[b] + r - offsets[b].  Rows past the last sequence's are zero in the results.  out: the tensors to write into,
+    q and k themselves if they are to be replaced, but no other rows that overlap them."""
+    device = _device(q, k, past, frequencies, offsets, q_norm, k_norm, *(out or ()))
+    rows, heads, kv_heads, dim, sequences, q_at, k_at, rotary = _turns(q, k, past, frequencies, offsets, q_norm, k_norm,
+                                                                       eps)
+    q_out, k_out = _like(q, out and out[0], "the first of out"), _like(k, out and out[1], "the second of out")
+    if rows:
+        _run("ivonar_rotate", device, q.data_ptr(), k.data_ptr(), _DTYPES[q.dtype], *q_at, *k_at, heads, kv_heads, dim,
+             rows, past.data_ptr(), _address(offsets), sequences, frequencies.data_ptr(), rotary, bool(interleaved),
+             _address(q_norm), _address(k_norm), eps, q_out.data_ptr(), k_out.data_ptr(), *q_out.stride()[:2],
+             *k_out.stride()[:2])
+    return q_out, k_out
+
+
+def rotate_write(pages: Tensor, q: Tensor, k: Tensor, v: Tensor, table: Tensor, past: Tensor, frequencies: Tensor,
+                 offsets: Tensor | None = None, q_norm: Tensor | None = None, k_norm: Tensor | None = None,
+                 eps: float = 1e-6, interleaved: bool = False, out: Tensor | None = None) -> Tensor:
+    """rotate(q, k, ..) and cache_write(pages, its k, v, table, past, offsets) in one launch: the rotated q, and the same
+    bytes in the cache.  out: the tensor to write q into, q itself if it is to be replaced."""
+    device = _device(pages, q, k, v, table, past, frequencies, offsets, q_norm, k_norm, out)
+    count, kv_heads, tiles, dim, sequences, width = _geometry(pages, table, "rotate_write")
+    rows, heads, _, _, past_count, q_at, k_at, rotary = _turns(q, k, past, frequencies, offsets, q_norm, k_norm, eps,
+                                                               kv_heads, dim)
+    if past_count != sequences:
+        raise KernelError(f"past must be contiguous int32 [{sequences}]")
+    v_rows, _, v_row, v_head = _rows(v, kv_heads, dim, "v")
+    if v_rows != rows or v.dtype is not k.dtype:
+        raise KernelError("k and v must have the same rows and type")
+    out = _like(q, out, "out")
+    if rows:
+        _run("ivonar_rotate_write", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[q.dtype], *q_at, *k_at,
+             v_row, v_head, heads, rows, pages.data_ptr(), count, kv_heads, tiles, dim, table.data_ptr(), width,
+             past.data_ptr(), _address(offsets), sequences, frequencies.data_ptr(), rotary, bool(interleaved),
+             _address(q_norm), _address(k_norm), eps, out.data_ptr(), *out.stride()[:2])
+    return out
 
 
 def _scale(scale: float | None, head_dim: int, window: int, sinks: int) -> float:

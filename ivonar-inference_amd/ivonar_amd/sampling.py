@@ -5,20 +5,27 @@ configure_sampling; kernel_decoder.py:213-224 and :619-681 the logit_bounds / sa
 inverse_penalty, top_k, seen, bounds, uniform, token), validates the rule on the host as the
 reference's ``configure_sampling`` does, and launches both kernels on the current stream.  Nothing
 here synchronises except ``sample()``, which returns the token as a Python int.
+
+``log_probabilities(logits, tokens, top, temperature)`` gives the log probabilities of tokens that are
+known (a prompt's, or the ones just drawn), the entropy, and the likeliest alternatives (the reference has
+no counterpart).
 """
 
 from __future__ import annotations
 
-from typing import Iterable
+import functools
+from typing import Iterable, NamedTuple
 
 import torch
 from torch import Tensor
 
+from .attention import _DTYPES, _device, _run
 from .runtime import KernelError, check, current_stream, int32, library, pointer
 
 SAMPLE_THREADS = 1024  # largest top-k one sampling block handles (kernel_decoder.py:25)
 BOUND_GROUP = 64       # logits per bound (kernel_decoder.py:26)
 MAX_VOCAB = 1 << 18
+MAX_TOP = 64           # most alternatives of log_probabilities
 
 
 class DeviceSampler:
@@ -89,3 +96,51 @@ class DeviceSampler:
         self.uniform.uniform_()
         self.launch(logits)
         return int(self.token[0])
+
+
+class LogProbabilities(NamedTuple):
+    """Of every row: log_probability and entropy [rows] (fp32, nats), and the likeliest tokens, falling:
+    top_log_probability [rows, top] (fp32) and top_token [rows, top] (int64)."""
+
+    log_probability: Tensor
+    entropy: Tensor
+    top_log_probability: Tensor
+    top_token: Tensor
+
+
+@functools.lru_cache(maxsize=4096)
+def _score_workspace(*sizes: int) -> int:
+    return library().ivonar_log_probabilities_work(*sizes)
+
+
+def log_probabilities(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0) -> LogProbabilities:
+    """Scores of tokens [rows] (int64) under softmax(logits / temperature), logits [rows, vocab] in fp32, fp16 or
+    bfloat16 with any row stride.
+
+    A token outside the vocabulary has the log probability -inf.  `top` (at most 64) alternatives are listed, of equal
+    logits the lowest token first; a NaN counts as less than every number.  A row whose logits are all -inf has log
+    probabilities of -inf and the entropy 0; a row with a NaN or +inf has NaN for all of its numbers, but for a token
+    outside the vocabulary.  Nothing synchronises, and calls can be captured into a graph."""
+    device = _device(logits, tokens)
+    dtype = _DTYPES.get(logits.dtype)
+    if logits.dim() != 2 or dtype is None or not 0 < logits.shape[1] <= 1 << 30:
+        raise KernelError("logits must be float32, float16 or bfloat16 [rows, vocab]")
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1 and vocab > 1:
+        raise KernelError("logits must have a row's values side by side")
+    if tokens.dtype is not torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous():
+        raise KernelError(f"tokens must be contiguous int64 [{rows}]")
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise KernelError(f"top {top} outside 0..{min(MAX_TOP, vocab)}")
+    if not (2e-38 < temperature < 1e38):
+        raise KernelError("temperature must be positive and finite, and so must its inverse")
+    numbers = torch.empty((rows * (2 + top),), dtype=torch.float32, device=logits.device)
+    chosen, entropy, best = numbers[:rows], numbers[rows:2 * rows], numbers[2 * rows:].view(rows, top)
+    token = torch.empty((rows, top), dtype=torch.int64, device=logits.device)
+    if rows:
+        need = _score_workspace(dtype, rows, vocab, top)
+        work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need > 0 else None
+        _run("ivonar_log_probabilities", device, logits.data_ptr(), dtype, logits.stride(0), rows, vocab,
+             tokens.data_ptr(), top, temperature, chosen.data_ptr(), entropy.data_ptr(), best.data_ptr(), token.data_ptr(),
+             None if work is None else work.data_ptr(), need)
+    return LogProbabilities(chosen, entropy, best, token)
