@@ -317,6 +317,20 @@ hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, 
                                   const int32_t* lengths, const int32_t* offsets, int sequences, int window, int sinks,
                                   float scale, int max_length, void* out, void* work, long long work_bytes);
 
+/* ivonar_cache_attention without a window, for sequences that share the pages of a prefix: the same results up to the
+ * order of sums, the shared keys read and multiplied once for all rows of a group.  Group g has the sequences groups[g]
+ * .. groups[g + 1] - 1 (groups [group_count + 1], not decreasing; sequences outside all groups share nothing), whose
+ * tables begin alike: their positions 0 .. prefix[g] - 1 lie in the same pages.  max_prefix: about the longest prefix, a
+ * hint as max_length.  work: ivonar_prefix_attention_work bytes, 16-byte aligned. */
+long long ivonar_prefix_attention_work(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
+                                       int sequences, int rows, int groups, int max_prefix, int max_length);
+hipError_t ivonar_prefix_attention(hipStream_t stream, const void* q, int dtype, long long q_token_stride,
+                                   long long q_head_stride, int heads, int rows, const uint8_t* pages, int page_count,
+                                   int kv_heads, int page_tiles, int head_dim, const int32_t* table, int table_width,
+                                   const int32_t* lengths, const int32_t* offsets, int sequences, const int32_t* groups,
+                                   const int32_t* prefix, int group_count, float scale, int max_prefix, int max_length,
+                                   void* out, void* work, long long work_bytes);
+
 /* Causal attention within packed prompts over fp16 or bf16 rows (dtype 1 or 2): out [rows, heads, head_dim], a row of
  * sequence b at position r - offsets[b] sees the sequence's rows up to its own, with a window and sinks as above.
  * offsets NULL: one sequence of all rows (sequences == 1).  Rows of no sequence are 0.  Addresses are multiples of 16

@@ -751,6 +751,60 @@ hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, 
   return launch_cache_attention(stream, a);
 }
 
+static PrefixAttentionArgs prefix_attention_sizes(int dtype, int heads, int kv_heads, int head_dim,
+                                                  const int32_t* offsets, int sequences, int rows, int groups,
+                                                  int max_prefix, int max_length) {
+  PrefixAttentionArgs args{};
+  args.a = cache_attention_sizes(dtype, heads, kv_heads, head_dim, offsets, sequences, rows, 0, 0, max_length);
+  args.group_count = groups;
+  args.max_prefix = max_prefix > 0 ? max_prefix : 0;
+  return args;
+}
+
+long long ivonar_prefix_attention_work(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
+                                       int sequences, int rows, int groups, int max_prefix, int max_length) {
+  if (!attention_sizes(dtype, heads, kv_heads, head_dim, sequences, rows, 0, 0, 1.0f) || groups < 0 ||
+      groups > sequences)
+    return -1;
+  return prefix_attention_work(prefix_attention_sizes(dtype, heads, kv_heads, head_dim, offsets, sequences, rows, groups,
+                                                      max_prefix, max_length));
+}
+
+hipError_t ivonar_prefix_attention(hipStream_t stream, const void* q, int dtype, long long q_token_stride,
+                                   long long q_head_stride, int heads, int rows, const uint8_t* pages, int page_count,
+                                   int kv_heads, int page_tiles, int head_dim, const int32_t* table, int table_width,
+                                   const int32_t* lengths, const int32_t* offsets, int sequences, const int32_t* groups,
+                                   const int32_t* prefix, int group_count, float scale, int max_prefix, int max_length,
+                                   void* out, void* work, long long work_bytes) {
+  int shift = 0;
+  if (!attention_sizes(dtype, heads, kv_heads, head_dim, sequences, rows, 0, 0, scale) ||
+      !cache_geometry(pages, page_count, kv_heads, page_tiles, head_dim, table, table_width, sequences, rows, &shift))
+    return hipErrorInvalidValue;
+  if (q == nullptr || out == nullptr || (lengths == nullptr && sequences > 0) || !aligned16(out)) return hipErrorInvalidValue;
+  if (offsets == nullptr && rows != sequences) return hipErrorInvalidValue;
+  if (group_count < 0 || group_count > sequences || groups == nullptr || (prefix == nullptr && group_count > 0))
+    return hipErrorInvalidValue;
+  PrefixAttentionArgs args = prefix_attention_sizes(dtype, heads, kv_heads, head_dim, offsets, sequences, rows,
+                                                    group_count, max_prefix, max_length);
+  const long long need = prefix_attention_work(args);
+  if (need > 0 && (work == nullptr || !aligned16(work) || work_bytes < need)) return hipErrorInvalidValue;
+  CacheAttentionArgs& a = args.a;
+  a.q = q;
+  a.q_strides = RowStrides{q_token_stride, q_head_stride};
+  a.pages = pages;
+  a.table = table;
+  a.lengths = lengths;
+  a.out = out;
+  a.work = static_cast<float*>(work);
+  a.page_count = page_count;
+  a.page_shift = shift;
+  a.table_width = table_width;
+  a.scale = scale;
+  args.groups = groups;
+  args.prefix = prefix;
+  return launch_prefix_attention(stream, args);
+}
+
 hipError_t ivonar_window_attention(hipStream_t stream, const void* q, const void* k, const void* v, int dtype,
                                    long long q_token_stride, long long q_head_stride, long long k_token_stride,
                                    long long k_head_stride, long long v_token_stride, long long v_head_stride,

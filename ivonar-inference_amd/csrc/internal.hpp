@@ -333,6 +333,17 @@ struct CacheAttentionArgs {
 long long cache_attention_work(const CacheAttentionArgs& a);
 hipError_t launch_cache_attention(hipStream_t stream, const CacheAttentionArgs& a);
 
+// The same where groups of sequences share their first pages.
+struct PrefixAttentionArgs {
+  CacheAttentionArgs a;  // no window
+  const int* groups;  // [group_count + 1] sequences before each group
+  const int* prefix;  // [group_count] tokens in shared pages
+  int group_count;
+  int max_prefix;
+};
+long long prefix_attention_work(const PrefixAttentionArgs& args);
+hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs& args);
+
 // Causal attention within packed prompts.
 struct WindowAttentionArgs {
   const void* q;

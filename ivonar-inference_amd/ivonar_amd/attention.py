@@ -14,6 +14,8 @@ The reference keeps fp16 keys and values and attends to them in ``attention_step
 * ``cache_attention(q, pages, table, lengths, offsets, window, sinks)``: the last rows of each sequence (one token
   while decoding, several for a chunk of a prompt) over all of its cached tokens, or over a sliding window and the
   first few (sinks);
+* ``prefix_attention(q, pages, table, lengths, groups, prefix, offsets)``: the same for sequences that share the pages
+  of a long prefix, whose keys and values are read once for all of them;
 * ``window_attention(q, k, v, offsets, window, sinks)``: causal attention within packed prompts over their fp16 or
   bfloat16 keys and values as they are.
 
@@ -328,6 +330,57 @@ def cache_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, of
     _run("ivonar_cache_attention", device, q.data_ptr(), dtype, q_row, q_head, heads, rows, pages.data_ptr(), count,
          kv_heads, tiles, dim, table.data_ptr(), width, lengths.data_ptr(), _address(offsets), sequences, window, sinks,
          scale, longest, out.data_ptr(), _address(work), need)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_workspace(*sizes: int) -> int:
+    """Bytes that a call of these sizes needs besides its operands."""
+    *head, ragged, sequences, rows, groups, longest_prefix, longest = sizes
+    return library().ivonar_prefix_attention_work(*head, 1 if ragged else None, sequences, rows, groups, longest_prefix,
+                                                  longest)
+
+
+def prefix_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, groups: Tensor, prefix: Tensor,
+                     offsets: Tensor | None = None, scale: float | None = None, max_length: int | None = None,
+                     max_prefix: int | None = None, out: Tensor | None = None) -> Tensor:
+    """cache_attention(q, pages, table, lengths, offsets, scale=scale) of sequences that share the pages of a prefix, as
+    forks do (paging.fork): the shared keys are read and multiplied once for all rows of a group.
+
+    groups (int32 [groups + 1], not decreasing): the sequences before each group; those outside all groups share
+    nothing.  prefix (int32 [groups]): how many tokens the sequences of each group have in the same pages, from the
+    first on (for forks, their parent's finished pages; fewer is right as well).  The result is cache_attention's up to
+    the order of sums.  max_prefix and max_length, about the longest ones, set how keys are shared between blocks
+    (default: what the table can hold); any values give the same result up to that order."""
+    device = _device(q, pages, table, lengths, groups, prefix, offsets, out)
+    count, kv_heads, tiles, dim, sequences, width = _geometry(pages, table, "prefix_attention")
+    rows, heads, q_row, q_head = _rows(q, None, dim, "q")
+    if heads == 0 or heads % kv_heads:
+        raise KernelError(f"{heads} heads do not share {kv_heads} key/value heads")
+    if rows * (heads // kv_heads) > 1 << 30:
+        raise KernelError("too many rows for one call")
+    _offsets(offsets, sequences, rows)
+    _index(lengths, sequences, "lengths")
+    group_count = prefix.shape[0] if prefix.dim() == 1 else -1
+    _index(prefix, max(group_count, 0), "prefix")
+    _index(groups, group_count + 1, "groups")
+    if group_count > sequences:
+        raise KernelError(f"{sequences} sequences do not make {group_count} groups")
+    scale = _scale(scale, dim, 0, 0)
+    out = _output(q, out)
+    if rows == 0:
+        return out
+    capacity = width * tiles * TOKENS_PER_TILE
+    longest = capacity if max_length is None else max(1, min(int(max_length), capacity))
+    longest_prefix = longest if max_prefix is None else max(0, min(int(max_prefix), capacity))
+    dtype = _DTYPES[q.dtype]
+    need = _prefix_workspace(dtype, heads, kv_heads, dim, offsets is not None, sequences, rows, group_count,
+                             longest_prefix, longest)
+    work = pages.new_empty(need) if need > 0 else None
+    _run("ivonar_prefix_attention", device, q.data_ptr(), dtype, q_row, q_head, heads, rows, pages.data_ptr(), count,
+         kv_heads, tiles, dim, table.data_ptr(), width, lengths.data_ptr(), _address(offsets), sequences,
+         groups.data_ptr(), prefix.data_ptr(), group_count, scale, longest_prefix, longest, out.data_ptr(),
+         _address(work), need)
     return out
 
 

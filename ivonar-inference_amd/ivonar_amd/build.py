@@ -31,7 +31,7 @@ LIBRARY = PACKAGE / "_lib" / "libivonar_ternary.so"
 ARCH = "gfx950"
 SOURCES = ("quantize.hip", "gemv.hip", "gemv_tokens.hip", "gemm.hip", "gemm_wide.hip", "gemm_scaled.hip",
            "gemm_skinny.hip", "embed.hip", "sample.hip", "score.hip", "stream_read.hip", "validate.hip", "cache.hip",
-           "rotate.hip", "paging.hip", "attention_cache.hip", "attention_prompt.hip", "capi.hip")
+           "rotate.hip", "paging.hip", "attention_cache.hip", "attention_prefix.hip", "attention_prompt.hip", "capi.hip")
 HIP_FLAGS = (
     f"--offload-arch={ARCH}",
     "-O3",

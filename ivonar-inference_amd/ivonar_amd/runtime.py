@@ -77,6 +77,8 @@ SIGNATURES: dict[str, list] = {
     "ivonar_cache_read": [_P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _P, _P],
     "ivonar_cache_attention": [_P, _I, _L, _L, _I, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _F, _I, _P, _P,
                                _L],
+    "ivonar_prefix_attention": [_P, _I, _L, _L, _I, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _P, _P, _I, _F, _I, _I,
+                                _P, _P, _L],
     "ivonar_window_attention": [_P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _I, _I, _I, _I, _P, _I, _I, _I, _F, _P],
     "ivonar_rotate": [_P, _P, _I, *[_L] * 4, _I, _I, _I, _I, _P, _P, _I, _P, _I, _I, _P, _P, _F, _P, _P, *[_L] * 4],
     "ivonar_rotate_write": [_P, _P, _P, _I, *[_L] * 6, _I, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _I, _P, _I, _I, _P, _P,
@@ -134,6 +136,8 @@ def library() -> ctypes.CDLL:
             lib.ivonar_linear_half.restype = c_int
             lib.ivonar_cache_attention_work.argtypes = [c_int, c_int, c_int, c_int, c_void_p, *[c_int] * 5]
             lib.ivonar_cache_attention_work.restype = c_longlong
+            lib.ivonar_prefix_attention_work.argtypes = [c_int, c_int, c_int, c_int, c_void_p, *[c_int] * 5]
+            lib.ivonar_prefix_attention_work.restype = c_longlong
             lib.ivonar_log_probabilities_work.argtypes = [c_int, c_int, c_int, c_int]
             lib.ivonar_log_probabilities_work.restype = c_longlong
             lib.ivonar_token_finish_limit.argtypes = [c_int]
