@@ -3,8 +3,10 @@
 // For a row x of V logits and a temperature T, with m = max x, z_i = (x_i - m) / T, S = sum e^z_i, U = sum z_i e^z_i:
 //   log p_i = z_i - log S,   H = -sum p_i log p_i = log S - U / S.
 // m, S and U are kept per thread in fp32 and rescaled when a chunk raises m: S' = f S, U' = f (U + d S) for a maximum
-// that rises by -d T, f = e^d.  A logit of -inf has no weight; a row of nothing else has log probabilities of -inf and
-// no entropy.  A NaN or +inf makes all of its row's numbers NaN.
+// that rises by -d T, f = e^d.  In units of log 2, z = x c - M with c = log2(e) / T and M = m c rounded to fp32: one
+// rounding of z itself, and since everything is relative to the same M, that of M does not count.  A logit of -inf has no
+// weight; a row of nothing else has log probabilities of -inf and no entropy.  A NaN or +inf makes all of its row's
+// numbers NaN.
 //
 // The `top` largest logits are found in the same pass.  A logit's key is its value as an ordered number, then its index
 // from the end, so no two keys are alike and ties go to the lowest index; a NaN has the lowest value.  A wave keeps the
@@ -25,7 +27,8 @@ constexpr int kWaves = 4;
 constexpr int kValues = 32;                 // logits of a lane at a time
 constexpr int kWaveChunk = 64 * kValues;    // and of a wave
 constexpr int kBuffer = 128;                // keys above the bound that a wave holds before it merges 64
-constexpr float kLowest = -3.402823466e38f;
+constexpr float kFar = 0x1p100f;            // from here on logits either are the maximum or have no weight beside it
+constexpr int kCrowd = 12;                  // logits of a lane above the first bound that tell of ties
 typedef unsigned long long Key;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -36,6 +39,8 @@ struct Params {
   int row_waves;  // waves of a block that share a row: 1 or kWaves
 };
 
+constexpr float kLog2 = 0.69314718055994530942f;
+
 // What a part of a row leaves: m, S, U (in units of log 2), and its largest keys.
 struct Part {
   float m, sum, weighted;
@@ -43,14 +48,6 @@ struct Part {
 };
 constexpr int kPartFloats = 4 + 2 * 64;
 
-template <typename In>
-__device__ __forceinline__ In minus_infinity();
-template <>
-__device__ __forceinline__ float minus_infinity<float>() { return -INFINITY; }
-template <>
-__device__ __forceinline__ Half minus_infinity<Half>() { return Half{0xfc00u}; }
-template <>
-__device__ __forceinline__ Bfloat minus_infinity<Bfloat>() { return Bfloat{0xff80u}; }
 // 16 bytes of logits as fp32.
 template <typename In>
 __device__ __forceinline__ void unpack(const u32x4& words, float* x) {
@@ -100,30 +97,46 @@ __device__ __forceinline__ unsigned xor_lane(unsigned v) {
 template <int X>
 __device__ __forceinline__ float xor_lane(float v) { return __uint_as_float(xor_lane<X>(__float_as_uint(v))); }
 
+template <int X>
+__device__ __forceinline__ float keep(float v, bool larger) {
+  const float other = xor_lane<X>(v);
+  return larger ? fmaxf(v, other) : fminf(v, other);
+}
+
 // Compares with lane ^ X and keeps the larger key or the smaller one.
 template <int X>
 __device__ __forceinline__ Key keep(Key key, bool larger) {
   const Key other = (Key)xor_lane<X>((unsigned)(key >> 32)) << 32 | xor_lane<X>((unsigned)key);
   return (other > key) == larger ? other : key;
 }
-// Keys that rise and then fall (or the reverse) over SIZE lanes, sorted: falling where `falling`.
-template <int SIZE>
-__device__ __forceinline__ Key merge_lanes(Key key, bool falling) {
+// Keys (or numbers alone) that rise and then fall, or the reverse, over SIZE lanes, sorted: falling where `falling`.
+template <int SIZE, typename V>
+__device__ __forceinline__ V merge_lanes(V v, int lane, bool falling) {
   if constexpr (SIZE > 1) {
-    key = keep<SIZE / 2>(key, ((threadIdx.x & (SIZE / 2)) == 0) == falling);
-    key = merge_lanes<SIZE / 2>(key, falling);
+    v = keep<SIZE / 2>(v, ((lane & (SIZE / 2)) == 0) == falling);
+    v = merge_lanes<SIZE / 2>(v, lane, falling);
   }
-  return key;
+  return v;
+}
+template <int SIZE, typename V>
+__device__ __forceinline__ V sort_parts(V v, int lane) {
+  if constexpr (SIZE > 2) v = sort_parts<SIZE / 2>(v, lane);
+  return merge_lanes<SIZE>(v, lane, SIZE < 64 && (lane & SIZE) != 0);
+}
+// The lane, as a number that the compiler cannot form the stages' masks from ahead of a loop: they would take up most
+// of the scalar registers.
+__device__ __forceinline__ int opaque_lane() {
+  int lane = threadIdx.x;
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 // Sorted over the wave, rising from lane 0 on.
-template <int SIZE = 64>
-__device__ __forceinline__ Key sort_lanes(Key key) {
-  if constexpr (SIZE > 2) key = sort_lanes<SIZE / 2>(key);
-  return merge_lanes<SIZE>(key, SIZE < 64 && (threadIdx.x & SIZE) != 0);
-}
+template <typename V>
+__device__ __forceinline__ V sort_lanes(V v) { return sort_parts<64>(v, opaque_lane()); }
+
 // The 64 largest of a falling list and a rising one, falling.
 __device__ __forceinline__ Key join(Key falling, Key rising) {
-  return merge_lanes<64>(falling > rising ? falling : rising, true);
+  return merge_lanes<64>(falling > rising ? falling : rising, opaque_lane(), true);
 }
 __device__ __forceinline__ Key lane_key(Key key, int lane) {
   return (Key)(unsigned)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
@@ -150,9 +163,14 @@ __device__ __forceinline__ float all_sum(float v) {
 // z no further down than where its weight is zero: zero times the result is zero.
 __device__ __forceinline__ float bounded(float z) { return fmaxf(z, -1000.0f); }
 
+// Whether m c may be out of range; not of a maximum of nothing.
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
+__device__ __forceinline__ float scaled(float m, float scale) { return m == -INFINITY ? 0.0f : m * scale; }
+
 // S and U moved to the maximum `to`.
 __device__ __forceinline__ void raise(float& m, float& sum, float& weighted, float to, float scale) {
-  const float d = bounded((m - to) * scale);
+  const float apart = fabsf(m) >= kFar || fabsf(to) >= kFar ? (m == to ? 0.0f : -1000.0f) : m * scale - to * scale;
+  const float d = bounded(apart);
   const float factor = __builtin_amdgcn_exp2f(d);
   weighted = fmaf(sum, d, weighted) * factor;
   sum *= factor;
@@ -163,9 +181,14 @@ __device__ __forceinline__ void raise(float& m, float& sum, float& weighted, flo
 __device__ __forceinline__ void finish(const Params& p, int row, const Part& part) {
   const ScoreArgs& a = p.a;
   const int lane = threadIdx.x & 63;
-  const float log_sum = logf(part.sum);
-  const bool none = part.sum == 0.0f;
-  auto log_probability = [&](float x) { return none ? -INFINITY : (x - part.m) * a.inverse_temperature - log_sum; };
+  const float log_sum = log2f(part.sum);
+  const bool none = part.sum == 0.0f, far = is_far(part.m);
+  auto log_probability = [&](float x) {
+    if (none) return -INFINITY;
+    // Far from everything in range, in nats: in units of log 2 they may not be.
+    if (far || fabsf(x) >= kFar) return (x - part.m) * a.inverse_temperature - kLog2 * log_sum;
+    return kLog2 * (fmaf(x, p.scale, -scaled(part.m, p.scale)) - log_sum);
+  };
   if (lane == 0) {
     const int64_t token = a.tokens[row];
     float chosen = -INFINITY;
@@ -177,7 +200,7 @@ __device__ __forceinline__ void finish(const Params& p, int row, const Part& par
       chosen = log_probability(x);
     }
     a.log_probability[row] = chosen;
-    a.entropy[row] = none ? 0.0f : log_sum - 0.69314718055994530942f * (part.weighted / part.sum);
+    a.entropy[row] = none ? 0.0f : kLog2 * (log_sum - part.weighted / part.sum);
   }
   if (lane < a.top) {
     const long long at = (long long)row * a.top + lane;
@@ -187,10 +210,11 @@ __device__ __forceinline__ void finish(const Params& p, int row, const Part& par
 }
 
 template <typename In, bool TOP>
-__global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 4) void score_kernel(Params p) {
   constexpr int kVec = 16 / sizeof(In), kVectors = kValues / kVec;
   const ScoreArgs& a = p.a;
   __shared__ Key buffers[TOP ? kWaves : 1][TOP ? kBuffer : 1];
+  __shared__ __align__(16) float places[TOP ? kWaves : 1][TOP ? 64 : 1][kValues];
   __shared__ Key bounds[kWaves];  // of each row of the block, the best bound so far
   __shared__ float sums[kWaves][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -204,38 +228,35 @@ __global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
     __syncthreads();
   }
 
-  // Element e of the row, counted from the 16 bytes that its first logit lies in, is logit e - lead.
+  // The row's whole 16-byte vectors in chunks, and up to 2 (kVec - 1) logits before and behind them in a last one.
   const In* begin = static_cast<const In*>(a.logits) + row * a.row_stride;
   const int lead = (int)(((uintptr_t)begin & 15u) / sizeof(In));
-  const In* base = begin - lead;
-  const long long end = (long long)lead + a.vocab;
-  const int chunks = there ? (int)((end + kWaveChunk - 1) / kWaveChunk) : 0;
+  const int head = lead == 0 ? 0 : min(kVec - lead, a.vocab);
+  const int vectors = (a.vocab - head) / kVec, whole = (vectors + 64 * kVectors - 1) / (64 * kVectors);
+  const int rest = a.vocab - vectors * kVec;  // head + tail
+  const int chunks = there ? whole + (rest > 0 ? 1 : 0) : 0;
+  const int rest_index = lane < head ? lane : lane < rest ? vectors * kVec + lane : -1;
   const int step = p.splits * p.row_waves;
+  const u32x4* const aligned = reinterpret_cast<const u32x4*>(begin + head);
   auto load = [&](int chunk, u32x4 (&to)[kVectors]) {
-    const long long from = (long long)chunk * kWaveChunk;
-    if (from >= lead && from + kWaveChunk <= end) {
+    if (chunk < whole) {
+      // Places past the last vector take that one, and are cleared when they are used.
 #pragma unroll
-      for (int v = 0; v < kVectors; ++v)
-        to[v] = reinterpret_cast<const u32x4*>(base + from)[v * 64 + lane];
+      for (int v = 0; v < kVectors; ++v) to[v] = aligned[min((chunk * kVectors + v) * 64 + lane, vectors - 1)];
     } else {
+      In values[kVec];
+      values[0] = begin[max(rest_index, 0)];
 #pragma unroll
-      for (int v = 0; v < kVectors; ++v) {
-        const long long e = from + (v * 64 + lane) * kVec;
-        In values[kVec];
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          values[j] = minus_infinity<In>();
-          if (e + j >= lead && e + j < end) values[j] = base[e + j];
-        }
-        __builtin_memcpy(&to[v], values, 16);
-      }
+      for (int j = 1; j < kVec; ++j) values[j] = In{};
+      __builtin_memcpy(&to[0], values, 16);
     }
   };
 
-  float m = kLowest, sum = 0.0f, weighted = 0.0f;
+  float m = -INFINITY, sum = 0.0f, weighted = 0.0f;
   Key list = 0, bound = 0;
   int held = 0;  // keys in the buffer
   Key* buffer = buffers[TOP ? wave : 0];
+  float(*found)[kValues] = places[TOP ? wave : 0];
   // Merges the first `count` keys of the buffer into the list.
   auto merge = [&](int count) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -255,18 +276,46 @@ __global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
     float x[kValues];
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) unpack<In>(current[v], x + v * kVec);
+    if (chunk >= whole - 1) {
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) {
+        const bool inside = chunk < whole ? (chunk * kVectors + j / kVec) * 64 + lane < vectors
+                                          : j == 0 && rest_index >= 0;
+        x[j] = inside ? x[j] : -INFINITY;
+      }
+    }
     float most = x[0];
 #pragma unroll
     for (int j = 1; j < kValues; ++j) most = fmaxf(most, x[j]);
     if (most > m) raise(m, sum, weighted, most, p.scale);
+    const float shift = scaled(m, p.scale);
     float part_sum[2] = {}, part_weighted[2] = {};
+    bool slow = __ballot(is_far(m)) != 0ull;
+    if (!slow) {
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-      // The difference first: a scaled logit of the type's lowest value may overflow.
-      const float z = (x[j] - m) * p.scale;
-      const float weight = __builtin_amdgcn_exp2f(z);
-      part_sum[j & 1] += weight;
-      part_weighted[j & 1] = fmaf(bounded(z), weight, part_weighted[j & 1]);
+      for (int j = 0; j < kValues; ++j) {
+        const float z = fmaf(x[j], p.scale, -shift);
+        const float weight = __builtin_amdgcn_exp2f(z);
+        part_sum[j & 1] += weight;
+        part_weighted[j & 1] = fmaf(z, weight, part_weighted[j & 1]);  // no number for -inf
+        if (j % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // or all weights would be held at once
+      }
+      const float of_sum = part_sum[0] + part_sum[1], of_weighted = part_weighted[0] + part_weighted[1];
+      slow = __ballot(of_weighted != of_weighted && of_sum == of_sum) != 0ull;
+    }
+    if (slow) {
+      part_sum[0] = part_sum[1] = part_weighted[0] = part_weighted[1] = 0.0f;
+      const bool far = is_far(m);
+      float again = shift;
+      asm volatile("" : "+v"(again));  // or the compiler would hold all z from above for here
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) {
+        const float z = far ? (x[j] - m) * p.scale : fmaf(x[j], p.scale, -again);
+        const float weight = __builtin_amdgcn_exp2f(z);
+        part_sum[j & 1] += weight;
+        part_weighted[j & 1] = fmaf(bounded(z), weight, part_weighted[j & 1]);
+        if (j % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+      }
     }
     sum += part_sum[0] + part_sum[1];
     weighted += part_weighted[0] + part_weighted[1];
@@ -274,10 +323,38 @@ __global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
     if constexpr (TOP) {
       const Key shared = *(volatile Key*)&bounds[first_wave];
       bound = shared > bound ? shared : bound;
-      const int offset = (int)((long long)chunk * kWaveChunk - lead) + lane * kVec;  // the lane's first logit
-      auto index_of = [&](int j) { return offset + j / kVec * (64 * kVec) + j % kVec; };
-      if (bound == 0) {
-        // Of the lanes' largest keys the top'th is no larger than that of all keys.
+      // The lane's logit j in the row, outside the vocabulary where it has none.
+      const int start = chunk < whole ? head + chunk * kWaveChunk : -1;
+      auto index_of = [&](int j) {
+        const int vector = (chunk * kVectors + j / kVec) * 64 + lane;
+        if (chunk < whole) return vector < vectors ? head + vector * kVec + j % kVec : -1;
+        return j == 0 ? rest_index : -1;
+      };
+      const bool first = bound == 0;
+      if (first) {
+        // Of the lanes' largest logits the top'th is no larger than that of all.
+        const float largest = sort_lanes(fmaxf(most, -INFINITY));
+        const float last = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(largest), 64 - a.top));
+        // Below the keys of its value: those of the number before it (before +0 comes -0, which compares like it).
+        if (last > -INFINITY) bound = ((Key)(ordered(last) - (last == 0.0f ? 1u : 0u)) << 32) - 1;
+      }
+      unsigned above = 0;  // bit j: logit j may be
+      // Behind the bound's index equal logits are below it.  Without a bound all logits are above it, NaN among them.
+      auto compare = [&]() {
+        const float least = value_of(bound);
+        above = 0;
+        if (bound != 0 && start > (int)~(unsigned)bound) {
+          if (__ballot(most > least) != 0ull)
+#pragma unroll
+            for (int j = kValues - 1; j >= 0; --j) above = above + above + (x[j] > least ? 1u : 0u);
+        } else if (__ballot(!(most < least)) != 0ull) {
+#pragma unroll
+          for (int j = kValues - 1; j >= 0; --j) above = above + above + (!(x[j] < least) ? 1u : 0u);
+        }
+      };
+      compare();
+      if (first && __ballot(__popc(above) >= kCrowd) != 0ull) {
+        // Ties: the top'th of the lanes' largest keys.
         int best = -1;
 #pragma unroll
         for (int j = kValues - 1; j >= 0; --j) {
@@ -286,35 +363,37 @@ __global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
         }
         const Key key = sort_lanes(best >= 0 ? key_of(most, best) : 0);
         const Key last = lane_key(key, 64 - a.top);
-        bound = last > 0 ? last - 1 : 0;
+        bound = last > bound + 1 ? last - 1 : bound;
+        compare();
       }
-      const float least = value_of(bound);  // NaN: none yet
-      if (__ballot(!(most < least)) != 0ull) {
-        unsigned above = 0;  // bit j: logit j may be
+      if (above != 0u) {
+        // For the loop below, which takes a lane's logits by number: loads of them, though near, would take longer.
 #pragma unroll
-        for (int j = 0; j < kValues; ++j) above |= !(x[j] < least) ? 1u << j : 0u;
-        while (__ballot(above != 0u) != 0ull) {
-          bool add = false;
-          Key key = 0;
-          if (above != 0u) {
-            const int j = __builtin_ctz(above);
-            above &= above - 1u;
-            const int index = index_of(j);
-            if ((unsigned)index < (unsigned)a.vocab) {
-              key = key_of(to_float(begin[index]), index);
-              add = key > bound;
-            }
+        for (int j = 0; j < kValues; j += 4)
+          *reinterpret_cast<float4*>(&found[lane][j]) = float4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+      while (__ballot(above != 0u) != 0ull) {
+        bool add = false;
+        Key key = 0;
+        if (above != 0u) {
+          const int j = __builtin_ctz(above);
+          above &= above - 1u;
+          const int index = index_of(j);
+          if ((unsigned)index < (unsigned)a.vocab) {
+            key = key_of(found[lane][j], index);
+            add = key > bound;
           }
-          const unsigned long long adds = __ballot(add);
-          if (add) buffer[held + __popcll(adds & ((1ull << lane) - 1ull))] = key;
-          held += __popcll(adds);
-          if (held >= 64) {
-            merge(64);
-            const Key rest = buffer[64 + lane];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            buffer[lane] = rest;
-            held -= 64;
-          }
+        }
+        const unsigned long long adds = __ballot(add);
+        if (add) buffer[held + __popcll(adds & ((1ull << lane) - 1ull))] = key;
+        held += __popcll(adds);
+        if (held >= 64) {
+          merge(64);
+          const Key rest = buffer[64 + lane];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          buffer[lane] = rest;
+          held -= 64;
         }
       }
     }
@@ -338,8 +417,7 @@ __global__ __launch_bounds__(kThreads) void score_kernel(Params p) {
     if (TOP) buffer[lane] = list;
     __syncthreads();
     if (sub != 0) return;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
+    for (int w = wave + 1; w < wave + p.row_waves; ++w) {
       float other_m = sums[w][0], other_sum = sums[w][1], other_weighted = sums[w][2];
       const float top = fmaxf(part.m, other_m);
       raise(part.m, part.sum, part.weighted, top, p.scale);
@@ -366,7 +444,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
   if (row >= p.a.rows) return;
   const float* from = p.a.work + (long long)row * p.splits * kPartFloats;
   Part part;
-  part.m = kLowest;
+  part.m = -INFINITY;
   part.sum = part.weighted = 0.0f;
   part.list = 0;
   for (int i = lane; i < p.splits; i += 64) {
@@ -387,21 +465,17 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
   finish(p, row, part);
 }
 
-// Blocks that few rows are split into.
-constexpr long long kWanted = 1024;
-// Rows of up to this many chunks get a wave each.
-constexpr int kWaveRowChunks = 2;
+// Waves of all rows that keep the device busy, blocks that few long rows are split into, and chunks of a wave that are
+// not split.
+constexpr int kBusyWaves = 4096, kWantedBlocks = 1024, kLeastChunks = 4;
 
 Params plan(const ScoreArgs& a) {
   Params p{a, 1.44269504088896340736f * a.inverse_temperature, 1, kWaves};
-  const long long chunks = ((long long)a.vocab + 7 + kWaveChunk - 1) / kWaveChunk;
-  if (chunks <= kWaveRowChunks && a.rows >= kWanted) {
-    p.row_waves = 1;
-    return p;
-  }
-  const long long wanted = (kWanted + a.rows - 1) / (a.rows > 0 ? a.rows : 1);
-  const long long most = (chunks + kWaves - 1) / kWaves;
-  p.splits = (int)(wanted < most ? wanted : most);
+  const int chunks = (int)(((long long)a.vocab + kWaveChunk - 1) / kWaveChunk);
+  while (p.row_waves > 1 && ((long long)a.rows * p.row_waves >= 2 * kBusyWaves || chunks <= p.row_waves / 2))
+    p.row_waves /= 2;
+  if (p.row_waves == kWaves)
+    p.splits = max(1, min(kWantedBlocks / max(1, a.rows), chunks / (kWaves * kLeastChunks)));
   return p;
 }
 
