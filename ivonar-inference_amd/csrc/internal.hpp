@@ -271,8 +271,8 @@ struct RotateArgs {
   int rotary;
   bool interleaved;
   float eps;
-  bool aligned = false;  // the rows of q, k and v start on 16 bytes
-  bool out_aligned = false;
+  bool aligned = false;
+  bool tables_aligned = false;
 };
 hipError_t launch_rotate(hipStream_t stream, const CacheArgs& a, RotateArgs r, int head_dim, int dtype);
 

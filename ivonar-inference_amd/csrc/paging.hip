@@ -328,13 +328,15 @@ __global__ __launch_bounds__(kThreads) void renumber_kernel(PoolArgs p, int* tab
   if (is_page(p, page) && page >= *live) table[i] = moved[page];
 }
 
-// A block takes 16 KB of every gridDim.y'th page of the list.  It looks at 64 rows of the list at a time, most of which
-// hold no copy when a cache is compacted.
-constexpr int kCopyBytes = kThreads * 16 * 4;
+// A block takes 4 KB, 16 bytes a thread, of every gridDim.y'th page of the list.  It looks at 64 rows of the list at a
+// time, most of which hold no copy when a cache is compacted.  Pages of 68 KB: 60 copied in 3.2 us and 900 in 20 (6.4
+// TB/s); with two to four loads before their stores in a thread 16.5 and 28.
+constexpr int kCopyBytes = kThreads * 16;
 __global__ __launch_bounds__(kThreads) void copy_kernel(uint8_t* pages, int page_count, long long page_bytes,
                                                         const int* copies, int count) {
   const int lane = threadIdx.x & 63;
-  const long long words = page_bytes / 16, first = (long long)blockIdx.x * (kCopyBytes / 16) + threadIdx.x;
+  const long long at = (long long)blockIdx.x * kThreads + threadIdx.x;
+  const bool inside = at < page_bytes / 16;
   for (long long base = blockIdx.y; base < count; base += 64LL * gridDim.y) {
     const long long i = base + (long long)lane * gridDim.y;
     const int2 copy = i < count ? reinterpret_cast<const int2*>(copies)[i] : int2{-1, -1};
@@ -344,16 +346,11 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(uint8_t* pages, int page
       const int row = __builtin_ctzll(live);
       const float4* from = reinterpret_cast<const float4*>(pages + __shfl(copy.x, row) * page_bytes);
       float4* to = reinterpret_cast<float4*>(pages + __shfl(copy.y, row) * page_bytes);
-      float4 held[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) held[j] = from[min(first + j * kThreads, words - 1)];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (first + j * kThreads < words) to[first + j * kThreads] = held[j];
+      if (inside) to[at] = from[at];
     }
   }
 }
-constexpr int kCopyBlocks = 2048;
+constexpr int kCopyBlocks = 8192;
 
 }  // namespace
 

@@ -76,27 +76,6 @@ __device__ __forceinline__ Key key_of(float x, int index) {
   return (Key)ordered(x) << 32 | (unsigned)~index;
 }
 
-// The value of lane ^ X.
-template <int X>
-__device__ __forceinline__ unsigned xor_lane(unsigned v) {
-  if constexpr (X == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false);
-  if constexpr (X == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false);
-  if constexpr (X == 4)  // the mirror of eight lanes, then of four
-    return (unsigned)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF,
-                                              false);
-  if constexpr (X == 8) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, false);
-  if constexpr (X == 16) {
-    const auto swapped = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return threadIdx.x & 16 ? swapped[0] : swapped[1];
-  }
-  if constexpr (X == 32) {
-    const auto swapped = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return threadIdx.x & 32 ? swapped[0] : swapped[1];
-  }
-}
-template <int X>
-__device__ __forceinline__ float xor_lane(float v) { return __uint_as_float(xor_lane<X>(__float_as_uint(v))); }
-
 template <int X>
 __device__ __forceinline__ float keep(float v, bool larger) {
   const float other = xor_lane<X>(v);
