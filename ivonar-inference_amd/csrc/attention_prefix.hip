@@ -14,6 +14,10 @@
 namespace ivo {
 namespace {
 
+// Blocks per CU that the registers leave room for: as the cache attention's, and three where without its bookkeeping
+// they do.
+constexpr int resident(int D, int R, int NT) { return D == 64 && R == 32 && NT == 2 ? 3 : occupancy(D, R, NT); }
+
 struct SharedParams {
   Params p;
   const int* groups;
@@ -149,7 +153,7 @@ __device__ __forceinline__ void store_result(const CacheAttentionArgs& a, const 
 
 // The rows of a group over its prefix: a part per row tile, share of the keys, and head.
 template <int D, typename In, int R, int NT>
-__global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void prefix_kernel(SharedParams sp) {
+__global__ __launch_bounds__(kThreads, resident(D, R, NT)) void prefix_kernel(SharedParams sp) {
   const Params& p = sp.p;
   const CacheAttentionArgs& a = p.a;
   __shared__ __align__(16) unsigned char room_bytes[sizeof(Room<D>)];
@@ -206,7 +210,7 @@ __device__ __forceinline__ Span tail_span(const SharedParams& sp, int sequence, 
 // The rows of each sequence over its own keys: the results where they are not split, else a part per row tile, share
 // and head.
 template <int D, typename In, int R, int NT>
-__global__ __launch_bounds__(kThreads, occupancy(D, R, NT)) void tail_kernel(SharedParams sp) {
+__global__ __launch_bounds__(kThreads, resident(D, R, NT)) void tail_kernel(SharedParams sp) {
   const Params& p = sp.p;
   const CacheAttentionArgs& a = p.a;
   __shared__ __align__(16) unsigned char room_bytes[sizeof(Room<D>)];
@@ -270,8 +274,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(SharedParams sp) {
   store_result<D, In>(a, all, row, h, column);
 }
 
-// Blocks that row tiles and heads are split into where there are fewer, and key tiles that are not split.
-constexpr int kBlocks = 512, kLeastTiles = 8;
+// Keys are split where row tiles and heads make fewer blocks than the device holds at a time, but not below so many
+// tiles.  Four groups of 16 sequences with 4 rows each over 3957 tokens, 16/4 heads of 64, fp16: 22.1 us with as many
+// blocks as it holds, 768, and 24.9 with 512 or 1024.
+constexpr int kDeviceUnits = 256, kLeastTiles = 8;  // CUs
 constexpr int kWholeUnits = 128, kWholeTiles = 64;
 
 // Rows of a row tile: 8, 16 or 32, as `rows` of them fill.
@@ -300,8 +306,9 @@ Plan plan(const PrefixAttentionArgs& args) {
   sp.prefix = args.prefix;
   sp.group_count = args.group_count;
   const long long rows = (long long)a.rows * p.group;
-  auto split = [&](long long tiles, long long units, int& splits, int& chunk) {
-    const long long wanted = max(1LL, kBlocks / max(1LL, units));
+  const int terms = a.dtype == kFloat32 ? 3 : a.dtype == kFloat16 ? 2 : 1;
+  auto split = [&](int R, long long tiles, long long units, int& splits, int& chunk) {
+    const long long wanted = max(1LL, kDeviceUnits * resident(a.head_dim, R, terms) / max(1LL, units));
     const long long each = max((long long)kLeastTiles, (tiles + wanted - 1) / wanted);
     chunk = (int)each;
     splits = (int)max(1LL, (tiles + each - 1) / each);
@@ -309,7 +316,7 @@ Plan plan(const PrefixAttentionArgs& args) {
 
   const int R = sp.prefix_rows = tile_rows(a, rows / max(1, args.group_count));
   sp.prefix_slots = (int)(rows / R + args.group_count);
-  split((args.max_prefix + kCacheTile - 1) / kCacheTile, ((rows + R - 1) / R) * a.kv_heads, sp.prefix_splits,
+  split(R, (args.max_prefix + kCacheTile - 1) / kCacheTile, ((rows + R - 1) / R) * a.kv_heads, sp.prefix_splits,
         sp.prefix_chunk);
   const int T = plan.tail_rows = tile_rows(a, rows / max(1, a.sequences));
   p.slots = (int)(a.offsets == nullptr ? (long long)a.sequences * ((p.group + T - 1) / T) : rows / T + a.sequences);
@@ -319,7 +326,7 @@ Plan plan(const PrefixAttentionArgs& args) {
     sp.tail_splits = 1;
     sp.tail_chunk = 1;
   } else {
-    split(tiles, units, sp.tail_splits, sp.tail_chunk);
+    split(T, tiles, units, sp.tail_splits, sp.tail_chunk);
   }
   const long long floats = a.head_dim + 2;
   plan.shared_bytes = ((long long)args.group_count * 4 + 15) & ~15LL;
