@@ -31,10 +31,10 @@ layers) cost little more at many tokens than at few (3.4 us each at 32, 4.4 at
 The reference's mixers (recurrent scan, latent attention) are not part of this path: without ``attention`` the
 output projection reads the V third of the entry projection's output instead of a mixer's output. With
 ``attention`` (an ``AttentionConfig``) the thirds are the queries, keys and values of causal self-attention,
-with a sliding window and sinks if it has them: a decode step writes its token's keys and values into a 4-bit
-cache and attends to the cache; a prompt's first tile attends to its own keys and values, rounded to bfloat16
-(window_attention takes half types, and bfloat16 has fp32's range; what it drops, 2^-9 of a value, is little
-next to the cache's 4 bits), and later tiles to the cache. Greedy tokens are written on the device into a ring
+with a sliding window and sinks if it has them, queries and keys rotated by position if it has a rotary base: a
+decode step writes its token's keys and values into a 4-bit cache and attends to the cache; a prompt's first tile
+attends to its own keys and values, rounded to bfloat16 (window_attention takes half types, and bfloat16 has fp32's
+range; what it drops, 2^-9 of a value, is little next to the cache's 4 bits), and later tiles to the cache. Greedy tokens are written on the device into a ring
 of ``burst`` slots, so a burst of decode steps runs as one HIP graph replay with
 a single read-back, as the reference's burst graphs do (``kernel_decoder.py:694-735``).
 """
@@ -52,9 +52,9 @@ from . import attention as attn
 from . import runtime
 from .matrix import Matrix, _lanes_for
 from .quantization import TernaryLinear
-from .ops import MODE_NORM, MODE_PLAIN
+from .ops import MODE_NORM, MODE_PLAIN, gemm, quantize_rows
 from .runtime import KernelError, Launch, float32, int32, pointer
-from .sampling import DeviceSampler
+from .sampling import MAX_TOP, DeviceSampler, LogProbabilities, log_probabilities
 from .synthetic import LinearStackWeights
 
 TILE = 32
@@ -86,13 +86,14 @@ def _linear(layer) -> TernaryLinear:
 class AttentionConfig:
     """Self-attention between the entry and the output projection: `heads` heads (hidden / heads one of
     attention.HEAD_DIMS), the last `window` tokens (0: all) and the first `sinks` visible, a cache of `capacity`
-    tokens."""
+    tokens, queries and keys rotated by their positions with frequencies of base `rotary_base` (0: as they are)."""
 
     heads: int
     window: int = 0
     sinks: int = 0
     capacity: int = 4096
     page_size: int = 64
+    rotary_base: float = 0.0
 
 
 class _Attention:
@@ -105,6 +106,8 @@ class _Attention:
             raise KernelError("the cache needs room for at least one token")
         if config.window < 0 or config.sinks < 0:
             raise KernelError("window and sinks must not be negative")
+        if not (config.rotary_base >= 0 and math.isfinite(config.rotary_base)):
+            raise KernelError("rotary_base must be finite and not negative")
         self.config, self.shape = config, (config.heads, hidden // config.heads)
         pages = -(-config.capacity // max(1, config.page_size))  # cache_pages refuses other sizes
         self.pages = [attn.cache_pages(pages, *self.shape, config.page_size, device) for _ in range(layers)]
@@ -116,6 +119,9 @@ class _Attention:
         self.mixed_tile = torch.zeros(longest, hidden, dtype=torch.float32, device=device)
         self.half_tile = torch.zeros(longest, 3 * hidden, dtype=torch.bfloat16, device=device)
         self.half_out = torch.zeros(longest, hidden, dtype=torch.bfloat16, device=device)
+        self.frequencies = None
+        if config.rotary_base > 0:
+            self.frequencies = attn.rotary_frequencies(self.shape[1], config.rotary_base, device=device)
         self.tokens = 0  # in the cache
 
     def _thirds(self, rows: torch.Tensor):
@@ -123,7 +129,10 @@ class _Attention:
 
     def _cached(self, layer: int, rows: torch.Tensor, past, lengths, offsets, out: torch.Tensor) -> None:
         q, k, v = self._thirds(rows)
-        attn.cache_write(self.pages[layer], k, v, self.table, past, offsets)
+        if self.frequencies is None:
+            attn.cache_write(self.pages[layer], k, v, self.table, past, offsets)
+        else:
+            attn.rotate_write(self.pages[layer], q, k, v, self.table, past, self.frequencies, offsets, out=q)
         attn.cache_attention(q, self.pages[layer], self.table, lengths, offsets, self.config.window, self.config.sinks,
                              max_length=self.config.capacity, out=out.unflatten(1, self.shape))
 
@@ -136,7 +145,9 @@ class _Attention:
         if not first:
             self._cached(layer, mixer_in, index[:1], index[1:2], index[2:], self.mixed_tile[:rows])
             return
-        _, k, v = self._thirds(mixer_in)
+        q, k, v = self._thirds(mixer_in)
+        if self.frequencies is not None:
+            attn.rotate(q, k, index[:1], self.frequencies, index[2:], out=(q, k))
         attn.cache_write(self.pages[layer], k, v, self.table, index[:1], index[2:])
         half, out = self.half_tile[:rows], self.half_out[:rows]
         half.copy_(mixer_in)
@@ -379,14 +390,47 @@ class StackDecoder:
         """Runs the prompt in tiles (kernel_decoder.py:456-479), each the smallest of TILES that holds the
         tokens left, then the head on its last token: the logits are left in ``self.logits`` and the first
         token (greedy, or drawn by the sampler) in the ring's last slot."""
+        ids = self._prompt(input_ids)
+        for _ in self._run_tiles(ids):
+            pass
+        return self._end_prompt(int(ids.numel()))
+
+    @torch.no_grad()
+    def score(self, input_ids, top: int = 0) -> LogProbabilities:
+        """The log probabilities of a prompt's tokens behind its first one, each given those before it, with the
+        entropies and the `top` likeliest tokens of the same places (sampling.log_probabilities).  Leaves the decoder
+        as prefill() of the prompt does, ready to go on from it."""
+        if not 0 <= top <= min(MAX_TOP, self.config.vocab):
+            raise KernelError(f"top {top} outside 0..{min(MAX_TOP, self.config.vocab)}")
+        ids = self._prompt(input_ids)
+        length = int(ids.numel())
+        targets = ids[1:].to(self.device)
+        parts = []
+        for start, count in self._run_tiles(ids):
+            rows = min(count, length - 1 - start)  # the last token has no successor
+            if rows > 0:
+                normed = quantize_rows(self.residual_tile[:rows], MODE_NORM, self.final_norm, self.config.eps)
+                parts.append(log_probabilities(gemm(self.token_matrix, *normed), targets[start:start + rows], top))
+        self._end_prompt(length)
+        if not parts:  # a single token
+            parts.append(log_probabilities(self.logits[None, :][:0], targets, top))
+        return LogProbabilities(*(torch.cat(side) for side in zip(*parts)))
+
+    def _prompt(self, input_ids) -> torch.Tensor:
+        """A prompt's ids on the host, checked, and room for them in the cache."""
         ids = torch.as_tensor(input_ids, dtype=torch.int64).reshape(-1).cpu()
         length = int(ids.numel())
         if length == 0:
             raise ValueError("the prompt must not be empty")
         if int(ids.min()) < 0 or int(ids.max()) >= self.config.vocab:
             raise IndexError(f"token id is out of range for vocab_size={self.config.vocab}")
-        attention = self.attention
         self._reserve(length, held=0)
+        return ids
+
+    def _run_tiles(self, ids: torch.Tensor):
+        """Runs a prompt's tiles, and after each yields its first token's place and its tokens, whose residuals are in
+        ``self.residual_tile``."""
+        attention, length = self.attention, int(ids.numel())
         host, start = self._tile_host, 0
         while start < length:
             count = min(length - start, TILES[-1])
@@ -401,9 +445,12 @@ class StackDecoder:
                 (self._later_tile_graph if start else self._tile_graph)[tokens].replay()
             else:
                 self._run((self._later_tiles if start else self._tiles)[tokens])
+            yield start, count
             start += count
-        if attention is not None:
-            attention.step_index.copy_(torch.tensor([length, length + 1], dtype=torch.int32))
+
+    def _end_prompt(self, length: int) -> torch.Tensor:
+        if self.attention is not None:
+            self.attention.step_index.copy_(torch.tensor([length, length + 1], dtype=torch.int32))
         self._run(self._first)
         self.position = 0
         return self.logits
