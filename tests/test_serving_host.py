@@ -74,12 +74,13 @@ def test_prefix_attention_entry_refuses():
 def test_score_entry_refuses():
     lib = library()
     assert lib.ivonar_log_probabilities_work(0, 1000000, 1000, 20) == 0
-    need = lib.ivonar_log_probabilities_work(0, 1, 32000, 20)
+    assert lib.ivonar_log_probabilities_work(0, 1, 32000, 20) == 0  # one block a row
+    need = lib.ivonar_log_probabilities_work(0, 1, 1000000, 20)
     assert need > 0
     for sizes in ((3, 1, 100, 5), (0, -1, 100, 5), (0, 1, 0, 0), (0, 1, 100, 65), (0, 1, 10, 11), (0, 1, 100, -1),
                   (0, 1, (1 << 30) + 1, 5)):
         assert lib.ivonar_log_probabilities_work(*sizes) == -1
-    good = [P, 0, 32000, 1, 32000, P, 20, 1.0, P, P, P, P, P, need]
+    good = [P, 0, 1000000, 1, 1000000, P, 20, 1.0, P, P, P, P, P, need]
     _refused("ivonar_log_probabilities", good, [(0, None), (0, P + 2), (1, 3), (3, -1), (4, 0), (5, None), (6, 65), (6, -1),
                                                 (7, 0.0), (7, -1.0), (7, float("nan")), (7, float("inf")), (7, 1e-42),
                                                 (8, None), (9, None), (10, None), (11, None), (12, None), (12, P + 8),
