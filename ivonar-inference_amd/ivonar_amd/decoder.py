@@ -34,9 +34,9 @@ output projection reads the V third of the entry projection's output instead of 
 with a sliding window and sinks if it has them, queries and keys rotated by position if it has a rotary base: a
 decode step writes its token's keys and values into a 4-bit cache and attends to the cache; a prompt's first tile
 attends to its own keys and values, rounded to bfloat16 (window_attention takes half types, and bfloat16 has fp32's
-range; what it drops, 2^-9 of a value, is little next to the cache's 4 bits), and later tiles to the cache. Greedy tokens are written on the device into a ring
-of ``burst`` slots, so a burst of decode steps runs as one HIP graph replay with
-a single read-back, as the reference's burst graphs do (``kernel_decoder.py:694-735``).
+range; what it drops, 2^-9 of a value, is little next to the cache's 4 bits), and later tiles to the cache. Greedy
+tokens are written on the device into a ring of ``burst`` slots, so a burst of decode steps runs as one HIP graph
+replay with a single read-back, as the reference's burst graphs do (``kernel_decoder.py:694-735``).
 """
 
 from __future__ import annotations
