@@ -359,6 +359,9 @@ __device__ __forceinline__ void attend_run(const Params& p, const Span& s, int h
   constexpr int W = D / 32, kChunks = kNarrow ? 2 * W : W, kTiles = D / 16;
   constexpr int NP = NT < 2 ? 2 : NT;  // terms of a weight
   constexpr int kStages = stages(D);
+  // While it feeds the matrix cores a wave goes before the others of its SIMD, which take their softmax beside it: 1024
+  // rows over 16000 keys, eight heads of 128, bf16, 118 us instead of 127.
+  constexpr bool kRaised = SHARED && !kNarrow;
   const CacheAttentionArgs& a = p.a;
   auto& sums = room.sums;
   // Opaque to the compiler, which would otherwise compute every address of the loop's body ahead of it, and hold
@@ -463,6 +466,7 @@ __device__ __forceinline__ void attend_run(const Params& p, const Span& s, int h
       }
       strange = __ballot(found);
     }
+    if constexpr (kRaised) __builtin_amdgcn_s_setprio(1);
     // x[h][rt][r]: the logit of key 16 h + 4 b + r, or of up to 8 rows 16 (n / 8) + 4 b + r.
     f32x4 x[kHalves][RT];
 #pragma unroll
@@ -489,6 +493,7 @@ __device__ __forceinline__ void attend_run(const Params& p, const Span& s, int h
       if constexpr (kNarrow) x[h][0] += upper;
     }
 
+    if constexpr (kRaised) __builtin_amdgcn_s_setprio(0);
     uint2 v_scale = t.v_scale;
     unsigned hidden = 0;  // bit e: the scale of the lane's token e stands for no number
     if (!whole) {
@@ -608,6 +613,7 @@ __device__ __forceinline__ void attend_run(const Params& p, const Span& s, int h
       }
     }
 
+    if constexpr (kRaised) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       unsigned pairs[8];
@@ -635,6 +641,7 @@ __device__ __forceinline__ void attend_run(const Params& p, const Span& s, int h
         }
     }
 
+    if constexpr (kRaised) __builtin_amdgcn_s_setprio(0);
     there >>= 1;
     stage = stage == kStages - 1 ? 0 : stage + 1;
 
