@@ -126,6 +126,8 @@ def log_probabilities(logits: Tensor, tokens: Tensor, top: int = 0, temperature:
     if logits.dim() != 2 or dtype is None or not 0 < logits.shape[1] <= 1 << 30:
         raise KernelError("logits must be float32, float16 or bfloat16 [rows, vocab]")
     rows, vocab = logits.shape
+    if rows >= 1 << 31:
+        raise KernelError("log_probabilities takes fewer than 2**31 rows")
     if logits.stride(1) != 1 and vocab > 1:
         raise KernelError("logits must have a row's values side by side")
     if tokens.dtype is not torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous():
@@ -134,13 +136,13 @@ def log_probabilities(logits: Tensor, tokens: Tensor, top: int = 0, temperature:
         raise KernelError(f"top {top} outside 0..{min(MAX_TOP, vocab)}")
     if not (2e-38 < temperature < 1e38):
         raise KernelError("temperature must be positive and finite, and so must its inverse")
-    numbers = torch.empty((rows * (2 + top),), dtype=torch.float32, device=logits.device)
-    chosen, entropy, best = numbers[:rows], numbers[rows:2 * rows], numbers[2 * rows:].view(rows, top)
-    token = torch.empty((rows, top), dtype=torch.int64, device=logits.device)
+    numbers = tokens.new_empty((rows * (2 + top),), dtype=torch.float32)
+    chosen, entropy, best = numbers.split_with_sizes((rows, rows, rows * top))
+    best, token = best.view(rows, top), tokens.new_empty((rows, top))
     if rows:
         need = _score_workspace(dtype, rows, vocab, top)
-        work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need > 0 else None
+        work = tokens.new_empty((need,), dtype=torch.uint8) if need > 0 else None
         _run("ivonar_log_probabilities", device, logits.data_ptr(), dtype, logits.stride(0), rows, vocab,
-             tokens.data_ptr(), top, temperature, chosen.data_ptr(), entropy.data_ptr(), best.data_ptr(), token.data_ptr(),
-             None if work is None else work.data_ptr(), need)
+             tokens.data_ptr(), top, temperature, chosen.data_ptr(), entropy.data_ptr(), best.data_ptr(),
+             token.data_ptr(), None if work is None else work.data_ptr(), need)
     return LogProbabilities(chosen, entropy, best, token)

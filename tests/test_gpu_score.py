@@ -247,5 +247,7 @@ def test_refusals(cuda):
             sampling.log_probabilities(**{**good, name: value})
     with pytest.raises(KernelError):
         sampling.log_probabilities(logits[:, :4].contiguous(), tokens, 5)
+    with pytest.raises(KernelError):
+        sampling.log_probabilities(logits[:1, :1].expand(1 << 31, 1), tokens)
     empty = sampling.log_probabilities(logits[:0], tokens[:0], 5)
     assert [tuple(r.shape) for r in empty] == [(0,), (0,), (0, 5), (0, 5)]
