@@ -69,26 +69,28 @@ __device__ __forceinline__ FreePages scan_free(const PoolArgs& p, int* sums, int
   __syncthreads();
   return f;
 }
-// The free page of a rank below `available`.
+// The free page of a rank below `available`.  (The walk ends with the words all the same where another call on the pool,
+// against the order that they need, has taken pages since the scan.)
 __device__ __forceinline__ int free_page(const PoolArgs& p, const FreePages& f, int rank) {
   int thread = 0;
 #pragma unroll
   for (int step = kBlock / 2; step > 0; step >>= 1)
     if (f.sums[thread + step] <= rank) thread += step;
   rank -= f.sums[thread];
-  int w = thread * f.per;
+  const int words = (p.pages + 31) / 32;
+  int w = min(thread * f.per, words - 1);
   unsigned word = free_word(p, w);
-  for (int count = __popc(word); rank >= count; count = __popc(word)) {
+  for (int count = __popc(word); rank >= count && w + 1 < words; count = __popc(word)) {
     rank -= count;
     word = free_word(p, ++w);
   }
   for (; rank > 0; --rank) word &= word - 1u;
-  return w * 32 + __builtin_ctz(word);
+  return word == 0u ? 0 : w * 32 + __builtin_ctz(word);
 }
 // Clears the bits of the first `given` free pages.  No thread may look for a page any more.
 __device__ __forceinline__ void take_free(const PoolArgs& p, const FreePages& f, int given) {
   int mine = min(given - f.before, f.own);
-  for (int w = threadIdx.x * f.per; mine > 0; ++w) {
+  for (int w = threadIdx.x * f.per; mine > 0 && w < min((int)(threadIdx.x + 1) * f.per, (p.pages + 31) / 32); ++w) {
     unsigned word = free_word(p, w);
     for (; word != 0u && mine > 0; --mine) word &= word - 1u;
     p.free[w] = (int)word;
@@ -190,8 +192,10 @@ __global__ __launch_bounds__(kThreads) void release_kernel(PoolArgs p, int* tabl
 
 __device__ __forceinline__ int whole_pages(const PoolArgs& p, int length) { return max(length, 0) >> p.page_shift; }
 
-// Block 0 gives out pages for the unfinished pages of the rows that share their parent with an earlier row, and writes
-// all lengths and copies.  The other blocks write the rows' other slots, each kBlock slots of one row.
+// Block 0 writes the rows' slots with unfinished pages, and all lengths and copies: it gives out pages to the rows that
+// share their parent with an earlier row, and to the others (a parent's heirs) whose unfinished page is in more entries
+// of the table than theirs.  The other blocks write the rows' other slots, each kBlock slots of one row.  They may
+// count up a page while block 0 looks at its count, but only one that is in two entries before.
 __global__ __launch_bounds__(kBlock) void fork_kernel(PoolArgs p, ForkArgs a) {
   __shared__ int sums[kBlock];
   __shared__ int totals[kBlockWaves];
@@ -208,8 +212,7 @@ __global__ __launch_bounds__(kBlock) void fork_kernel(PoolArgs p, ForkArgs a) {
     int page = -1;
     if (there) {
       const int length = a.lengths[parent], whole = whole_pages(p, length);
-      // Block 0 writes the page of a row that may need a copy.
-      if (!heir && slot == whole && max(length, 0) & ((1 << p.page_shift) - 1)) return;
+      if (slot == whole && max(length, 0) & ((1 << p.page_shift) - 1)) return;  // block 0's
       if (heir || slot < whole) page = a.table[(long long)parent * a.width + slot];
     }
     a.out_table[(long long)r * a.width + slot] = page;
@@ -228,20 +231,22 @@ __global__ __launch_bounds__(kBlock) void fork_kernel(PoolArgs p, ForkArgs a) {
   for (int base = 0; base < a.rows; base += kBlock) {
     const int r = base + (int)threadIdx.x;
     int length = 0, whole = 0, source = -1;
-    bool slot = false;  // this block writes the row's slot `whole`
+    bool slot = false, heir = false;  // this block writes the row's slot `whole`
     if (r < a.rows) {
       const int parent = a.parents[r];
       if ((unsigned)parent < (unsigned)a.sequences) {
         length = max(a.lengths[parent], 0);
         whole = whole_pages(p, length);
-        slot = first[parent] != r && whole < a.width && (length & ((1 << p.page_shift) - 1)) != 0;
+        heir = first[parent] == r;
+        slot = whole < a.width && (length & ((1 << p.page_shift) - 1)) != 0;
         if (slot) source = a.table[(long long)parent * a.width + whole];
       }
     }
-    const bool wants = slot && is_page(p, source);
+    const bool wants = is_page(p, source) && (!heir || p.refs[source] > 1);
     int all = 0;
     const int rank = given + block_scan(wants ? 1 : 0, totals, all);
-    int page = -1;
+    int page = heir && !wants ? source : -1;
+    if (is_page(p, page)) atomicAdd(p.refs + page, 1);
     if (wants && rank < f.available) {
       page = free_page(p, f, rank);
       p.refs[page] = 1;

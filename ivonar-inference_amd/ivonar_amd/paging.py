@@ -105,7 +105,10 @@ def reserve(pool: PagePool, table: Tensor, lengths: Tensor, counts: Tensor) -> T
 
 def release(pool: PagePool, table: Tensor, first: Tensor | None = None, last: Tensor | None = None) -> None:
     """Sequence b gives back the pages of its slots first[b] .. last[b] - 1 (default: all); their entries become -1.  A
-    page that a fork still holds stays held."""
+    page that a fork still holds stays held.
+
+    A sequence that has dropped tokens gives back the pages behind its new end, and where that lies within a page that a
+    fork holds as well, it has to go through fork() before its next write, which gives it a page of its own."""
     device = _device(pool.refs, pool.free, table, first, last)
     at = _pool(pool, "release")
     sequences, width = _table(table, pool.page_size, "release")
@@ -121,8 +124,9 @@ def fork(pool: PagePool, table: Tensor, lengths: Tensor, parents: Tensor,
     """The next batch: row r goes on from row parents[r] of `table` (an empty row where that is none, such as -1).
 
     The first row of a parent takes over all of its entries; further ones share its finished pages, and get a copy of the
-    page that is not full (and none of those reserved behind it).  `table` and `lengths` are used up: rows without a child
-    give their pages back.  The copies' pages come from those free before the call; a row that gets none ends with its
+    page that is not full (and none of those reserved behind it).  The first gets one as well where another entry of
+    `table` has that page, as after tokens were dropped from a fork.  `table` and `lengths` are used up: rows without a
+    child give their pages back.  The copies' pages come from those free before the call; a row that gets none ends with its
     last finished page.  Call copy() with the result's copies for every cache before the next write.
     out: a table [rows, width] and lengths [rows] to write the results into, other ones than those given."""
     device = _device(pool.refs, pool.free, table, lengths, parents, *(out or ()))
@@ -175,6 +179,8 @@ def copy(pages: Tensor, copies: Tensor) -> None:
         raise KernelError("copy needs pages as cache_pages() makes them")
     if copies.dim() != 2 or copies.shape[1] != 2 or copies.dtype is not torch.int32 or not copies.is_contiguous():
         raise KernelError("copies must be contiguous int32 [count, 2]")
+    if copies.shape[0] >= 1 << 31:
+        raise KernelError("copy takes fewer than 2**31 copies")
     if copies.data_ptr() & 7:
         copies = copies.clone()
     page_bytes = pages.numel() // pages.shape[0]

@@ -59,12 +59,16 @@ class Pool:
             length = max(0, int(lengths[parent]))
             whole = length // self.size
             new_lengths[r] = length
+            unfinished = length % self.size and whole < width and self.holds(table[parent, whole])
             if parent not in seen:
                 seen.add(parent)
                 new[r] = table[parent]
-                continue
-            new[r, :whole] = table[parent, :whole]
-            if length % self.size and whole < width and self.holds(table[parent, whole]):
+                if not unfinished or self.refs[table[parent, whole]] < 2:
+                    continue
+                new[r, whole] = -1
+            else:
+                new[r, :whole] = table[parent, :whole]
+            if unfinished:
                 page = self.give(taken)
                 if page < 0:
                     missing += 1

@@ -149,6 +149,45 @@ def test_slots_past_the_table(cuda):
     assert both.reserve([0, 96], [32 * 10, 32 * 1000]) == 7 + 1000
 
 
+def test_dropped_tokens_in_a_page_that_a_fork_holds(cuda):
+    """The next fork gives each of those that end in it a page of its own, or none where there is none."""
+    both = Both(cuda, 12, 32, 1, 4)
+    both.reserve([0], [83])
+    lengths, _ = both.fork([83], [0, 0, 0])  # two pages shared, three unfinished ones
+    both.release(first=[3, 2, 2])
+    lengths, copies = both.fork([83, 50, 50], [0, 1, 2])
+    assert lengths.tolist() == [83, 50, 50] and (copies[:, 0] == int(both.expected[0, 1])).sum() == 2
+    assert len(set(both.expected[:, 1].tolist())) == 3
+    lengths, copies = both.fork(lengths, [2, 1, 0, 1])  # pages of their own move on
+    assert (copies[:, 0] >= 0).sum() == 1
+    both.release()
+    assert not both.plain.refs.any()
+    both = Both(cuda, 3, 32, 2, 4)
+    both.reserve([0, 0], [64, 0])
+    both.fork([64, 0], [0, 0])
+    lengths, copies = both.fork([40, 41], [0, 1])  # one page is left for two
+    assert lengths.tolist() == [40, 32] and (copies[:, 0] >= 0).sum() == 1
+
+
+def test_smallest_pools_and_batches(cuda):
+    """A pool of one page, tables without rows, forks to none and from none."""
+    from ivonar_amd import attention
+
+    both = Both(cuda, 1, 32, 1, 1)
+    both.reserve([0], [5])
+    assert both.compact().shape == (0, 2)
+    lengths, copies = both.fork([5], [])
+    assert lengths.shape == (0,) and copies.shape == (0, 2) and not both.plain.refs.any()
+    assert both.reserve([], []) == 0
+    both.release()
+    both.compact()
+    lengths, copies = both.fork([], [-1, 0])
+    assert lengths.tolist() == [0, 0] and (copies.cpu() == -1).all()
+    pages = attention.cache_pages(1, 1, 64, 32, cuda)
+    both.paging.copy(pages, copies)
+    both.paging.copy(pages, copies[:0])
+
+
 @pytest.mark.parametrize("kv,dim,page,count", [(1, 64, 32, 40), (8, 128, 64, 60), (3, 256, 128, 9)])
 def test_copies(cuda, kv, dim, page, count):
     """Forked and compacted sequences read back what they held, in every layer, and nothing else changes."""
