@@ -4,11 +4,12 @@
 // The sequences groups[g] .. groups[g + 1] - 1 hold their first prefix[g] tokens in the same pages.  The softmax over all
 // of a row's keys is the sum over two stretches of them, each with its own maximum m, sum l and weighted values o:
 //   m = max(m1, m2), out = (2^(m1 - m) o1 + 2^(m2 - m) o2) / (2^(m1 - m) l1 + 2^(m2 - m) l2).
-// One launch takes the rows of a group together over the prefix, read through the table row of its first sequence, as
+// One launch takes the rows of a group together over the prefix, read through a table row of theirs, as
 // if they were one sequence's: a tile of keys is loaded and converted once for 32 rows instead of for each sequence's
 // few.  The next takes each sequence's own keys behind it and adds the prefix's parts.  A row sees the whole prefix, so
 // where a sequence's rows begin before its end, the group's prefix ends there: P_g is the least of prefix[g] and the
-// positions of its sequences' first rows, and what lies behind it is read through each sequence's own table row.
+// positions of its sequences' first rows, and what lies behind it is read through each sequence's own table row.  Rows
+// of a sequence without tokens, as in a padded batch, see nothing, and its group's prefix is as long without it.
 #include "attention_cache.hpp"
 
 namespace ivo {
@@ -48,18 +49,27 @@ __device__ __forceinline__ Group group_of(const SharedParams& sp, int g) {
   group.rows = max(0, row_before(a, group.end) - group.row0);
   return group;
 }
-// Tokens that all rows of a group see through the shared pages.  All lanes of a wave call this together.
-__device__ __forceinline__ int shared_tokens(const SharedParams& sp, int g, const Group& group) {
+// Tokens that all rows of a group see through the shared pages, and the sequence whose table row is read for them, the
+// first that has rows.  Sequences without tokens do not count: their rows see nothing.  All lanes of a wave call this
+// together.
+__device__ __forceinline__ int shared_tokens(const SharedParams& sp, int g, const Group& group, int& source) {
   const CacheAttentionArgs& a = sp.p.a;
-  int least = sp.prefix[g];
+  int least = sp.prefix[g], first = group.end;
   for (int b = group.begin + (int)(threadIdx.x & 63); b < group.end; b += 64) {
     int row0;
-    const int rows = rows_of(a, b, row0);
-    if (rows > 0) least = min(least, max(a.lengths[b], 0) - rows);
+    const int rows = rows_of(a, b, row0), length = a.lengths[b];
+    if (rows > 0 && length > 0) {
+      least = min(least, length - rows);
+      first = min(first, b);
+    }
   }
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) least = min(least, __shfl_xor(least, o));
-  return uniform(max(least, 0));
+  for (int o = 1; o < 64; o <<= 1) {
+    least = min(least, __shfl_xor(least, o));
+    first = min(first, __shfl_xor(first, o));
+  }
+  source = uniform(first);
+  return source < group.end ? uniform(max(least, 0)) : 0;
 }
 // First row tile of a group: leaves each group at least as many as it needs.
 __device__ __forceinline__ int first_slot(const SharedParams& sp, int g, int row0) {
@@ -123,7 +133,7 @@ __device__ __forceinline__ PrefixParts prefix_parts(const SharedParams& sp, int 
   }
   PrefixParts of{0, 0, 0, 0};
   const int g = uniform(before) - 1;
-  if (g < 0 || sequence >= sp.groups[g + 1]) return of;
+  if (g < 0 || sequence >= sp.groups[g + 1] || sp.p.a.lengths[sequence] <= 0) return of;
   of.tokens = max(sp.shared[g], 0);
   if (of.tokens == 0) return of;
   of.row0 = row_before(sp.p.a, max(0, min(sp.groups[g], sp.p.a.sequences)));
@@ -177,9 +187,10 @@ __global__ __launch_bounds__(kThreads, resident(D, R, NT)) void prefix_kernel(Sh
   s.start = (slot - first_slot(sp, g, group.row0)) * R;
   s.rows = group.rows * p.group;
   if (s.start < 0 || s.start >= s.rows) return;
-  const int tokens = shared_tokens(sp, g, group);
+  int source;
+  const int tokens = shared_tokens(sp, g, group, source);
   if (slot == first_slot(sp, g, group.row0) && split == 0 && head == 0 && threadIdx.x == 0) sp.shared[g] = tokens;
-  s.sequence = s.table_row = group.begin;
+  s.sequence = s.table_row = source;
   s.row0 = group.row0;
   s.first = s.low = s.high = tokens - 1;
   s.sink_tiles = s.window_tile = s.from = s.step = 0;

@@ -168,6 +168,24 @@ def test_sequences_without_rows_and_tokens(cuda, rng, dtype):
     batch.check(batch.run(groups=[6], prefix=[]), "no groups")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dead", [[0], [1, 3], [0, 1, 2, 3], [0, 2, 4, 5]])
+def test_padded_batch(cuda, rng, dtype, dead):
+    """Sequences of no tokens and no pages but with a row each, as a batch of a fixed size has: first in a group, in the
+    middle, and whole groups of them."""
+    sequences = [(0, 4, 5 + 9 * b, 1) for b in range(4)] + [(1, 2, 40, 1), (1, 2, 3, 1)]
+    batch = Batch(cuda, rng, sequences, 8, 2, 64, 32, dtype)
+    for b in dead:
+        batch.lengths[b] = 0
+        batch.table[b] = -1
+    live = [b for b in range(6) if b not in dead]
+    for offsets in (None, _ints(cuda, list(range(7)))):
+        for hints in ({}, {"max_prefix": 128, "max_length": 200}):
+            out = batch.run(offsets=offsets, **hints)
+            assert not out[dead].any()
+            batch.check(out, some=live)
+
+
 def test_many_groups(cuda, rng):
     """More groups and sequences than a wave has lanes, of one to three sequences."""
     sequences, b = [], 0
