@@ -15,15 +15,21 @@
 // hold no logit above the bound, which their maxima tell.  Keys above it go through a buffer in LDS and are sorted and
 // merged 64 at a time.
 //
-// A wave takes 2048 logits at a time, 32 per lane; the next ones are under way while these are used.  Few rows are
+// A wave takes 2048 logits at a time, 32 per lane; the next ones are under way while these are used.  Few long rows are
 // split between blocks, whose results a second kernel joins.
+//
+// Bound by the logits' bytes where there are many: 500 rows of 32000 in fp32 14.5 us without alternatives (4.4 TB/s) and
+// 19.2 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth).  Of
+// the instructions the exponentials take a third, the comparison with the bound a quarter.  One row of 32000 takes 5.8
+// us, and 12.3 with 20: a chain of about seventy compare stages of a sort and merges.
 #include "internal.hpp"
 #include "ternary_device.hpp"
 
 namespace ivo {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;                   // of a block
+constexpr int kManyWaves = 16;              // of a block where there are few rows
 constexpr int kValues = 32;                 // logits of a lane at a time
 constexpr int kWaveChunk = 64 * kValues;    // and of a wave
 constexpr int kBuffer = 128;                // keys above the bound that a wave holds before it merges 64
@@ -36,7 +42,8 @@ struct Params {
   ScoreArgs a;
   float scale;   // log2(e) / T
   int splits;    // blocks that share a row
-  int row_waves;  // waves of a block that share a row: 1 or kWaves
+  int waves;      // of a block: kWaves or kManyWaves
+  int row_waves;  // that share a row
 };
 
 constexpr float kLog2 = 0.69314718055994530942f;
@@ -188,22 +195,22 @@ __device__ __forceinline__ void finish(const Params& p, int row, const Part& par
   }
 }
 
-template <typename In, bool TOP>
-__global__ __launch_bounds__(kThreads, 4) void score_kernel(Params p) {
+template <typename In, bool TOP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
   constexpr int kVec = 16 / sizeof(In), kVectors = kValues / kVec;
   const ScoreArgs& a = p.a;
-  __shared__ Key buffers[TOP ? kWaves : 1][TOP ? kBuffer : 1];
-  __shared__ __align__(16) float places[TOP ? kWaves : 1][TOP ? 64 : 1][kValues];
-  __shared__ Key bounds[kWaves];  // of each row of the block, the best bound so far
-  __shared__ float sums[kWaves][4];
+  __shared__ Key buffers[TOP ? WAVES : 1][TOP ? kBuffer : 1];
+  __shared__ __align__(16) float places[TOP ? WAVES : 1][TOP ? 64 : 1][kValues];
+  __shared__ Key bounds[WAVES];  // of each row of the block, the best bound so far
+  __shared__ float sums[WAVES][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sub = wave & (p.row_waves - 1), first_wave = wave - sub;
   const int split = blockIdx.x % p.splits;
-  const long long row_id = (long long)(blockIdx.x / p.splits) * (kWaves / p.row_waves) + wave / p.row_waves;
+  const long long row_id = (long long)(blockIdx.x / p.splits) * (WAVES / p.row_waves) + wave / p.row_waves;
   const bool there = row_id < a.rows;
   const int row = (int)(there ? row_id : a.rows - 1);
   if (TOP) {
-    if (threadIdx.x < kWaves) bounds[threadIdx.x] = 0;
+    if (threadIdx.x < WAVES) bounds[threadIdx.x] = 0;
     __syncthreads();
   }
 
@@ -313,7 +320,8 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(Params p) {
       if (first) {
         // Of the lanes' largest logits the top'th is no larger than that of all.
         const float largest = sort_lanes(fmaxf(most, -INFINITY));
-        const float last = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(largest), 64 - a.top));
+        const float last =
+            __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(largest), 64 - a.top));
         // Below the keys of its value: those of the number before it (before +0 comes -0, which compares like it).
         if (last > -INFINITY) bound = ((Key)(ordered(last) - (last == 0.0f ? 1u : 0u)) << 32) - 1;
       }
@@ -387,25 +395,29 @@ __global__ __launch_bounds__(kThreads, 4) void score_kernel(Params p) {
   part.sum = all_sum(sum);
   part.weighted = all_sum(weighted);
   part.list = list;
-  if (p.row_waves > 1) {
+  // The parts of a row's waves, four at a time.
+  for (int apart = 1; apart < p.row_waves; apart *= 4) {
+    if (apart > 1) __syncthreads();  // the parts have been read
     if (lane == 0) {
       sums[wave][0] = part.m;
       sums[wave][1] = part.sum;
       sums[wave][2] = part.weighted;
     }
-    if (TOP) buffer[lane] = list;
+    if (TOP) buffer[lane] = part.list;
     __syncthreads();
-    if (sub != 0) return;
-    for (int w = wave + 1; w < wave + p.row_waves; ++w) {
-      float other_m = sums[w][0], other_sum = sums[w][1], other_weighted = sums[w][2];
+    if (sub % (4 * apart) != 0) continue;
+    for (int w = sub + apart; w < min(sub + 4 * apart, p.row_waves); w += apart) {
+      float other_m = sums[first_wave + w][0], other_sum = sums[first_wave + w][1];
+      float other_weighted = sums[first_wave + w][2];
       const float top = fmaxf(part.m, other_m);
       raise(part.m, part.sum, part.weighted, top, p.scale);
       raise(other_m, other_sum, other_weighted, top, p.scale);
       part.sum += other_sum;
       part.weighted += other_weighted;
-      if (TOP) part.list = join(part.list, buffers[TOP ? w : 0][TOP ? 63 - lane : 0]);
+      if (TOP) part.list = join(part.list, buffers[TOP ? first_wave + w : 0][TOP ? 63 - lane : 0]);
     }
   }
+  if (sub != 0) return;
   if (!there) return;
   if (p.splits == 1) {
     finish(p, row, part);
@@ -438,32 +450,58 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
   raise(part.m, part.sum, part.weighted, top, p.scale);
   part.sum = all_sum(part.sum);
   part.weighted = all_sum(part.weighted);
-  if (p.a.top > 0)
-    for (int i = 0; i < p.splits; ++i)
-      part.list = join(part.list, reinterpret_cast<const Key*>(from + (long long)i * kPartFloats + 4)[63 - lane]);
+  if (p.a.top > 0) {
+    constexpr int kAtOnce = 8;
+    for (int base = 0; base < p.splits; base += kAtOnce) {
+      Key lists[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const long long i = min(base + k, p.splits - 1);
+        lists[k] = reinterpret_cast<const Key*>(from + i * kPartFloats + 4)[63 - lane];
+      }
+      for (int k = 0; k < kAtOnce && base + k < p.splits; ++k) {
+        part.list = join(part.list, lists[0]);
+#pragma unroll
+        for (int j = 0; j + 1 < kAtOnce; ++j) lists[j] = lists[j + 1];
+      }
+    }
+  }
   finish(p, row, part);
 }
 
 // Waves of all rows that keep the device busy, blocks that few long rows are split into, and chunks of a wave that are
 // not split.
 constexpr int kBusyWaves = 4096, kWantedBlocks = 1024, kLeastChunks = 4;
+// Few rows of middling length take a block of sixteen waves each, up to two chunks a wave: top 20 of 1 x 32000 fp32 12.6
+// us and of 32 x 50000 bf16 16.0, with four waves 13.7 and 19.3.  Longer rows are faster in several blocks of four waves
+// (1 x 128256 bf16 20.0 us and 22.3), and more rows than compute units fill the device that way.
+constexpr int kManyRows = 256, kManyLeast = 8, kManyMost = 32;
 
 Params plan(const ScoreArgs& a) {
-  Params p{a, 1.44269504088896340736f * a.inverse_temperature, 1, kWaves};
+  Params p{a, 1.44269504088896340736f * a.inverse_temperature, 1, kWaves, kWaves};
   const int chunks = (int)(((long long)a.vocab + kWaveChunk - 1) / kWaveChunk);
-  while (p.row_waves > 1 && ((long long)a.rows * p.row_waves >= 2 * kBusyWaves || chunks <= p.row_waves / 2))
+  if (a.rows <= kManyRows && chunks >= kManyLeast && chunks <= kManyMost) p.waves = p.row_waves = kManyWaves;
+  while (p.waves == kWaves && p.row_waves > 1 &&
+         ((long long)a.rows * p.row_waves >= 2 * kBusyWaves || chunks <= p.row_waves / 2))
     p.row_waves /= 2;
   if (p.row_waves == kWaves)
     p.splits = max(1, min(kWantedBlocks / max(1, a.rows), chunks / (kWaves * kLeastChunks)));
   return p;
 }
 
+template <typename In, int WAVES>
+void run_waves(hipStream_t stream, const Params& p, unsigned blocks) {
+  if (p.a.top > 0)
+    hipLaunchKernelGGL((score_kernel<In, true, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
+  else
+    hipLaunchKernelGGL((score_kernel<In, false, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
+}
 template <typename In>
 void run(hipStream_t stream, const Params& p, unsigned blocks) {
-  if (p.a.top > 0)
-    hipLaunchKernelGGL((score_kernel<In, true>), dim3(blocks), dim3(kThreads), 0, stream, p);
+  if (p.waves == kWaves)
+    run_waves<In, kWaves>(stream, p, blocks);
   else
-    hipLaunchKernelGGL((score_kernel<In, false>), dim3(blocks), dim3(kThreads), 0, stream, p);
+    run_waves<In, kManyWaves>(stream, p, blocks);
 }
 
 }  // namespace
@@ -476,7 +514,7 @@ long long score_work(const ScoreArgs& a) {
 hipError_t launch_score(hipStream_t stream, const ScoreArgs& a) {
   if (a.rows == 0) return hipSuccess;
   const Params p = plan(a);
-  const int block_rows = kWaves / p.row_waves;
+  const int block_rows = p.waves / p.row_waves;
   const long long blocks = ((long long)a.rows + block_rows - 1) / block_rows * p.splits;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   if (a.dtype == kFloat32)
