@@ -19,9 +19,9 @@
 // split between blocks, whose results a second kernel joins.
 //
 // Bound by the logits' bytes where there are many: 500 rows of 32000 in fp32 14.5 us without alternatives (4.4 TB/s) and
-// 19.2 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth).  Of
-// the instructions the exponentials take a third, the comparison with the bound a quarter.  One row of 32000 takes 5.8
-// us, and 12.3 with 20: a chain of about seventy compare stages of a sort and merges.
+// 19.2 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth),
+// where vector instructions take three quarters of the SIMDs' cycles.  One row of 32000 takes 5.8 us, and 12.3 with 20:
+// a chain of about seventy compare stages of sorts and merges.
 #include "internal.hpp"
 #include "ternary_device.hpp"
 

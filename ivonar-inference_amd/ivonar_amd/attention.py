@@ -34,7 +34,8 @@ synchronises, so all of them can be captured into a graph.  Where blocks share a
 counts them in the library's scratch of the stream, and under capture in that of the capture stream if it has made an
 eager call before, else of the device.  So graphs captured on one stream, or an eager call on that stream and a replay
 on another, must not run at the same time: their results would be undefined, and the counts they leave would spoil
-later calls until the library's ``ivonar_init`` clears them.  Eager calls on different streams may overlap.
+later calls until the library's ``ivonar_init`` clears them.  Eager calls on different streams may overlap, and
+``prefix_attention``, whose parts are joined by a second launch, uses its own workspace alone.
 """
 
 from __future__ import annotations
@@ -204,7 +205,8 @@ def _turns(q: Tensor, k: Tensor, past: Tensor, frequencies: Tensor, offsets: Ten
     _index(past, max(sequences, 0), "past")
     _offsets(offsets, sequences, rows)
     rotary = 2 * frequencies.shape[0] if frequencies.dim() == 1 else 0
-    if frequencies.dtype is not torch.float32 or not frequencies.is_contiguous() or not 0 < rotary <= dim or rotary % 16:
+    if (frequencies.dtype is not torch.float32 or not frequencies.is_contiguous() or not 0 < rotary <= dim
+            or rotary % 16):
         raise KernelError(f"frequencies must be contiguous float32 [rotary / 2], rotary a multiple of 16 up to {dim}")
     for norm, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if norm is not None and (norm.dtype is not torch.float32 or norm.shape != (dim,) or not norm.is_contiguous()):
