@@ -93,3 +93,34 @@ def test_a_prompt_goes_on_in_many_ways(cuda, dtype):
             assert int(held) == int((pool.refs > 0).sum()) and not pool.refs[int(held):].any()
     paging.release(pool, table)
     assert not pool.refs.any()
+
+
+def test_cache_past_32_bits(cuda):
+    """Pages that lie 4 GiB and more into the cache: rotated keys written there, and read as a shared prefix."""
+    import torch
+    from ivonar_amd import attention
+
+    generator = torch.Generator().manual_seed(3)
+    pages = torch.empty((2200, 16, 4, 34 * 256), dtype=torch.uint8, device=cuda)  # 1.2 GB
+    pages = torch.cat((pages, pages, pages, pages))  # 4.9 GB, 557056 bytes a page
+    count = pages.shape[0]
+    assert pages.numel() > 1 << 32
+    last = [count - 1, count - 7, 5, count - 2]  # shared, shared, and of either sequence
+    table = torch.tensor([last[:2] + [last[2]], last[:2] + [last[3]]], dtype=torch.int32, device=cuda)
+    frequencies = attention.rotary_frequencies(256, device=cuda)
+
+    def ints(*values):
+        return torch.tensor(values, dtype=torch.int32, device=cuda)
+
+    q, k, v = (torch.randn(300, n, 256, generator=generator).to(cuda) for n in (16, 16, 16))
+    offsets = ints(0, 290, 290)
+    _, turned = attention.rotate(q[:290], k[:290], ints(0, 256), frequencies, offsets)
+    attention.rotate_write(pages, q[:290], k[:290], v[:290], table, ints(0, 256), frequencies, offsets)
+    _, more = attention.rotate(q[290:], k[290:], ints(256, 256), frequencies, ints(0, 0, 10))
+    attention.rotate_write(pages, q[290:], k[290:], v[290:], table, ints(256, 256), frequencies, ints(0, 0, 10))
+    rows = torch.randn(2, 16, 256, generator=generator).to(cuda)
+    out = attention.prefix_attention(rows, pages, table, ints(290, 266), ints(0, 2), ints(256))
+    for b, (own, value) in enumerate(((turned, v[:290]), (torch.cat((turned[:256], more)), torch.cat((v[:256], v[290:]))))):
+        keys, values = A.stored(own.cpu().numpy()), A.stored(value.cpu().numpy())
+        expected = A.attend(rows[b:b + 1].double().cpu().numpy(), keys, values, len(keys) - 1)
+        A.check(out[b:b + 1].double().cpu().numpy(), *expected, "float32", len(keys) + JOINS, 256, f"sequence {b}")

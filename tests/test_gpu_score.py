@@ -251,3 +251,17 @@ def test_refusals(cuda):
         sampling.log_probabilities(logits[:1, :1].expand(1 << 31, 1), tokens)
     empty = sampling.log_probabilities(logits[:0], tokens[:0], 5)
     assert [tuple(r.shape) for r in empty] == [(0,), (0,), (0, 5), (0, 5)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_past_32_bits(cuda, dtype):
+    """Rows that lie 4 GiB and more apart."""
+    import torch
+    from ivonar_amd import sampling
+
+    vocab, apart = 5003, (1 << 32) // (4 if dtype == "float32" else 2) + 12345
+    flat = torch.empty(2 * apart + vocab, dtype=getattr(torch, dtype), device=cuda)
+    logits = flat.as_strided((3, vocab), (apart, 1))
+    logits.copy_(torch.randn(3, vocab, generator=torch.Generator().manual_seed(1)))
+    tokens = torch.tensor([0, 5002, 77], device=cuda)
+    check(sampling.log_probabilities(logits, tokens, 9), logits.clone(), tokens, 9, 1.0)
