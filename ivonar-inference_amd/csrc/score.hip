@@ -10,7 +10,7 @@
 //
 // The `top` largest logits are found in the same pass.  A logit's key is its value as an ordered number, then its index
 // from the end, so no two keys are alike and ties go to the lowest index; a NaN has the lowest value.  A wave keeps the
-// 64 largest keys that it has met, sorted over its lanes, and a bound below which a key cannot be among the row's top:
+// 64 largest keys that it has met, or 32 where those are enough, sorted over its lanes, and a bound below which a key cannot be among the row's top:
 // the top'th of them, or of the first chunk's per-lane maxima, or what another wave of the row has found.  Most chunks
 // hold no logit above the bound, which their maxima tell.  Keys above it go through a buffer in LDS and are sorted and
 // merged 64 at a time.
@@ -19,9 +19,9 @@
 // split between blocks, whose results a second kernel joins.
 //
 // Bound by the logits' bytes where there are many: 500 rows of 32000 in fp32 14.5 us without alternatives (4.4 TB/s) and
-// 19.2 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth),
-// where vector instructions take three quarters of the SIMDs' cycles.  One row of 32000 takes 5.8 us, and 12.3 with 20:
-// a chain of about seventy compare stages of sorts and merges.
+// 18.7 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth),
+// where vector instructions take three quarters of the SIMDs' cycles.  One row of 32000 takes 5.9 us, and 11.3 with 20:
+// a chain of about fifty compare stages of sorts and merges (with lists of 64 keys, seventy stages, 12.3).
 #include "internal.hpp"
 #include "ternary_device.hpp"
 
@@ -120,9 +120,18 @@ __device__ __forceinline__ int opaque_lane() {
 template <typename V>
 __device__ __forceinline__ V sort_lanes(V v) { return sort_parts<64>(v, opaque_lane()); }
 
-// The 64 largest of a falling list and a rising one, falling.
+// The KEEP largest of a falling list and a rising one, over the first KEEP lanes, falling.
+template <int KEEP>
 __device__ __forceinline__ Key join(Key falling, Key rising) {
-  return merge_lanes<64>(falling > rising ? falling : rising, opaque_lane(), true);
+  return merge_lanes<KEEP>(falling > rising ? falling : rising, opaque_lane(), true);
+}
+// The 32 largest of a falling list and of `count` keys, one a lane.
+__device__ __forceinline__ Key add_keys32(Key list, Key keys, int count) {
+  const int lane = opaque_lane();
+  keys = sort_parts<32>(keys, lane);  // the first half rises, the other falls
+  list = join<32>(list, keys);
+  if (count > 32) list = join<32>(list, __shfl(keys, 63 - lane));
+  return list;
 }
 __device__ __forceinline__ Key lane_key(Key key, int lane) {
   return (Key)(unsigned)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
@@ -195,7 +204,8 @@ __device__ __forceinline__ void finish(const Params& p, int row, const Part& par
   }
 }
 
-template <typename In, bool TOP, int WAVES>
+// TOP: how many keys a list has, 64, 32 or none.
+template <typename In, int TOP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
   constexpr int kVec = 16 / sizeof(In), kVectors = kValues / kVec;
   const ScoreArgs& a = p.a;
@@ -248,7 +258,10 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     Key key = buffer[lane];
     key = lane < count ? key : 0;
-    list = join(list, sort_lanes(key));
+    if constexpr (TOP == 32)
+      list = add_keys32(list, key, count);
+    else
+      list = join<64>(list, sort_lanes(key));
     const Key last = lane_key(list, a.top - 1);
     bound = last > bound ? last : bound;
     if (lane == 0) atomicMax(&bounds[first_wave], bound);
@@ -306,7 +319,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
     sum += part_sum[0] + part_sum[1];
     weighted += part_weighted[0] + part_weighted[1];
 
-    if constexpr (TOP) {
+    if constexpr (TOP > 0) {
       const Key shared = *(volatile Key*)&bounds[first_wave];
       bound = shared > bound ? shared : bound;
       // The lane's logit j in the row, outside the vocabulary where it has none.
@@ -388,6 +401,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
     for (int v = 0; v < kVectors; ++v) current[v] = next[v];
   }
   if (TOP && held > 0) merge(held);
+  if (TOP == 32 && lane >= 32) list = 0;
 
   Part part;
   part.m = all_max(m);
@@ -414,7 +428,17 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
       raise(other_m, other_sum, other_weighted, top, p.scale);
       part.sum += other_sum;
       part.weighted += other_weighted;
-      if (TOP) part.list = join(part.list, buffers[TOP ? first_wave + w : 0][TOP ? 63 - lane : 0]);
+      if constexpr (TOP == 64) part.list = join<64>(part.list, buffers[first_wave + w][63 - lane]);
+    }
+    if constexpr (TOP == 32) {
+      // Of 32 keys two lists at a time, in either half of the lanes, the upper one rising, and then those.
+      auto key_of_wave = [&](int w, int at) { return w < p.row_waves ? buffers[first_wave + w][at] : 0; };
+      const bool low = lane < 32;
+      const Key falling = low ? part.list : key_of_wave(sub + 2 * apart, lane & 31);
+      const Key rising = key_of_wave(low ? sub + apart : sub + 3 * apart, 31 - (lane & 31));
+      const Key two = merge_lanes<32>(falling > rising ? falling : rising, opaque_lane(), low);
+      part.list = join<32>(two, (Key)xor_lane<32>((unsigned)(two >> 32)) << 32 | xor_lane<32>((unsigned)two));
+      if (!low) part.list = 0;
     }
   }
   if (sub != 0) return;
@@ -460,7 +484,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
         lists[k] = reinterpret_cast<const Key*>(from + i * kPartFloats + 4)[63 - lane];
       }
       for (int k = 0; k < kAtOnce && base + k < p.splits; ++k) {
-        part.list = join(part.list, lists[0]);
+        part.list = join<64>(part.list, lists[0]);
 #pragma unroll
         for (int j = 0; j + 1 < kAtOnce; ++j) lists[j] = lists[j + 1];
       }
@@ -472,9 +496,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Params p) {
 // Waves of all rows that keep the device busy, blocks that few long rows are split into, and chunks of a wave that are
 // not split.
 constexpr int kBusyWaves = 4096, kWantedBlocks = 1024, kLeastChunks = 4;
-// Few rows of middling length take a block of sixteen waves each, up to two chunks a wave: top 20 of 1 x 32000 fp32 12.6
-// us and of 32 x 50000 bf16 16.0, with four waves 13.7 and 19.3.  Longer rows are faster in several blocks of four waves
-// (1 x 128256 bf16 20.0 us and 22.3), and more rows than compute units fill the device that way.
+// Few rows of middling length take a block of sixteen waves each, up to two chunks a wave: top 20 of 1 x 32000 fp32 12.3
+// us and of 32 x 50000 bf16 15.8, with four waves 13.7 and 19.3 (lists of 64 keys).  Longer rows are faster in several
+// blocks of four waves (1 x 128256 bf16 20.0 us and 22.3), and more rows than compute units fill the device that way.
 constexpr int kManyRows = 256, kManyLeast = 8, kManyMost = 32;
 
 Params plan(const ScoreArgs& a) {
@@ -491,10 +515,12 @@ Params plan(const ScoreArgs& a) {
 
 template <typename In, int WAVES>
 void run_waves(hipStream_t stream, const Params& p, unsigned blocks) {
-  if (p.a.top > 0)
-    hipLaunchKernelGGL((score_kernel<In, true, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
+  if (p.a.top > 32)
+    hipLaunchKernelGGL((score_kernel<In, 64, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
+  else if (p.a.top > 0)
+    hipLaunchKernelGGL((score_kernel<In, 32, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
   else
-    hipLaunchKernelGGL((score_kernel<In, false, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
+    hipLaunchKernelGGL((score_kernel<In, 0, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, p);
 }
 template <typename In>
 void run(hipStream_t stream, const Params& p, unsigned blocks) {
