@@ -360,7 +360,7 @@ __device__ __forceinline__ void attend_run(const Params& p, const Span& s, int h
   constexpr int NP = NT < 2 ? 2 : NT;  // terms of a weight
   constexpr int kStages = stages(D);
   // While it feeds the matrix cores a wave goes before the others of its SIMD, which take their softmax beside it: 1024
-  // rows over 16000 keys, eight heads of 128, bf16, 118 us instead of 127.
+  // rows over 16000 keys, eight heads of 128, bf16, 118 to 125 us from run to run, 124 to 128 without.
   constexpr bool kRaised = SHARED && !kNarrow;
   const CacheAttentionArgs& a = p.a;
   auto& sums = room.sums;

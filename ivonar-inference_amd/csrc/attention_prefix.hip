@@ -12,7 +12,7 @@
 // of a sequence without tokens, as in a padded batch, see nothing, and its group's prefix is as long without it.
 //
 // The prefix is bound by the instructions that convert keys and values and take the softmax, beside the matrix cores: 256
-// sequences of one row over 16000 tokens, 32/8 heads of 128, bf16: 118 us, 570 TFLOP/s (850 with the second terms of the
+// sequences of one row over 16000 tokens, 32/8 heads of 128, bf16: 122 us, 550 TFLOP/s (820 with the second terms of the
 // weights), vector units busy 60 % of the cycles and matrix units 35 %, which overlap by half at best.  64 rows of a row
 // tile instead of 32, so with half the conversions, leave room for one wave per SIMD: 139 us instead of 128.  The tails
 // are bound by their bytes: 500 tokens each of the same 256 36 us, 3.9 TB/s.  Short calls are two launches' chains of
