@@ -36,6 +36,13 @@ std::map<std::pair<int, uintptr_t>, Scratch> g_stream_scratch;  // node-based: e
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+// Clears a scratch's counters and waits until they are clear: hipMemset returns before that, and nothing orders it before
+// the first launch on a stream that does not wait for the null stream (torch's do not).
+hipError_t clear_counters(unsigned* sync) {
+  const hipError_t status = hipMemset(sync, 0, kSyncAllBytes);
+  return status == hipSuccess ? hipStreamSynchronize(nullptr) : status;
+}
+
 hipError_t allocate_scratch(Scratch& s) {
   if (s.q8 != nullptr) return hipSuccess;
   void* q8 = nullptr;
@@ -48,7 +55,7 @@ hipError_t allocate_scratch(Scratch& s) {
   if (status == hipSuccess) status = hipMalloc(&scale, 256);
   if (status == hipSuccess) status = hipMalloc(&partials, (size_t)kTokenPartialFloats * sizeof(float));
   if (status == hipSuccess) status = hipMalloc(&sync, kSyncAllBytes);
-  if (status == hipSuccess) status = hipMemset(sync, 0, kSyncAllBytes);  // the argmax's block count starts at zero
+  if (status == hipSuccess) status = clear_counters(static_cast<unsigned*>(sync));
   if (status != hipSuccess) {
     if (q8) (void)hipFree(q8);
     if (xsum) (void)hipFree(xsum);
@@ -205,11 +212,11 @@ hipError_t init_device(int device) {
   status = allocate_scratch(g_scratch[device]);
   // The argmax's block count is zero between launches; clearing it here
   // recovers a scratch that overlapping graph replays left set.
-  if (status == hipSuccess) status = hipMemset(g_scratch[device].sync, 0, kSyncAllBytes);
+  if (status == hipSuccess) status = clear_counters(g_scratch[device].sync);
   for (auto it = g_stream_scratch.lower_bound({device, 0}); status == hipSuccess && it != g_stream_scratch.end() &&
                                                              it->first.first == device;
        ++it)
-    status = hipMemset(it->second.sync, 0, kSyncAllBytes);
+    status = clear_counters(it->second.sync);
   if (current != device) (void)hipSetDevice(current);
   return status;
 }
