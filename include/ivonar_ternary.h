@@ -380,6 +380,7 @@ hipError_t ivonar_page_copy(hipStream_t stream, uint8_t* pages, int page_count, 
  * temperature: the log probability of tokens[row] (-inf outside the vocabulary), the entropy in nats, and the `top` (at
  * most 64 and vocab) largest logits' log probabilities and tokens, falling, of equal logits the lowest token first (NaN
  * counts as less than all).  A row of -inf has log probabilities of -inf and entropy 0; one with a NaN or +inf has NaN.
+ * temperature: positive and finite, and so is 4 / temperature.
  * work: ivonar_log_probabilities_work bytes (-1 for sizes that the call refuses), 16-byte aligned. */
 long long ivonar_log_probabilities_work(int dtype, int rows, int vocab, int top);
 hipError_t ivonar_log_probabilities(hipStream_t stream, const void* logits, int dtype, long long row_stride, int rows,

@@ -684,7 +684,7 @@ hipError_t ivonar_log_probabilities(hipStream_t stream, const void* logits, int 
                                     float* entropy, float* top_log_probability, int64_t* top_token, void* work,
                                     long long work_bytes) {
   if (!score_sizes(dtype, rows, vocab, top) || !(temperature > 0.0f) || !isfinite(temperature) ||
-      !isfinite(2.0f / temperature))
+      !isfinite(4.0f / temperature))
     return hipErrorInvalidValue;
   if (rows == 0) return hipSuccess;
   if (logits == nullptr || tokens == nullptr || log_probability == nullptr || entropy == nullptr ||

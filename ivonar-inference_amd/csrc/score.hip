@@ -4,9 +4,10 @@
 //   log p_i = z_i - log S,   H = -sum p_i log p_i = log S - U / S.
 // m, S and U are kept per thread in fp32 and rescaled when a chunk raises m: S' = f S, U' = f (U + d S) for a maximum
 // that rises by -d T, f = e^d.  In units of log 2, z = x c - M with c = log2(e) / T and M = m c rounded to fp32: one
-// rounding of z itself, and since everything is relative to the same M, that of M does not count.  A logit of -inf has no
-// weight; a row of nothing else has log probabilities of -inf and no entropy.  A NaN or +inf makes all of its row's
-// numbers NaN.
+// rounding of z itself, and since everything is relative to the same M, that of M does not count as long as it is half a
+// unit at most, |M| < 2^24.  From there on it would be the largest weight's exponent (2^128 and more from |M| = 2^31 on,
+// as of masked logits or low temperatures), and z = (x - m) c instead.  A logit of -inf has no weight; a row of nothing
+// else has log probabilities of -inf and no entropy.  A NaN or +inf makes all of its row's numbers NaN.
 //
 // The `top` largest logits are found in the same pass.  A logit's key is its value as an ordered number, then its index
 // from the end, so no two keys are alike and ties go to the lowest index; a NaN has the lowest value.  A wave keeps the
@@ -33,7 +34,8 @@ constexpr int kManyWaves = 16;              // of a block where there are few ro
 constexpr int kValues = 32;                 // logits of a lane at a time
 constexpr int kWaveChunk = 64 * kValues;    // and of a wave
 constexpr int kBuffer = 128;                // keys above the bound that a wave holds before it merges 64
-constexpr float kFar = 0x1p100f;            // from here on logits either are the maximum or have no weight beside it
+constexpr float kFar = 0x1p24f;             // |m c| from which on the rounding of it counts
+constexpr float kOverflow = 0x1p100f;       // |x c| below which z is in range
 constexpr int kCrowd = 12;                  // logits of a lane above the first bound that tell of ties
 typedef unsigned long long Key;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -158,14 +160,24 @@ __device__ __forceinline__ float all_sum(float v) {
 // z no further down than where its weight is zero: zero times the result is zero.
 __device__ __forceinline__ float bounded(float z) { return fmaxf(z, -1000.0f); }
 
-// Whether m c may be out of range; not of a maximum of nothing.
-__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
+// M, and none of a maximum of nothing.
 __device__ __forceinline__ float scaled(float m, float scale) { return m == -INFINITY ? 0.0f : m * scale; }
+// What is relative to m has z = (x - m) c where m is far and else z = x c - M.
+__device__ __forceinline__ bool is_far(float m, float scale) { return fabsf(scaled(m, scale)) >= kFar; }
+// (x - m) factor, by halves, whose difference is in range.
+__device__ __forceinline__ float apart(float x, float m, float factor) {
+  return fmaf(0.5f, x, -0.5f * m) * (2.0f * factor);
+}
 
 // S and U moved to the maximum `to`.
 __device__ __forceinline__ void raise(float& m, float& sum, float& weighted, float to, float scale) {
-  const float apart = fabsf(m) >= kFar || fabsf(to) >= kFar ? (m == to ? 0.0f : -1000.0f) : m * scale - to * scale;
-  const float d = bounded(apart);
+  const bool from_far = is_far(m, scale), to_far = is_far(to, scale);
+  float between = m * scale - to * scale;
+  if (from_far || to_far)
+    between = !to_far    ? fmaf(m, scale, -(to * scale))
+              : from_far ? apart(m, to, scale)
+                         : fmaf(-to, scale, m * scale);
+  const float d = bounded(between);
   const float factor = __builtin_amdgcn_exp2f(d);
   weighted = fmaf(sum, d, weighted) * factor;
   sum *= factor;
@@ -177,11 +189,11 @@ __device__ __forceinline__ void finish(const Params& p, int row, const Part& par
   const ScoreArgs& a = p.a;
   const int lane = threadIdx.x & 63;
   const float log_sum = log2f(part.sum);
-  const bool none = part.sum == 0.0f, far = is_far(part.m);
+  const bool none = part.sum == 0.0f, far = is_far(part.m, p.scale);
   auto log_probability = [&](float x) {
     if (none) return -INFINITY;
-    // Far from everything in range, in nats: in units of log 2 they may not be.
-    if (far || fabsf(x) >= kFar) return (x - part.m) * a.inverse_temperature - kLog2 * log_sum;
+    // In nats, which may be in range where units of log 2 are not.
+    if (far || fabsf(x * p.scale) >= kOverflow) return apart(x, part.m, a.inverse_temperature) - kLog2 * log_sum;
     return kLog2 * (fmaf(x, p.scale, -scaled(part.m, p.scale)) - log_sum);
   };
   if (lane == 0) {
@@ -289,7 +301,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
     if (most > m) raise(m, sum, weighted, most, p.scale);
     const float shift = scaled(m, p.scale);
     float part_sum[2] = {}, part_weighted[2] = {};
-    bool slow = __ballot(is_far(m)) != 0ull;
+    const bool far = fabsf(shift) >= kFar;
+    bool slow = __ballot(far) != 0ull;
     if (!slow) {
 #pragma unroll
       for (int j = 0; j < kValues; ++j) {
@@ -304,12 +317,11 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
     }
     if (slow) {
       part_sum[0] = part_sum[1] = part_weighted[0] = part_weighted[1] = 0.0f;
-      const bool far = is_far(m);
       float again = shift;
       asm volatile("" : "+v"(again));  // or the compiler would hold all z from above for here
 #pragma unroll
       for (int j = 0; j < kValues; ++j) {
-        const float z = far ? (x[j] - m) * p.scale : fmaf(x[j], p.scale, -again);
+        const float z = far ? apart(x[j], m, p.scale) : fmaf(x[j], p.scale, -again);
         const float weight = __builtin_amdgcn_exp2f(z);
         part_sum[j & 1] += weight;
         part_weighted[j & 1] = fmaf(bounded(z), weight, part_weighted[j & 1]);
