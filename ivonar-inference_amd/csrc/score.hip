@@ -351,11 +351,12 @@ __global__ __launch_bounds__(WAVES * 64, 4) void score_kernel(Params p) {
         if (last > -INFINITY) bound = ((Key)(ordered(last) - (last == 0.0f ? 1u : 0u)) << 32) - 1;
       }
       unsigned above = 0;  // bit j: logit j may be
-      // Behind the bound's index equal logits are below it.  Without a bound all logits are above it, NaN among them.
+      // Behind the bound's index equal logits are below it.  Without a bound, and where it is that of a NaN, all logits
+      // may be above it.
       auto compare = [&]() {
         const float least = value_of(bound);
         above = 0;
-        if (bound != 0 && start > (int)~(unsigned)bound) {
+        if (bound >> 32 != 0 && start > (int)~(unsigned)bound) {
           if (__ballot(most > least) != 0ull)
 #pragma unroll
             for (int j = kValues - 1; j >= 0; --j) above = above + above + (x[j] > least ? 1u : 0u);
