@@ -348,7 +348,7 @@ hipError_t ivonar_window_attention(hipStream_t stream, const void* q, const void
  *
  * ivonar_page_reserve: sequence b gets a page for every slot that its positions lengths[b] .. lengths[b] + counts[b] - 1
  * are the first to use and that has none, sequence by sequence.  *missing: slots that got none, for want of free pages
- * or of table entries (they stay as they are). */
+ * or of table entries (they stay as they are), at most 2^31 - 1. */
 hipError_t ivonar_page_reserve(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size, int32_t* table,
                                int table_width, const int32_t* lengths, const int32_t* counts, int sequences,
                                int32_t* missing);

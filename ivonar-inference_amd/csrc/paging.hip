@@ -44,6 +44,18 @@ __device__ __forceinline__ int block_scan(int v, int* totals, int& all) {
   return before + sum - v;
 }
 
+// Sum of v over the block, in thread 0.
+__device__ __forceinline__ long long block_sum(long long v, long long* totals) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if ((threadIdx.x & 63) == 0) totals[threadIdx.x >> 6] = v;
+  __syncthreads();
+  long long all = 0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < kBlockWaves; ++w) all += totals[w];
+  return all;
+}
+
 // Word w of the free pages; bits past the last page do not count.
 __device__ __forceinline__ unsigned free_word(const PoolArgs& p, int w) {
   const int left = p.pages - w * 32;
@@ -135,6 +147,7 @@ __global__ __launch_bounds__(kBlock) void reserve_kernel(PoolArgs p, int* table,
                                                          const int* counts, int sequences, int* missing) {
   __shared__ int sums[kBlock];
   __shared__ int totals[kBlockWaves];
+  __shared__ long long totals_outside[kBlockWaves];
   const FreePages f = scan_free(p, sums, totals);
   const int lane = threadIdx.x & 63;
   int given = 0;             // ranks of the sequences before these
@@ -166,10 +179,9 @@ __global__ __launch_bounds__(kBlock) void reserve_kernel(PoolArgs p, int* table,
                   });
     given += all;
   }
-  int outside_all = 0;
-  block_scan((int)min(outside, 1LL << 20), totals, outside_all);  // and everybody has found its pages
+  outside = block_sum(outside, totals_outside);  // and everybody has found its pages
   take_free(p, f, min(given, f.available));
-  if (threadIdx.x == 0) *missing = max(given - f.available, 0) + outside_all;
+  if (threadIdx.x == 0) *missing = (int)min(max(given - f.available, 0) + outside, 0x7fffffffLL);
 }
 
 // One holder of a page less.

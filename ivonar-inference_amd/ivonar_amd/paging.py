@@ -91,7 +91,7 @@ def _table(table: Tensor, page_size: int, what: str) -> tuple[int, int]:
 
 def reserve(pool: PagePool, table: Tensor, lengths: Tensor, counts: Tensor) -> Tensor:
     """Gives sequence b the pages for its positions lengths[b] .. lengths[b] + counts[b] - 1, where they are the first to
-    use a page and the table has none.  Returns how many got none, for want of free pages or of table entries."""
+    use a page and the table has none.  Returns how many got none, for want of free pages or of table entries, at most 2**31 - 1."""
     device = _device(pool.refs, pool.free, table, lengths, counts)
     at = _pool(pool, "reserve")
     sequences, width = _table(table, pool.page_size, "reserve")
