@@ -320,8 +320,9 @@ hipError_t ivonar_cache_attention(hipStream_t stream, const void* q, int dtype, 
 /* ivonar_cache_attention without a window, for sequences that share the pages of a prefix: the same results up to the
  * order of sums, the shared keys read and multiplied once for all rows of a group.  Group g has the sequences groups[g]
  * .. groups[g + 1] - 1 (groups [group_count + 1], not decreasing; sequences outside all groups share nothing), whose
- * tables begin alike: their positions 0 .. prefix[g] - 1 lie in the same pages.  max_prefix: about the longest prefix, a
- * hint as max_length.  work: ivonar_prefix_attention_work bytes, 16-byte aligned. */
+ * tables begin alike: their positions 0 .. prefix[g] - 1 lie in the same pages.  max_prefix: about the longest prefix
+ * (negative: not known), a hint as max_length; a sequence is taken to have at most about max_length - max_prefix keys of its
+ * own.  work: ivonar_prefix_attention_work bytes, 16-byte aligned. */
 long long ivonar_prefix_attention_work(int dtype, int heads, int kv_heads, int head_dim, const int32_t* offsets,
                                        int sequences, int rows, int groups, int max_prefix, int max_length);
 hipError_t ivonar_prefix_attention(hipStream_t stream, const void* q, int dtype, long long q_token_stride,

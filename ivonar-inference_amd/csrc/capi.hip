@@ -764,7 +764,7 @@ static PrefixAttentionArgs prefix_attention_sizes(int dtype, int heads, int kv_h
   PrefixAttentionArgs args{};
   args.a = cache_attention_sizes(dtype, heads, kv_heads, head_dim, offsets, sequences, rows, 0, 0, max_length);
   args.group_count = groups;
-  args.max_prefix = max_prefix > 0 ? max_prefix : 0;
+  args.max_prefix = max_prefix;
   return args;
 }
 

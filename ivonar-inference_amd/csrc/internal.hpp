@@ -339,7 +339,7 @@ struct PrefixAttentionArgs {
   const int* groups;  // [group_count + 1] sequences before each group
   const int* prefix;  // [group_count] tokens in shared pages
   int group_count;
-  int max_prefix;
+  int max_prefix;  // negative: not known
 };
 long long prefix_attention_work(const PrefixAttentionArgs& args);
 hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs& args);

@@ -352,8 +352,10 @@ def prefix_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, g
     groups (int32 [groups + 1], not decreasing): the sequences before each group; those outside all groups share
     nothing.  prefix (int32 [groups]): how many tokens the sequences of each group have in the same pages, from the
     first on (for forks, their parent's finished pages; fewer is right as well).  The result is cache_attention's up to
-    the order of sums.  max_prefix and max_length, about the longest ones, set how keys are shared between blocks
-    (default: what the table can hold); any values give the same result up to that order."""
+    the order of sums.  max_prefix and max_length, about the longest ones, set how keys are shared between blocks; any
+    values give the same result up to that order.  By default a sequence has what the table can hold, any part of it
+    shared; with max_prefix it has about max_length - max_prefix keys of its own, so sequences outside all groups, or of
+    groups with shorter prefixes, that have many more than that do better without it."""
     device = _device(q, pages, table, lengths, groups, prefix, offsets, out)
     count, kv_heads, tiles, dim, sequences, width = _geometry(pages, table, "prefix_attention")
     rows, heads, q_row, q_head = _rows(q, None, dim, "q")
@@ -374,7 +376,7 @@ def prefix_attention(q: Tensor, pages: Tensor, table: Tensor, lengths: Tensor, g
         return out
     capacity = width * tiles * TOKENS_PER_TILE
     longest = capacity if max_length is None else max(1, min(int(max_length), capacity))
-    longest_prefix = longest if max_prefix is None else max(0, min(int(max_prefix), capacity))
+    longest_prefix = -1 if max_prefix is None else max(0, min(int(max_prefix), capacity))
     dtype = _DTYPES[q.dtype]
     need = _prefix_workspace(dtype, heads, kv_heads, dim, offsets is not None, sequences, rows, group_count,
                              longest_prefix, longest)

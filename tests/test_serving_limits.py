@@ -19,3 +19,17 @@ def test_temperatures_whose_inverse_is_out_of_range():
         assert call(temperature) == INVALID
     if not torch.cuda.is_available():
         assert call(1.2e-38) != INVALID  # past the checks, and finds no device
+
+
+def test_tails_are_shared_out_where_no_prefix_is_known():
+    """A split tail needs room for its parts, beside the prefix's; a tail of a few tiles needs none."""
+    work = library().ivonar_prefix_attention_work
+    sizes = (2, 32, 8, 128, None, 8, 8, 1)  # eight rows, one group
+    whole, part = 8 * 8 * (128 + 2) * 4, 16  # of a row tile of each head; the groups' shared tokens
+    for longest in (2000, 20000, 130000):
+        assert work(*sizes, longest - 21, longest) < work(*sizes, -1, longest)
+        prefix = work(*sizes, longest, longest)  # tails of nothing
+        tails = work(*sizes, 0, longest) - work(*sizes, 0, 0)  # of all keys
+        assert tails > 0 and tails % (8 * whole) == 0
+        assert work(*sizes, -1, longest) == prefix + tails
+        assert (prefix - part) % whole == 0
