@@ -361,7 +361,8 @@ hipError_t ivonar_page_release(hipStream_t stream, int32_t* refs, int32_t* free,
  * outside 0 .. sequences - 1: an empty row).  The first row of a parent takes its whole row over.  Further ones share
  * its finished pages, and a page that is not full is copied, for the first row too where refs counts another entry:
  * copies [rows, 2] lists (source, target), then -1, for ivonar_page_copy.  *missing: rows for whose copy there was no page; they end with their last finished page.  Pages that
- * no row holds any more are free after the call, not for it.  At most 8192 sequences. */
+ * no row holds any more are free after the call, not for it.  The results may not overlap what is read.  At most 8192
+ * sequences. */
 hipError_t ivonar_page_fork(hipStream_t stream, int32_t* refs, int32_t* free, int pages, int page_size,
                             const int32_t* table, int table_width, const int32_t* lengths, int sequences,
                             const int32_t* parents, int rows, int32_t* out_table, int32_t* out_lengths, int32_t* copies,

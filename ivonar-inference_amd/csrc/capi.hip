@@ -641,7 +641,7 @@ hipError_t ivonar_page_fork(hipStream_t stream, int32_t* refs, int32_t* free, in
       (lengths == nullptr && sequences > 0))
     return hipErrorInvalidValue;
   if (rows > 0 && (parents == nullptr || out_table == nullptr || out_lengths == nullptr || copies == nullptr ||
-                   out_table == table || out_lengths == lengths))
+                   out_table == table || out_lengths == lengths || out_lengths == parents))
     return hipErrorInvalidValue;
   return launch_page_fork(stream, pool, ForkArgs{table, lengths, parents, out_table, out_lengths, copies, missing,
                                                  table_width, sequences, rows});

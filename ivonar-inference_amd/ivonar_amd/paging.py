@@ -128,7 +128,7 @@ def fork(pool: PagePool, table: Tensor, lengths: Tensor, parents: Tensor,
     `table` has that page, as after tokens were dropped from a fork.  `table` and `lengths` are used up: rows without a
     child give their pages back.  The copies' pages come from those free before the call; a row that gets none ends with its
     last finished page.  Call copy() with the result's copies for every cache before the next write.
-    out: a table [rows, width] and lengths [rows] to write the results into, other ones than those given."""
+    out: a table [rows, width] and lengths [rows] to write the results into, other tensors than those given."""
     device = _device(pool.refs, pool.free, table, lengths, parents, *(out or ()))
     at = _pool(pool, "fork")
     sequences, width = _table(table, pool.page_size, "fork")
@@ -145,8 +145,8 @@ def fork(pool: PagePool, table: Tensor, lengths: Tensor, parents: Tensor,
         if _table(out[0], pool.page_size, "fork") != (rows, width):
             raise KernelError(f"out must be a table [{rows}, {width}] and lengths [{rows}]")
         _index(out[1], rows, "the lengths of out")
-        if rows and (_overlap(out[0], table) or _overlap(out[1], lengths)):
-            raise KernelError("fork cannot write into the table or lengths that it reads")
+        if rows and (any(_overlap(to, given) for to in out for given in (table, lengths, parents)) or _overlap(*out)):
+            raise KernelError("fork cannot write into the table, lengths or parents that it reads, nor both results alike")
     copies, missing = table.new_empty((rows, 2)), table.new_empty(1)
     _run("ivonar_page_fork", device, *at, table.data_ptr(), width, lengths.data_ptr(), sequences, parents.data_ptr(),
          rows, out[0].data_ptr(), out[1].data_ptr(), copies.data_ptr(), missing.data_ptr())

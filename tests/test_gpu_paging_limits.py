@@ -24,3 +24,20 @@ def test_slots_far_past_the_table(cuda, sequences, width, page, free):
         missing = paging.reserve(pool, table, *ints)
         assert int(missing) == min(sequences * slots - given, 2 ** 31 - 1)
         assert int((table >= 0).sum()) == int(pool.refs.sum()) == given
+
+
+def test_fork_into_what_it_reads(cuda):
+    """Results that lie, in part, in the table, the lengths, the parents or each other are refused."""
+    import torch
+    from ivonar_amd import paging
+    from ivonar_amd.runtime import KernelError
+
+    pool = paging.page_pool(40, 64, cuda)
+    ints = torch.full((60,), -1, dtype=torch.int32, device=cuda)
+    table, lengths, parents, other = ints[:6].view(2, 3), ints[8:10].zero_(), ints[12:14].zero_(), ints[20:]
+    apart = other[:6].view(2, 3), other[6:8]
+    paging.fork(pool, table.clone(), lengths.clone(), parents, out=apart)
+    for out in ((table, apart[1]), (apart[0], lengths), (apart[0], parents), (apart[0], ints[5:7]), (ints[9:15].view(2, 3), apart[1]),
+                (ints[3:9].view(2, 3), apart[1]), (apart[0], other[5:7]), (apart[0], ints[13:15])):
+        with pytest.raises(KernelError):
+            paging.fork(pool, table, lengths, parents, out=out)

@@ -33,3 +33,13 @@ def test_tails_are_shared_out_where_no_prefix_is_known():
         assert tails > 0 and tails % (8 * whole) == 0
         assert work(*sizes, -1, longest) == prefix + tails
         assert (prefix - part) % whole == 0
+
+
+def test_fork_writes_into_none_of_its_inputs():
+    good = [P, P, 40, 64, P, 4, P, 2, 2 * P, 3, 3 * P, 4 * P, P, P]
+    for at, value in ((10, P), (11, P), (11, 2 * P)):  # the table, the lengths, the parents
+        args = list(good)
+        args[at] = value
+        assert library().ivonar_page_fork(None, *args) == INVALID
+    if not torch.cuda.is_available():
+        assert library().ivonar_page_fork(None, *good) != INVALID
