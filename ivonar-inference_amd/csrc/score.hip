@@ -20,8 +20,9 @@
 // split between blocks, whose results a second kernel joins.
 //
 // Bound by the logits' bytes where there are many: 500 rows of 32000 in fp32 14.5 us without alternatives (4.4 TB/s) and
-// 18.7 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth),
-// where vector instructions take three quarters of the SIMDs' cycles.  One row of 32000 takes 5.9 us, and 11.3 with 20:
+// 18.8 with 5; 2048 rows of 100003 in bf16 95 us with 20 (4.3 TB/s; their rows start anywhere, which costs a tenth),
+// where vector instructions take three quarters of the SIMDs' cycles, and as many more where most logits are masked by
+// -1e9 (95 us for 87 with masks of -1e4).  One row of 32000 takes 5.8 us, and 11.3 with 20:
 // a chain of about fifty compare stages of sorts and merges (with lists of 64 keys, seventy stages, 12.3).
 #include "internal.hpp"
 #include "ternary_device.hpp"

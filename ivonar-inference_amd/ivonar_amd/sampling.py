@@ -120,7 +120,8 @@ def log_probabilities(logits: Tensor, tokens: Tensor, top: int = 0, temperature:
     A token outside the vocabulary has the log probability -inf.  `top` (at most 64) alternatives are listed, of equal
     logits the lowest token first; a NaN counts as less than every number.  A row whose logits are all -inf has log
     probabilities of -inf and the entropy 0; a row with a NaN or +inf has NaN for all of its numbers, but for a token
-    outside the vocabulary.  Nothing synchronises, and calls can be captured into a graph."""
+    outside the vocabulary.  The fp32 results are parts of one tensor, which each of them keeps alive.  Nothing
+    synchronises, and calls can be captured into a graph."""
     device = _device(logits, tokens)
     dtype = _DTYPES.get(logits.dtype)
     if logits.dim() != 2 or dtype is None or not 0 < logits.shape[1] <= 1 << 30:
